@@ -151,6 +151,7 @@ def prepare(case, seed):
             s["dlogprob"] = -torch.rand(rows, generator=g, device=DEVICE) - 0.5
             s["dentropy"] = normal(rows, scale=0.01)
             s["dlog_norm"] = normal(rows, scale=0.001)
+            s["stats"] = torch.empty(rows, 2, device=DEVICE)
     elif op in ("rotary", "qknorm"):
         b, t = case["batch"], case["time"]
         start = torch.randint(0, case["far"] + 1, (b, 1), generator=g, device=DEVICE)
@@ -199,7 +200,7 @@ def _handles(s):
         h = {"x": wrap(s["x"], s.get("dx")), "token": wrap(s["token"])}
         for name in ("logprob", "entropy", "log_norm"):
             h[name] = wrap(s[name], s.get("d" + name))
-        for name in ("top_logprob", "top_index"):
+        for name in ("stats", "top_logprob", "top_index"):
             h[name] = wrap(s[name]) if name in s else None
         return h
     if op in ("rotary", "qknorm"):
@@ -241,10 +242,10 @@ def _logprob_own(s):
     import plast_b200 as pb
     c, h = s["case"], s["handles"]
     pb.token_logprob(h["x"], h["token"], h["logprob"], entropy=h["entropy"], log_norm=h["log_norm"],
-                     top_logprob=h["top_logprob"], top_index=h["top_index"], temperature=c["temperature"])
+                     stats=h["stats"], top_logprob=h["top_logprob"], top_index=h["top_index"], temperature=c["temperature"])
     if c["train"]:
-        pb.token_logprob_backward(h["x"], h["token"], h["logprob"], entropy=h["entropy"], log_norm=h["log_norm"],
-                                  temperature=c["temperature"])
+        pb.token_logprob_backward(h["x"], h["token"], h["stats"], h["logprob"], entropy=h["entropy"],
+                                  log_norm=h["log_norm"], temperature=c["temperature"])
     return _results(s, "logprob", "entropy", "log_norm", "top_logprob", "top_index", "dx")
 
 
