@@ -169,6 +169,34 @@ void log_softmax_cuda_backward(Tensor **inputs, const Tensor *output, KernelPara
  * into a host-side one-hot matrix; here the label indexes the row directly. */
 void cross_entropy_cuda_forward(const Tensor **inputs, Tensor *output, KernelParams params);
 void cross_entropy_cuda_backward(Tensor **inputs, const Tensor *output, KernelParams params);
+/* token_logprob: for every row of logits [..., C] (FLOAT32, any strides) the log probability of one
+ * given token at a temperature, in one pass over the logits. With z = logits / temperature:
+ *   log_norm = log sum_j exp(z_j)       logprob = z[token] - log_norm
+ *   entropy  = -sum_j p_j log p_j       p_j = exp(z_j - log_norm)
+ *   top_*    the k = top_index->shape[last] largest logits in descending order, of equal ones the
+ *            lower index first: their log probabilities and indices.
+ *   stats    what backward needs: the row's largest logit m and sum_j exp((x_j - m) / temperature)
+ * tokens: INT32, the logits' shape without the last dim (any strides). logprob, entropy, log_norm:
+ * FLOAT32, contiguous, one element per row; stats: FLOAT32, contiguous, two elements per row, aligned
+ * to 8 bytes; top_logprob (FLOAT32) and top_index (INT32): contiguous, k elements per row,
+ * k <= PLAST_TOKEN_TOP_MAX and <= C. All but logprob may be NULL (top_* together). temperature is in
+ * [1e-30, 1e30].
+ * A token outside [0, C) marks a row of padding: logprob 0 and no gradient through it (as
+ * cross_entropy treats such a label); its entropy and the rest are computed. A logit of -inf is a
+ * masked token: probability 0. A row without any other logit has log_norm and every log probability
+ * -inf, entropy 0 and no gradient. A NaN or +inf logit makes its row's results NaN; a NaN is never an
+ * alternative, places that remain hold index -1 and NaN.
+ * Backward: logits->grad += d/dlogits of the upstream gradients in logprob->grad, entropy->grad and
+ * log_norm->grad (each contiguous; a tensor or a gradient that is NULL counts as zero). stats, and
+ * entropy where its gradient is given, hold the forward's results for the same logits and
+ * temperature. The alternatives are reported only: nothing flows through top_logprob. */
+#define PLAST_TOKEN_TOP_MAX 32
+void plast_b200_token_logprob(const Tensor *logits, const Tensor *tokens, Tensor *logprob, Tensor *entropy,
+                              Tensor *log_norm, Tensor *stats, Tensor *top_logprob, Tensor *top_index,
+                              float temperature);
+void plast_b200_token_logprob_backward(Tensor *logits, const Tensor *tokens, const Tensor *stats,
+                                       const Tensor *logprob, const Tensor *entropy, const Tensor *log_norm,
+                                       float temperature);
 /* sigmoid: plast/nn/functional.py:42-47 (neg -> exp -> +1 -> 1/.). inputs = {x}. */
 void sigmoid_cuda_forward(const Tensor **inputs, Tensor *output, KernelParams params);
 void sigmoid_cuda_backward(Tensor **inputs, const Tensor *output, KernelParams params);

@@ -59,6 +59,22 @@ class ChainStep(C.Structure):
     _fields_ = [("opcode", C.c_int32), ("a", C.c_int32), ("b", C.c_int32), ("fval", C.c_float)]
 
 
+class QkNormParams(C.Structure):
+    """PlastQkNormParams of include/plast_b200_rotary.h"""
+
+    _fields_ = [("epsilon", C.c_float), ("amplitude", C.c_float), ("layout", C.c_int)]
+
+
+class RotaryScaling(C.Structure):
+    """PlastRotaryScaling of include/plast_b200_rotary.h"""
+
+    _fields_ = [("kind", C.c_int), ("factor", C.c_float), ("slow", C.c_float), ("fast", C.c_float),
+                ("context", C.c_uint64)]
+
+
+ROTARY_HALVES, ROTARY_INTERLEAVED = 0, 1       # how a head's elements pair up (params.dim of the rotary op)
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "parts": 3, "bands": 4}
+
 CHAIN_OPCODES = {
     "add": 0, "sub": 1, "mul": 2, "div": 3, "neg": 4, "abs": 5, "exp": 6, "log": 7, "sin": 8,
     "cos": 9, "tan": 10, "leaky_relu": 11, "add_scalar": 12, "rsub_scalar": 13, "mul_scalar": 14,
@@ -70,7 +86,7 @@ ERROR_NAMES = {0: "OK", 1: "DTYPE", 2: "SHAPE", 3: "NULL", 4: "CUDA", 5: "UNSUPP
 FORWARD_OPS = [
     "add", "sub", "mul", "div", "abs", "cos", "sin", "tan", "exp", "log", "neg", "leaky_relu",
     "sum", "mean", "max", "min", "argmax", "softmax", "log_softmax", "cross_entropy", "sigmoid",
-    "scale_bias_leaky_relu", "add_leaky_relu",
+    "scale_bias_leaky_relu", "add_leaky_relu", "rotary",
 ]
 BACKWARD_OPS = [op for op in FORWARD_OPS if op != "argmax"]
 
@@ -102,6 +118,8 @@ def declared_symbols() -> list[str]:
         "plast_b200_peer_group_status", "plast_b200_peer_group_clear_status", "plast_b200_peer_group_release",
         "plast_b200_peer_group_local", "plast_b200_chain_jit_available", "plast_b200_peer_full_reduce", "plast_b200_peer_cross_entropy_mean",
         "plast_b200_peer_reduce_begin", "plast_b200_peer_reduce_end",
+        "plast_b200_token_logprob", "plast_b200_token_logprob_backward",
+        "plast_b200_rotary_frequencies", "plast_b200_qk_norm_rotary", "plast_b200_qk_norm_rotary_backward",
     ]
     return syms
 
@@ -133,6 +151,16 @@ def _load() -> C.CDLL:
     lib.plast_b200_chain_forward_host.restype = None
     lib.plast_b200_add_leaky_relu_row_sum.argtypes = [C.POINTER(CTensor)] * 4 + [C.c_float]
     lib.plast_b200_add_leaky_relu_row_sum.restype = None
+    lib.plast_b200_token_logprob.argtypes = [C.POINTER(CTensor)] * 8 + [C.c_float]
+    lib.plast_b200_token_logprob_backward.argtypes = [C.POINTER(CTensor)] * 6 + [C.c_float]
+    lib.plast_b200_qk_norm_rotary.argtypes = [C.POINTER(CTensor)] * 8 + [QkNormParams]
+    lib.plast_b200_qk_norm_rotary_backward.argtypes = [C.POINTER(CTensor)] * 8 + [QkNormParams]
+    lib.plast_b200_rotary_frequencies.argtypes = [C.POINTER(RotaryScaling), C.c_uint64, C.c_float, C.POINTER(C.c_float),
+                                                  C.POINTER(C.c_float)]
+    lib.plast_b200_rotary_frequencies.restype = C.c_int
+    for name in ("plast_b200_token_logprob", "plast_b200_token_logprob_backward", "plast_b200_qk_norm_rotary",
+                 "plast_b200_qk_norm_rotary_backward"):
+        getattr(lib, name).restype = None
     lib.plast_b200_relu_grad_modulate.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_float]
     lib.plast_b200_bias_grad_reduce.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64]
     lib.plast_b200_bias_grad_masked.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_float]
@@ -278,6 +306,13 @@ class Tensor:
         self.c.requires_grad = True
         return g
 
+    def set_grad(self, grad: "Tensor"):
+        """Makes `grad` (a Tensor over memory of its own or somebody else's) this tensor's gradient."""
+        self.grad = grad
+        self.c.grad = C.pointer(grad.c)
+        self.c.requires_grad = True
+        return grad
+
     def view(self, shape, strides, offset: int = 0) -> "Tensor":
         """Metadata-only view sharing this tensor's memory (what plast's shape ops produce,
         src/kernels/cpu/shape_ops.c:28-80); `offset` elements into it (a slice: the view's data
@@ -377,6 +412,65 @@ def backward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fv
     """``<op>_cuda_backward(inputs, output, params)``: accumulates into inputs[i].grad."""
     getattr(lib, f"{op}_cuda_backward")(_ptr_array(inputs), C.byref(output.c),
                                         KernelParams(dim, keepdim, fval))
+    if check:
+        check_error()
+
+
+def _ref(t):
+    return None if t is None else C.byref(t.c)
+
+
+def token_logprob(logits, tokens, logprob, entropy=None, log_norm=None, stats=None, top_logprob=None, top_index=None,
+                  temperature: float = 1.0, check: bool = True):
+    """Log probability of one given token per row of logits [..., C], with the distribution's entropy and log
+    normaliser, the statistics that the backward needs ([..., 2]) and the k = top_index.shape[-1] best
+    alternatives; optional outputs may be None."""
+    lib.plast_b200_token_logprob(_ref(logits), _ref(tokens), _ref(logprob), _ref(entropy), _ref(log_norm), _ref(stats),
+                                 _ref(top_logprob), _ref(top_index), temperature)
+    if check:
+        check_error()
+    return logprob
+
+
+def token_logprob_backward(logits, tokens, stats, logprob=None, entropy=None, log_norm=None, temperature: float = 1.0,
+                           check: bool = True):
+    """logits.grad += the gradient of the upstream gradients in logprob.grad, entropy.grad and log_norm.grad."""
+    lib.plast_b200_token_logprob_backward(_ref(logits), _ref(tokens), _ref(stats), _ref(logprob), _ref(entropy),
+                                          _ref(log_norm), temperature)
+    if check:
+        check_error()
+
+
+def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                       slow: float = 1.0, fast: float = 32.0, context: int = 0):
+    """(frequencies, amplitude): the table of the rotary ops for a head's first `rotated` elements, as a float32
+    array of rotated / 2 angles per position, and the amplitude that goes with it. `scaling` is one of
+    ROTARY_SCALINGS; see include/plast_b200_rotary.h."""
+    table, amplitude = np.empty(max(int(rotated) // 2, 1), dtype=np.float32), C.c_float(1.0)
+    sc = RotaryScaling(ROTARY_SCALINGS[scaling], factor, slow, fast, context)
+    lib.plast_b200_rotary_frequencies(C.byref(sc), rotated, base, table.ctypes.data_as(C.POINTER(C.c_float)),
+                                      C.byref(amplitude))
+    check_error()
+    return table, amplitude.value
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, epsilon: float = 1e-6,
+                   layout: int = ROTARY_HALVES, amplitude: float = 1.0, check: bool = True):
+    """Root-mean-square norm of every query and key head, its weight and the rotation, in one launch. k, k_weight
+    and k_out may be None together, a weight alone too."""
+    lib.plast_b200_qk_norm_rotary(_ref(q), _ref(k), _ref(q_weight), _ref(k_weight), _ref(positions), _ref(inv_freq),
+                                  _ref(q_out), _ref(k_out), QkNormParams(epsilon, amplitude, layout))
+    if check:
+        check_error()
+    return q_out, k_out
+
+
+def qk_norm_rotary_backward(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, epsilon: float = 1e-6,
+                            layout: int = ROTARY_HALVES, amplitude: float = 1.0, check: bool = True):
+    """Adds to q.grad, k.grad and the weights' gradients, reading q_out.grad and k_out.grad."""
+    lib.plast_b200_qk_norm_rotary_backward(_ref(q), _ref(k), _ref(q_weight), _ref(k_weight), _ref(positions),
+                                           _ref(inv_freq), _ref(q_out), _ref(k_out),
+                                           QkNormParams(epsilon, amplitude, layout))
     if check:
         check_error()
 

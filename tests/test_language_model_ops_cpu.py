@@ -1,0 +1,175 @@
+"""What token_logprob, rotary and qk_norm_rotary refuse, and the host-side frequency tables: no GPU needed, a
+refused call launches nothing."""
+import numpy as np
+import pytest
+
+import plast_b200 as pb
+
+F, I = pb.FLOAT32, pb.INT32
+
+
+def T(*shape, dtype=F, **kw):
+    return pb.Tensor(shape, device="cpu", dtype=dtype, **kw)
+
+
+def refused(code, fn, *args, **kw):
+    with pytest.raises(pb.PlastError) as e:
+        fn(*args, **kw)
+    assert pb.ERROR_NAMES[e.value.code] == code, str(e.value)
+
+
+def expanded(t, shape, strides):
+    return t.view(shape, strides)
+
+
+def test_token_logprob_refusals():
+    x, tok, row = T(4, 10), T(4, dtype=I), T(4)
+    f = pb.token_logprob
+    refused("NULL", f, None, tok, row)
+    refused("NULL", f, x, None, row)
+    refused("NULL", f, x, tok, None)
+    refused("DTYPE", f, T(4, 10, dtype=I), tok, row)
+    refused("DTYPE", f, x, T(4), row)
+    refused("DTYPE", f, x, tok, T(4, dtype=I))
+    refused("SHAPE", f, x, T(3, dtype=I), row)
+    refused("SHAPE", f, x, T(2, 2, dtype=I), row)
+    refused("SHAPE", f, T(4, 0), tok, row)
+    refused("SHAPE", f, T(), T(dtype=I), T(1))
+    refused("SHAPE", f, x, tok, T(5))
+    refused("SHAPE", f, x, tok, row, entropy=T(3))
+    refused("UNSUPPORTED", f, x, tok, T(8).view((4,), (2,)))
+    refused("SHAPE", f, x, tok, row, stats=T(4))
+    for bad in (0.0, -1.0, float("nan"), float("inf"), 1e-38):
+        refused("UNSUPPORTED", f, x, tok, row, temperature=bad)
+    refused("NULL", f, x, tok, row, top_logprob=T(4, 3))
+    refused("NULL", f, x, tok, row, top_index=T(4, 3, dtype=I))
+    refused("SHAPE", f, x, tok, row, top_logprob=T(4, 11), top_index=T(4, 11, dtype=I))
+    refused("SHAPE", f, x, tok, row, top_logprob=T(4, 3), top_index=T(3, 3, dtype=I))
+    refused("DTYPE", f, x, tok, row, top_logprob=T(4, 3), top_index=T(4, 3))
+    refused("LIMIT", f, T(4, 50), tok, row, top_logprob=T(4, 33), top_index=T(4, 33, dtype=I))
+    big = T(1).view((1 << 28, 2), (0, 0))
+    refused("LIMIT", f, big, T(1, dtype=I).view((1 << 28,), (0,)), row)
+
+
+def test_token_logprob_backward_refusals():
+    b = pb.token_logprob_backward
+    tok, st, row, H, L = T(4, dtype=I), T(4, 2), T(4), T(4), T(4)
+    x = T(4, 10)
+    b(x, tok, st, row, H, L)                             # no gradient wanted: nothing to do
+    x = T(4, 10, requires_grad=True)
+    refused("NULL", b, x, tok, None, row, H, L)
+    refused("SHAPE", b, x, tok, T(4), row, H, L)
+    refused("UNSUPPORTED", b, x, tok, T(10).view((4, 2), (2, 1), offset=1), row, H, L)
+    lp = T(4)
+    lp.set_grad(T(3))
+    refused("SHAPE", b, x, tok, st, lp, H, L)
+    ent = T(4, requires_grad=True)
+    ent.c.data = None
+    refused("NULL", b, x, tok, st, row, ent, L)
+    x.set_grad(T(4, 9))
+    refused("SHAPE", b, x, tok, st, row, H, L)
+    x.set_grad(T(4, 10, dtype=I))
+    refused("DTYPE", b, x, tok, st, row, H, L)
+    x.set_grad(T(10).view((4, 10), (0, 1)))              # an expanded gradient
+    refused("UNSUPPORTED", b, x, tok, st, row, H, L)
+    x.c.grad = None
+    refused("NULL", b, x, tok, st, row, H, L)
+
+
+def test_rotary_refusals():
+    x, pos, freq, out = T(2, 3, 4, 16), T(2, 3, 1, dtype=I), T(8), T(2, 3, 4, 16)
+
+    def f(x=x, pos=pos, freq=freq, out=out, dim=0, fval=1.0):
+        pb.forward("rotary", [x, pos, freq], out, dim=dim, fval=fval)
+
+    refused("DTYPE", f, x=T(2, 3, 4, 16, dtype=I))
+    refused("DTYPE", f, pos=T(2, 3, 1))
+    refused("DTYPE", f, freq=T(8, dtype=I))
+    refused("SHAPE", f, pos=T(2, 5, 1, dtype=I))
+    refused("SHAPE", f, pos=T(2, 3, 4, 16, dtype=I))
+    refused("SHAPE", f, freq=T(9))
+    refused("SHAPE", f, freq=T(0))
+    refused("SHAPE", f, freq=T(2, 4))
+    refused("SHAPE", f, out=T(2, 3, 4, 8))
+    refused("SHAPE", f, x=T(), out=T())
+    refused("LIMIT", f, x=T(2, 1, 1, 1025), pos=T(2, 1, 1, dtype=I), out=T(2, 1, 1, 1025))
+    refused("UNSUPPORTED", f, dim=2)
+    for bad in (0.0, -1.0, float("nan"), float("inf")):
+        refused("UNSUPPORTED", f, fval=bad)
+    refused("UNSUPPORTED", f, out=T(16).view((2, 3, 4, 16), (0, 0, 0, 1)))
+    refused("UNSUPPORTED", f, out=x.view((2, 3, 4, 16), (12 * 16, 16, 48, 1)))   # in place with other strides
+    refused("UNSUPPORTED", f, freq=T(8, requires_grad=True))
+    wide = T(1).view((1 << 16, 1 << 15, 2), (0, 0, 0))
+    refused("LIMIT", f, x=wide, pos=T(1, 1, dtype=I), freq=T(1), out=T(1).view((1 << 16, 1 << 15, 2), (2 << 15, 2, 1)))
+    x.set_grad(T(2, 3, 4, 16))
+    with pytest.raises(pb.PlastError):                                           # no upstream gradient
+        pb.backward("rotary", [x, pos, freq], out, fval=1.0)
+    x.set_grad(T(16).view((2, 3, 4, 16), (0, 0, 0, 1)))
+    out.attach_grad()
+    refused("UNSUPPORTED", pb.backward, "rotary", [x, pos, freq], out, fval=1.0)
+
+
+def test_qk_norm_refusals():
+    base = dict(q=T(2, 3, 4, 16), k=T(2, 3, 2, 16), qw=T(16), kw=T(16), pos=T(2, 3, 1, dtype=I), freq=T(8),
+                qo=T(2, 3, 4, 16), ko=T(2, 3, 2, 16))
+
+    def f(call=pb.qk_norm_rotary, epsilon=1e-6, layout=0, amplitude=1.0, **kw):
+        a = {**base, **kw}
+        call(*[a[n] for n in ("q", "k", "qw", "kw", "pos", "freq", "qo", "ko")], epsilon=epsilon, layout=layout,
+           amplitude=amplitude)
+
+    refused("NULL", f, q=None)
+    refused("NULL", f, qo=None)
+    refused("NULL", f, k=None)
+    refused("NULL", f, k=None, kw=None)
+    refused("DTYPE", f, k=T(2, 3, 2, 16, dtype=I))
+    refused("SHAPE", f, k=T(2, 3, 2, 8))
+    refused("SHAPE", f, ko=T(2, 3, 4, 16))
+    refused("SHAPE", f, qw=T(8))
+    refused("SHAPE", f, kw=T(2, 16))
+    refused("SHAPE", f, k=T(2, 4, 2, 16), ko=T(2, 4, 2, 16))           # positions do not fit the keys
+    refused("UNSUPPORTED", f, epsilon=-1.0)
+    refused("UNSUPPORTED", f, epsilon=float("nan"))
+    refused("UNSUPPORTED", f, layout=3)
+    refused("UNSUPPORTED", f, layout=-1)
+    refused("UNSUPPORTED", f, amplitude=0.0)
+    same = T(2, 3, 4, 16)
+    refused("UNSUPPORTED", f, k=T(2, 3, 4, 16), qo=same, ko=same)
+    back = pb.qk_norm_rotary_backward
+    f(call=back)                                                          # no gradient wanted
+    refused("NULL", f, call=back, qw=T(16, requires_grad=True))         # no upstream gradient
+    refused("NULL", f, call=back, q=T(2, 3, 4, 16, requires_grad=True))
+    g = T(2, 3, 4, 16)
+    q, k = T(2, 3, 4, 16), T(2, 3, 4, 16)
+    q.set_grad(g)
+    k.set_grad(g)
+    refused("UNSUPPORTED", f, call=back, q=q, k=k, qo=T(2, 3, 4, 16, requires_grad=True), ko=T(2, 3, 4, 16, requires_grad=True))
+
+
+def test_frequency_tables():
+    n, base = 64, 10000.0
+    i = np.arange(n)
+    plain = base ** (-2.0 * i / 128)
+    table, amplitude = pb.rotary_frequencies(128, base)
+    np.testing.assert_allclose(table, plain, rtol=2.0 ** -24)
+    assert amplitude == 1.0
+    np.testing.assert_allclose(pb.rotary_frequencies(128, base, "linear", factor=4.0)[0], plain / 4, rtol=2.0 ** -23)
+    slow, _ = pb.rotary_frequencies(128, base, "base", factor=8.0)
+    np.testing.assert_allclose([slow[0], slow[-1]], [1.0, plain[-1] / 8], rtol=1e-6)
+    parts, amplitude = pb.rotary_frequencies(128, base, "parts", factor=16.0, slow=1, fast=32, context=4096)
+    turns = 4096 * plain / (2 * np.pi)
+    assert np.allclose(parts[turns > 40], plain[turns > 40], rtol=1e-6)
+    assert np.allclose(parts[turns < 0.8], plain[turns < 0.8] / 16, rtol=1e-6)
+    assert ((parts <= plain * 1.000001) & (parts >= plain / 16 * 0.999999)).all()
+    assert (np.diff(parts) < 0).all()
+    np.testing.assert_allclose(amplitude, 0.1 * np.log(16.0) + 1.0, rtol=2.0 ** -24)
+    bands, _ = pb.rotary_frequencies(128, base, "bands", factor=8.0, slow=1, fast=4, context=8192)
+    turns = 8192 * plain / (2 * np.pi)
+    keep = np.clip((turns - 1) / 3, 0, 1)
+    np.testing.assert_allclose(bands, plain * keep + plain / 8 * (1 - keep), rtol=2.0 ** -23)
+    for bad in (dict(rotated=3), dict(rotated=0), dict(rotated=2048)):
+        refused("SHAPE", pb.rotary_frequencies, base=base, **bad)
+    for bad in (dict(base=1.0), dict(base=float("inf")), dict(scaling="linear", factor=0.5),
+                dict(scaling="parts", factor=2.0, slow=32, fast=1, context=4096),
+                dict(scaling="bands", factor=2.0, slow=1, fast=4, context=0), dict(scaling="base", factor=2.0, rotated=2)):
+        refused("UNSUPPORTED", pb.rotary_frequencies, **{"rotated": 8, "base": base, **bad})
