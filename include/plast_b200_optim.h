@@ -85,6 +85,42 @@ void adamw_step_cuda(AdamW *optimizer, Tensor **parameters, int num_parameters);
  * reference releases its arenas as a whole. */
 void plast_b200_adam_state_release(Tensor **m, Tensor **v);
 
+/* Muon: momentum whose update is orthogonalised, for weight matrices (biases, norms and embeddings
+ * take one of the optimisers above). No counterpart in the reference. */
+#define PLAST_MUON_SCALE_ASPECT 0 /* s = sqrt(max(1, rows / cols)) */
+#define PLAST_MUON_SCALE_RMS 1    /* s = 0.2 sqrt(max(rows, cols)): an update of AdamW's size */
+#define PLAST_MUON_SCALE_NONE 2   /* s = 1 */
+#define PLAST_MUON_MAX_STEPS 32
+#define PLAST_MUON_MAX_DIM 262144
+typedef struct {
+  float lr;
+  float momentum;     /* typically 0.95 */
+  float weight_decay; /* decoupled */
+  float epsilon;      /* added to the Frobenius norm, typically 1e-7 */
+  int nesterov;       /* 0 / 1 */
+  int ns_steps;       /* Newton-Schulz steps, typically 5 */
+  int scale;          /* PLAST_MUON_SCALE_* */
+  Tensor **m;         /* momenta; NULL before the first step */
+} Muon;
+
+/* One step over a list of contiguous FLOAT32 parameters of two or more dims, each a matrix of
+ * shape[0] rows (at most PLAST_MUON_MAX_DIM rows or columns); entries that are NULL or have no grad
+ * are skipped. Per matrix, with gradient g:
+ *   m = momentum m + g,  u = nesterov ? g + momentum m : m
+ *   data = data (1 - lr weight_decay) - lr s orthogonalised(u)
+ * optimizer->m holds one momentum per parameter, contiguous and of its size; where it is NULL the
+ * first step creates zeros for the list (freed by plast_b200_muon_state_release, like Adam's), so a
+ * first step is not captured into a graph. A call that is refused changes nothing. */
+void muon_step_cuda(Muon *optimizer, Tensor **parameters, int num_parameters);
+void plast_b200_muon_state_release(Tensor **m);
+
+/* The orthogonalisation alone, for `count` matrices at once: X = x / (|x|_F + epsilon), then `steps`
+ * times (0 to PLAST_MUON_MAX_STEPS) X <- a X + (b A + c A A) X with A = X X^T (of the smaller side)
+ * and (a, b, c) = (3.4445, -4.7750, 2.0315). Contiguous FLOAT32 tensors as above; an output may be
+ * its own input. The norm is summed in 64 bits, every product has fp32 accuracy. A matrix of zeros
+ * gives zeros; a NaN or an infinity makes its matrix NaN. */
+void plast_b200_orthogonalise(const Tensor **inputs, Tensor **outputs, int count, int steps, float epsilon);
+
 #ifdef __cplusplus
 }
 #endif

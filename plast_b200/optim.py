@@ -26,14 +26,41 @@ class AdamW(C.Structure):
                 ("v", C.POINTER(C.POINTER(CTensor))), ("data_arena", C.c_void_p), ("optimizer_arena", C.c_void_p)]
 
 
+MUON_SCALE_ASPECT, MUON_SCALE_RMS, MUON_SCALE_NONE = 0, 1, 2
+
+
+class Muon(C.Structure):
+    """Muon of include/plast_b200_optim.h; `create` fills in the usual settings."""
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("epsilon", C.c_float),
+                ("nesterov", C.c_int), ("ns_steps", C.c_int), ("scale", C.c_int),
+                ("m", C.POINTER(C.POINTER(CTensor)))]
+
+    @classmethod
+    def create(cls, lr=0.02, momentum=0.95, weight_decay=0.0, epsilon=1e-7, nesterov=True, ns_steps=5,
+               scale=MUON_SCALE_ASPECT, moments=None):
+        """`moments`: the caller's momentum Tensors, one per parameter; None: the library creates them."""
+        opt = cls(lr, momentum, weight_decay, epsilon, int(bool(nesterov)), ns_steps, scale)
+        if moments is not None:
+            opt._moments = list(moments)          # keeps the caller's structs alive
+            opt._moments_array = param_array(opt._moments)
+            opt.m = opt._moments_array
+        return opt
+
+
+assert C.sizeof(Muon) == 40 and Muon.m.offset == 32
 assert C.sizeof(SGD) == 4 and C.sizeof(Adam) == 56 and C.sizeof(AdamW) == 56
 assert Adam.t.offset == 16 and Adam.m.offset == 24 and AdamW.t.offset == 20 and AdamW.m.offset == 24
 
-for _name, _struct in (("sgd_step_cuda", SGD), ("adam_step_cuda", Adam), ("adamw_step_cuda", AdamW)):
+for _name, _struct in (("sgd_step_cuda", SGD), ("adam_step_cuda", Adam), ("adamw_step_cuda", AdamW), ("muon_step_cuda", Muon)):
     getattr(lib, _name).argtypes = [C.POINTER(_struct), C.POINTER(C.POINTER(CTensor)), C.c_int]
     getattr(lib, _name).restype = None
 lib.plast_b200_adam_state_release.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(C.POINTER(CTensor))]
 lib.plast_b200_adam_state_release.restype = None
+lib.plast_b200_muon_state_release.argtypes = [C.POINTER(C.POINTER(CTensor))]
+lib.plast_b200_muon_state_release.restype = None
+lib.plast_b200_orthogonalise.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(C.POINTER(CTensor)), C.c_int, C.c_int,
+                                         C.c_float]
+lib.plast_b200_orthogonalise.restype = None
 
 
 def param_array(params):
@@ -47,13 +74,26 @@ def param_array(params):
 
 def step(optimizer, params) -> None:
     """One optimiser step on the GPU over a list of parameters (Tensor objects with .grad)."""
-    fn = {SGD: lib.sgd_step_cuda, Adam: lib.adam_step_cuda, AdamW: lib.adamw_step_cuda}[type(optimizer)]
+    fn = {SGD: lib.sgd_step_cuda, Adam: lib.adam_step_cuda, AdamW: lib.adamw_step_cuda,
+          Muon: lib.muon_step_cuda}[type(optimizer)]
     fn(C.byref(optimizer), param_array(params), len(params))
     check_error()
 
 
+def orthogonalise(inputs, outputs, steps: int = 5, epsilon: float = 1e-7) -> None:
+    """outputs[i] = the Newton-Schulz orthogonalisation of inputs[i], all matrices at once."""
+    if len(inputs) != len(outputs):
+        raise ValueError("as many outputs as inputs")
+    lib.plast_b200_orthogonalise(param_array(inputs), param_array(outputs), len(inputs), steps, epsilon)
+    check_error()
+
+
 def release_state(optimizer) -> None:
-    if not isinstance(optimizer, SGD) and optimizer.m:
+    if isinstance(optimizer, Muon):
+        if optimizer.m:
+            lib.plast_b200_muon_state_release(optimizer.m)
+            optimizer.m = None
+    elif not isinstance(optimizer, SGD) and optimizer.m:
         lib.plast_b200_adam_state_release(optimizer.m, optimizer.v)
         optimizer.m = None
         optimizer.v = None

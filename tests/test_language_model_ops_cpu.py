@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import plast_b200 as pb
+from plast_b200 import optim as O
 
 F, I = pb.FLOAT32, pb.INT32
 
@@ -173,3 +174,63 @@ def test_frequency_tables():
                 dict(scaling="parts", factor=2.0, slow=32, fast=1, context=4096),
                 dict(scaling="bands", factor=2.0, slow=1, fast=4, context=0), dict(scaling="base", factor=2.0, rotated=2)):
         refused("UNSUPPORTED", pb.rotary_frequencies, **{"rotated": 8, "base": base, **bad})
+
+
+def test_muon_refusals_change_nothing():
+    def params(*shapes):
+        return [T(*s, requires_grad=True) for s in shapes]
+
+    def f(ps, moments=None, **kw):
+        opt = O.Muon.create(moments=moments, **{k: v for k, v in kw.items()})
+        try:
+            O.step(opt, ps)
+        finally:
+            assert moments is not None or not opt.m          # nothing was created
+
+    f([])
+    f([None, T(3, 3)])                                        # nothing to update
+    refused("SHAPE", f, params((4, 4), (5,)))
+    refused("SHAPE", f, params(()))
+    refused("LIMIT", f, params((1, 262145)))
+    refused("UNSUPPORTED", f, params((4, 4)), ns_steps=-1)
+    refused("UNSUPPORTED", f, params((4, 4)), ns_steps=33)
+    refused("UNSUPPORTED", f, params((4, 4)), epsilon=-1e-7)
+    refused("UNSUPPORTED", f, params((4, 4)), epsilon=float("nan"))
+    refused("UNSUPPORTED", f, params((4, 4)), scale=3)
+    p = params((4, 4))[0]
+    refused("UNSUPPORTED", f, [p, p])
+    refused("UNSUPPORTED", f, params((4, 4), (4, 4)), moments=[T(4, 4)] * 2)
+    refused("NULL", f, params((4, 4), (4, 4)), moments=[T(4, 4), None])
+    refused("SHAPE", f, params((4, 4)), moments=[T(4, 3)])
+    refused("DTYPE", f, params((4, 4)), moments=[T(4, 4, dtype=I)])
+    t = T(8, 8).transpose(0, 1)
+    t.set_grad(T(8, 8))
+    refused("UNSUPPORTED", f, [t])
+    t = T(8, 8)
+    t.set_grad(T(8, 8).transpose(0, 1))
+    refused("UNSUPPORTED", f, [t])
+    t.set_grad(T(8, 7))
+    refused("SHAPE", f, [t])
+    t = T(8, 8, dtype=I)
+    t.set_grad(T(8, 8))
+    refused("DTYPE", f, [t])
+    t = T(8, 8, requires_grad=True)
+    t.c.data = None
+    refused("NULL", f, [t])
+
+
+def test_orthogonalise_refusals():
+    x, y, o = T(4, 6), T(4, 6), T(4, 6)
+    O.orthogonalise([], [])
+    O.orthogonalise([T(0, 4)], [T(0, 4)])
+    refused("NULL", O.orthogonalise, [None], [o])
+    refused("NULL", O.orthogonalise, [x], [None])
+    refused("SHAPE", O.orthogonalise, [T(4)], [T(4)])
+    refused("SHAPE", O.orthogonalise, [x], [T(6, 4)])
+    refused("DTYPE", O.orthogonalise, [T(4, 6, dtype=I)], [o])
+    refused("DTYPE", O.orthogonalise, [x], [T(4, 6, dtype=I)])
+    refused("UNSUPPORTED", O.orthogonalise, [x.transpose(0, 1)], [T(6, 4)])
+    refused("UNSUPPORTED", O.orthogonalise, [x, y], [o, o])
+    refused("UNSUPPORTED", O.orthogonalise, [x, y], [y, o])
+    refused("UNSUPPORTED", O.orthogonalise, [x], [o], 40)
+    refused("UNSUPPORTED", O.orthogonalise, [x], [o], 5, -1.0)
