@@ -121,6 +121,12 @@ void plast_b200_muon_state_release(Tensor **m);
  * gives zeros; a NaN or an infinity makes its matrix NaN. */
 void plast_b200_orthogonalise(const Tensor **inputs, Tensor **outputs, int count, int steps, float epsilon);
 
+/* Every wait inside the product kernels is limited to about two seconds. Where one runs out (which
+ * takes a broken GPU or library) the results of that call and the following ones are NaN instead of
+ * wrong, and this returns 1 once, after which they work again; 0 = all is well, -1 = a CUDA error.
+ * Waits for the library stream. */
+int plast_b200_muon_status(void);
+
 #ifdef __cplusplus
 }
 #endif

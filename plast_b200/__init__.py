@@ -119,7 +119,7 @@ def declared_symbols() -> list[str]:
         "plast_b200_peer_group_local", "plast_b200_chain_jit_available", "plast_b200_peer_full_reduce", "plast_b200_peer_cross_entropy_mean",
         "plast_b200_peer_reduce_begin", "plast_b200_peer_reduce_end",
         "plast_b200_token_logprob", "plast_b200_token_logprob_backward",
-        "muon_step_cuda", "plast_b200_muon_state_release", "plast_b200_orthogonalise",
+        "muon_step_cuda", "plast_b200_muon_state_release", "plast_b200_muon_status", "plast_b200_orthogonalise",
         "plast_b200_rotary_frequencies", "plast_b200_qk_norm_rotary", "plast_b200_qk_norm_rotary_backward",
     ]
     return syms

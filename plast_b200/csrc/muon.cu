@@ -10,6 +10,7 @@
 // about 10^-3 to about 1 in five steps.
 #include "plast_b200_optim.h"
 #include "row_map.cuh"
+#include "split_gemm.cuh"
 #include "ew_kernel_device.cuh" // pdl_wait / pdl_launch_dependents
 
 #include <algorithm>
@@ -31,17 +32,18 @@ struct MuonMat {
   const float *g;  // gradient, or the input of orthogonalise
   float *v;        // momentum; NULL: u = g
   float *w;        // weight (w = w * keep - rate * X) or, with keep == 0 and rate == -1, the output
-  float *x[2], *a, *b;
+  char *x[2], *a, *b; // panels: X (two, in turn), A, B
   double *partial; // sums of squares of the momentum pass, then partial[0] holds their total
   float keep, rate;
   unsigned rows, cols; // as stored
   unsigned m, n;       // m <= n
-  unsigned first;      // first CTA of this matrix in the launch at hand
+  unsigned first;      // first CTA (or tile) of this matrix in the launch at hand
   unsigned chunks;
 };
 struct MuonTable {
   MuonMat mat[kMuonMax];
   int count;
+  unsigned total; // CTAs or tiles of the launch at hand
   float mu, epsilon;
   int nesterov;
 };
@@ -104,99 +106,287 @@ __global__ void __launch_bounds__(kMuonThreads) muon_norm_kernel(const __grid_co
   if (threadIdx.x == 0) q.partial[0] = part[0];
 }
 
-// X = u / (|u| + eps), turned so that it has at most as many rows as columns
+// X = u / (|u| + eps), turned so that it has at most as many rows as columns, into its panel: one CTA
+// per 128 x 64 block, eight values to a thread; what lies outside the matrix is zero.
 __global__ void __launch_bounds__(kMuonThreads) muon_load_kernel(const __grid_constant__ MuonTable t) {
   pdl_wait();
   pdl_launch_dependents();
   const MuonMat &q = t.mat[matrix_of(t, blockIdx.x)];
-  __shared__ float tile[32][33];
-  const float norm = (float)sqrt(q.partial[0]) + t.epsilon;
-  const unsigned per_row = (q.cols + 31) / 32, at = blockIdx.x - q.first;
-  const unsigned r0 = at / per_row * 32, c0 = at % per_row * 32;
-  const unsigned tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  for (unsigned i = ty; i < 32; i += 8) {
-    const unsigned r = r0 + i, c = c0 + tx;
-    float u = 0.0f;
-    if (r < q.rows && c < q.cols) {
-      const u64 j = (u64)r * q.cols + c;
-      u = q.g[j];
-      if (q.v) u = update_of(t, u, q.v[j]);
-      u = u / norm;
-      if (q.rows <= q.cols) q.x[0][j] = u;
+  __shared__ float tile[kPanelCols][kPanelRows + 1]; // the block, turned
+  // in 64 bits: the norm may be outside fp32's range where the quotient is not
+  const double inv = (double)kSplitScale / (sqrt(q.partial[0]) + (double)t.epsilon);
+  const unsigned col_blocks = panel_col_blocks(q.n), at = blockIdx.x - q.first;
+  const unsigned rb = at / col_blocks, cb = at % col_blocks;
+  const bool turned = q.rows > q.cols;
+  auto value = [&](u64 j) {
+    float u = q.g[j];
+    if (q.v) u = update_of(t, u, q.v[j]);
+    return (float)((double)u * inv);
+  };
+  if (turned) { // stored row = panel column
+    for (unsigned e = threadIdx.x; e < kPanelRows * kPanelCols; e += kMuonThreads) {
+      const unsigned i = e % kPanelRows, k = e / kPanelRows; // panel row, panel column
+      const unsigned r = cb * kPanelCols + k, c = rb * kPanelRows + i;
+      tile[k][i] = r < q.rows && c < q.cols ? value((u64)r * q.cols + c) : 0.0f;
     }
-    tile[i][tx] = u;
+    __syncthreads();
   }
-  if (q.rows <= q.cols) return;
-  __syncthreads();
-  for (unsigned i = ty; i < 32; i += 8) {
-    const unsigned r = r0 + tx, c = c0 + i;
-    if (r < q.rows && c < q.cols) q.x[0][(u64)c * q.rows + r] = tile[tx][i];
+  char *block = q.x[0] + panel_block(rb, cb, col_blocks);
+  for (unsigned e = threadIdx.x; e < kPanelRows * 8; e += kMuonThreads) {
+    const unsigned row = e / 8, chunk = e % 8;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (turned) v[i] = tile[chunk * 8 + i][row];
+      else {
+        const unsigned r = rb * kPanelRows + row, c = cb * kPanelCols + chunk * 8 + i;
+        v[i] = r < q.rows && c < q.cols ? value((u64)r * q.cols + c) : 0.0f;
+      }
+    }
+    uint4 hi, lo;
+    split8(v, hi, lo);
+    *reinterpret_cast<uint4 *>(block + panel_chunk(row, chunk)) = hi;
+    *reinterpret_cast<uint4 *>(block + kPanelHalf + panel_chunk(row, chunk)) = lo;
   }
 }
 
-// One 64 x 64 tile of a product, 4 x 4 per thread.
+// ---- the products --------------------------------------------------------------------------------------
+// Three kinds, all on panels of split fp16 numbers (split_gemm.cuh), all values scaled by 2^14:
+//   gram        A = X X^T          both operands X, K-major, K = n
+//   polynomial  B = b A + c A A    both operands A (symmetric), K-major, K = m
+//   apply       X = a X + B X      left B, K-major; right X, MN-major (its rows are K), K = m
+// A persistent CTA walks tiles of 128 x 128. One thread brings 64 KB stages (64 of K, hi and lo of
+// both operands) with bulk copies, one thread issues the twelve tcgen05.mma of a stage, small products
+// first, and eight warps drain the accumulators. Tensor-core accumulation truncates; every kNsChunk
+// stages the accumulator (one of two in tensor memory) is therefore added in fp32 registers, rounded
+// to nearest, while the next one fills.
 enum MuonProduct { kGram = 0, kPolynomial = 1, kApply = 2 };
+constexpr int kNsStages = 3;
+constexpr unsigned kNsStageBytes = 4 * kPanelHalf; // left hi, left lo, right hi, right lo
+constexpr int kNsEpilogueWarps = 8, kNsThreads = (kNsEpilogueWarps + 2) * 32;
+#ifndef NS_CHUNK
+#define NS_CHUNK 4
+#endif
+constexpr int kNsChunk = NS_CHUNK;
+constexpr unsigned kNsSmem = kNsStages * kNsStageBytes + 1024;
+
+__device__ unsigned g_ns_gave_up; // a wait ran out: results are NaN from then on, see plast_b200_muon_status
+
+struct NsTile {
+  unsigned i, j, k_blocks; // tile row, tile column, K / 64
+};
 template <int WHAT>
-__global__ void __launch_bounds__(kMuonThreads) muon_product_kernel(const __grid_constant__ MuonTable t, int from, int last) {
+__device__ __forceinline__ const MuonMat &tile_at(const MuonTable &t, unsigned tile, NsTile &out) {
+  const MuonMat &q = t.mat[matrix_of(t, tile)];
+  const unsigned across = panel_row_blocks(WHAT == kApply ? q.n : q.m), at = tile - q.first;
+  out.i = at / across;
+  out.j = at % across;
+  out.k_blocks = panel_col_blocks(WHAT == kGram ? q.n : q.m);
+  return q;
+}
+
+template <int WHAT>
+__global__ void __launch_bounds__(kNsThreads, 1) muon_product_kernel(const __grid_constant__ MuonTable t, int from, int last) {
+  extern __shared__ char dynamic_smem[];
+  __shared__ __align__(8) uint64_t full[kNsStages], empty[kNsStages], acc_full[2], acc_empty[2], drained;
+  __shared__ uint32_t tmem_base;
+  __shared__ volatile unsigned gave_up;
+  const uint32_t stages = (smem_address(dynamic_smem) + 1023) & ~1023u;
+  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr unsigned kColumns = 128; // of one accumulator
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kNsStages; ++s) {
+      barrier_init(smem_address(&full[s]), 1);
+      barrier_init(smem_address(&empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      barrier_init(smem_address(&acc_full[b]), 1);
+      barrier_init(smem_address(&acc_empty[b]), kNsEpilogueWarps);
+    }
+    barrier_init(smem_address(&drained), 1);
+    gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kNsEpilogueWarps + 1) tmem_alloc<1>(smem_address(&tmem_base), 2 * kColumns);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_base;
   pdl_wait();
   pdl_launch_dependents();
-  const MuonMat &q = t.mat[matrix_of(t, blockIdx.x)];
-  const float *x = q.x[from];
-  const float *p = WHAT == kGram ? x : WHAT == kPolynomial ? q.a : q.b;      // left operand, rows of length k
-  const float *r = WHAT == kApply ? x : p;                                    // right operand
-  const unsigned k = WHAT == kGram ? q.n : q.m, width = WHAT == kApply ? q.n : q.m;
-  const unsigned tiles = (width + 63) / 64, at = blockIdx.x - q.first;
-  const unsigned i0 = at / tiles * 64, j0 = at % tiles * 64;
-  __shared__ float sp[16][65], sr[16][65];
-  float acc[4][4] = {};
-  const unsigned tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (unsigned k0 = 0; k0 < k; k0 += 16) {
-    for (unsigned e = threadIdx.x; e < 64 * 16; e += kMuonThreads) {
-      const unsigned kk = e & 15, i = e >> 4;
-      sp[kk][i] = i0 + i < q.m && k0 + kk < k ? p[(u64)(i0 + i) * k + k0 + kk] : 0.0f;
-      if (WHAT != kApply) sr[kk][i] = j0 + i < q.m && k0 + kk < k ? r[(u64)(j0 + i) * k + k0 + kk] : 0.0f;
-      else {
-        const unsigned j = e & 63, kr = e >> 6;
-        sr[kr][j] = j0 + j < q.n && k0 + kr < k ? r[(u64)(k0 + kr) * q.n + j0 + j] : 0.0f;
+
+  if (warp == kNsEpilogueWarps) { // ---- loads
+    if (lane == 0) {
+      asm volatile("fence.proxy.async;" ::: "memory"); // the panels were written with plain stores
+      unsigned it = 0;
+      bool ok = true;
+      for (unsigned tile = blockIdx.x; ok && tile < t.total; tile += gridDim.x) {
+        NsTile at;
+        const MuonMat &q = tile_at<WHAT>(t, tile, at);
+        const unsigned xcb = panel_col_blocks(q.n), mcb = panel_col_blocks(q.m);
+        const char *left = WHAT == kGram ? q.x[from] : WHAT == kPolynomial ? q.a : q.b;
+        const unsigned left_cb = WHAT == kGram ? xcb : mcb;
+        const char *right = WHAT == kApply ? q.x[from] : left;
+        for (unsigned k = 0; k < at.k_blocks; ++k, ++it) {
+          const unsigned s = it % kNsStages, phase = (it / kNsStages) & 1;
+          if (!(ok = barrier_wait(smem_address(&empty[s]), phase ^ 1, &gave_up))) break;
+          const uint32_t bar = smem_address(&full[s]), dst = stages + s * kNsStageBytes;
+          if (WHAT != kApply) {
+            barrier_expect(bar, kNsStageBytes);
+            bulk_load(dst, left + panel_block(at.i, k, left_cb), 2 * kPanelHalf, bar);
+            bulk_load(dst + 2 * kPanelHalf, right + panel_block(at.j, k, left_cb), 2 * kPanelHalf, bar);
+          } else {
+            // right: rows 64 k .. 64 k + 63 of two neighbouring blocks of X, the second of which may
+            // lie beyond its last column (then those columns of the tile are not stored)
+            const bool both = 2 * at.j + 1 < xcb;
+            barrier_expect(bar, 2 * kPanelHalf + (both ? 2 : 1) * kPanelHalf);
+            bulk_load(dst, left + panel_block(at.i, k, left_cb), 2 * kPanelHalf, bar);
+            for (unsigned c = 0; c < (both ? 2u : 1u); ++c) {
+              const char *src = right + panel_block(k / 2, 2 * at.j + c, xcb) + (k & 1) * (kPanelHalf / 2);
+              bulk_load(dst + 2 * kPanelHalf + c * (kPanelHalf / 2), src, kPanelHalf / 2, bar);
+              bulk_load(dst + 3 * kPanelHalf + c * (kPanelHalf / 2), src + kPanelHalf, kPanelHalf / 2, bar);
+            }
+          }
+        }
+      }
+      if (!ok) // copies in flight end before shared memory goes away
+        for (unsigned back = 1; back <= kNsStages && back <= it; ++back) {
+          const unsigned i = it - back, s = i % kNsStages, phase = (i / kNsStages) & 1;
+          const long long start = clock64();
+          while (!barrier_try(smem_address(&full[s]), phase) && clock64() - start < 10000000) {}
+        }
+    }
+  } else if (warp == kNsEpilogueWarps + 1) { // ---- products
+    if (lane == 0) {
+      constexpr uint32_t desc = mma_desc(128, 128, false, WHAT == kApply);
+      unsigned it = 0, round = 0;
+      bool ok = true;
+      for (unsigned tile = blockIdx.x; ok && tile < t.total; tile += gridDim.x) {
+        NsTile at;
+        tile_at<WHAT>(t, tile, at);
+        for (unsigned k = 0; k < at.k_blocks; ++k, ++it) {
+          const unsigned s = it % kNsStages, phase = (it / kNsStages) & 1, buf = round & 1;
+          const bool first = k % kNsChunk == 0;
+          if (first && !(ok = barrier_wait(smem_address(&acc_empty[buf]), ((round >> 1) & 1) ^ 1, &gave_up))) break;
+          if (!(ok = barrier_wait(smem_address(&full[s]), phase, &gave_up))) break;
+          tmem_fence_after();
+          const uint32_t left = stages + s * kNsStageBytes, right = left + 2 * kPanelHalf;
+          const uint32_t acc = tmem + buf * kColumns;
+#pragma unroll
+          for (int part = 0; part < 3; ++part) { // lo hi, hi lo, hi hi
+            const uint32_t l = left + (part == 0 ? kPanelHalf : 0), r = right + (part == 1 ? kPanelHalf : 0);
+#pragma unroll
+            for (int step = 0; step < 4; ++step) { // 16 of K
+              const uint64_t da = operand_desc(l + step * 32, 16, 1024);
+              const uint64_t db = WHAT == kApply ? operand_desc(r + step * 2048, kPanelHalf / 2, 1024)
+                                                 : operand_desc(r + step * 32, 16, 1024);
+              mma_f16<1>(acc, da, db, desc, !(first && part == 0 && step == 0));
+            }
+          }
+          mma_commit<1>(smem_address(&empty[s]));
+          if (k % kNsChunk == kNsChunk - 1 || k + 1 == at.k_blocks) {
+            mma_commit<1>(smem_address(&acc_full[buf]));
+            ++round;
+          }
+        }
+      }
+      if (!ok) {
+        mma_commit<1>(smem_address(&drained));
+        const long long start = clock64();
+        while (!barrier_try(smem_address(&drained), 0) && clock64() - start < 10000000) {}
       }
     }
-    __syncthreads();
-    for (int kk = 0; kk < 16; ++kk)
+  } else { // ---- accumulators to results: warp w takes rows 32 (w % 4) .. and columns 64 (w / 4) ..
+    const unsigned row_in_tile = (warp & 3) * 32 + lane, half = warp >> 2;
+    unsigned round = 0;
+    bool ok = true;
+    for (unsigned tile = blockIdx.x; ok && tile < t.total; tile += gridDim.x) {
+      NsTile at;
+      const MuonMat &q = tile_at<WHAT>(t, tile, at);
+      float acc[64];
+      const unsigned rounds = (at.k_blocks + kNsChunk - 1) / kNsChunk;
+      for (unsigned c = 0; c < rounds; ++c, ++round) {
+        const unsigned buf = round & 1;
+        ok = __all_sync(0xffffffffu, barrier_wait(smem_address(&acc_full[buf]), (round >> 1) & 1, &gave_up));
+        if (!ok) break;
+        tmem_fence_after();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int h = 0; h < 2; ++h) {
+          float v[32];
+          tmem_load32(tmem + (((warp & 3) * 32) << 16) + buf * kColumns + half * 64 + h * 32, v);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __fmaf_rn(sp[kk][ty * 4 + i], sr[kk][tx * 4 + j], acc[i][j]);
-    __syncthreads();
-  }
+          for (int i = 0; i < 32; ++i) acc[h * 32 + i] = c == 0 ? v[i] : acc[h * 32 + i] + v[i];
+        }
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(smem_address(&acc_empty[buf]));
+      }
+      if (!ok) break;
+      // the warp's 64 columns are one block column of the result
+      const unsigned width = WHAT == kApply ? q.n : q.m;
+      const unsigned col_blocks = panel_col_blocks(width), cb = 2 * at.j + half;
+      if (cb >= col_blocks) continue;
+      const u64 offset = panel_block(at.i, cb, col_blocks);
+      const char *old = WHAT == kPolynomial ? q.a : q.x[from]; // the linear term
+      char *out = WHAT == kGram ? q.a : WHAT == kPolynomial ? q.b : q.x[from ^ 1];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+      for (int chunk = 0; chunk < 8; ++chunk) {
+        const u64 here = offset + panel_chunk(row_in_tile, chunk);
+        float v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned row = i0 + ty * 4 + i, col = j0 + tx * 4 + j;
-      if (row >= q.m || col >= width) continue;
-      const u64 at_ij = (u64)row * width + col;
-      if (WHAT == kGram) q.a[at_ij] = acc[i][j];
-      if (WHAT == kPolynomial) q.b[at_ij] = __fmaf_rn(kNsB, q.a[at_ij], kNsC * acc[i][j]);
-      if (WHAT == kApply) {
-        const float v = __fmaf_rn(kNsA, x[at_ij], acc[i][j]);
-        if (!last) q.x[from ^ 1][at_ij] = v;
-        else {
-          float *w = q.w + (q.rows <= q.cols ? at_ij : (u64)col * q.m + row);
-          *w = q.keep == 0.0f ? -q.rate * v : __fmaf_rn(-q.rate, v, q.keep * *w);
+        for (int i = 0; i < 8; ++i) v[i] = acc[chunk * 8 + i] * kSplitUnscale;
+        if (WHAT != kGram) {
+          float z[8];
+          join8(*reinterpret_cast<const uint4 *>(old + here), *reinterpret_cast<const uint4 *>(old + here + kPanelHalf), z);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            v[i] = WHAT == kPolynomial ? __fmaf_rn(kNsB, z[i], kNsC * v[i]) : __fmaf_rn(kNsA, z[i], v[i]);
+        }
+        if (WHAT != kApply || !last) {
+          uint4 hi, lo;
+          split8(v, hi, lo);
+          *reinterpret_cast<uint4 *>(out + here) = hi;
+          *reinterpret_cast<uint4 *>(out + here + kPanelHalf) = lo;
+        } else {
+          const unsigned row = at.i * 128 + row_in_tile;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const unsigned col = cb * kPanelCols + chunk * 8 + i;
+            if (row >= q.m || col >= q.n) continue;
+            float *w = q.w + (q.rows <= q.cols ? (u64)row * q.n + col : (u64)col * q.m + row);
+            const float x = g_ns_gave_up ? NAN : v[i] * kSplitUnscale;
+            *w = q.keep == 0.0f ? -q.rate * x : __fmaf_rn(-q.rate, x, q.keep * *w);
+          }
         }
       }
     }
+  }
+  __syncwarp();
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  if (threadIdx.x == 0 && gave_up) atomicOr(&g_ns_gave_up, 1u);
+  if (warp == kNsEpilogueWarps + 1) tmem_free<1>(tmem, 2 * kColumns);
 }
 
 // steps == 0: X itself
-__global__ void __launch_bounds__(kMuonThreads) muon_store_kernel(const __grid_constant__ MuonTable t, int from) {
+__global__ void __launch_bounds__(kMuonThreads) muon_store_kernel(const __grid_constant__ MuonTable t) {
   pdl_wait();
   pdl_launch_dependents();
   const MuonMat &q = t.mat[matrix_of(t, blockIdx.x)];
   const u64 total = (u64)q.rows * q.cols, begin = (u64)(blockIdx.x - q.first) * kMuonChunk;
+  const unsigned col_blocks = panel_col_blocks(q.n);
   for (u64 j = begin + threadIdx.x; j < begin + kMuonChunk && j < total; j += kMuonThreads) {
-    const u64 r = j / q.cols, c = j - r * q.cols;
-    const float v = q.x[from][q.rows <= q.cols ? j : c * q.rows + r];
+    unsigned r = (unsigned)(j / q.cols), c = (unsigned)(j % q.cols);
+    if (q.rows > q.cols) {
+      const unsigned s = r;
+      r = c;
+      c = s;
+    }
+    const char *at = q.x[0] + panel_block(r / kPanelRows, c / kPanelCols, col_blocks) +
+                     panel_chunk(r % kPanelRows, (c % kPanelCols) / 8) + (c & 7) * 2;
+    const float v = (__half2float(*(const __half *)at) + __half2float(*(const __half *)(at + kPanelHalf))) * kSplitUnscale;
     q.w[j] = q.keep == 0.0f ? -q.rate * v : __fmaf_rn(-q.rate, v, q.keep * q.w[j]);
   }
 }
@@ -204,54 +394,69 @@ __global__ void __launch_bounds__(kMuonThreads) muon_store_kernel(const __grid_c
 // ---- host --------------------------------------------------------------------------------------------
 static u64 padded(u64 bytes) { return (bytes + 255) & ~(u64)255; }
 static u64 scratch_bytes(const MuonMat &q) {
-  return 2 * padded((u64)q.m * q.n * 4) + 2 * padded((u64)q.m * q.m * 4) + padded((u64)(q.chunks + 1) * 8);
+  return 2 * panel_bytes(q.m, q.n) + 2 * panel_bytes(q.m, q.m) + padded((u64)(q.chunks + 1) * 8);
 }
 
-template <class Blocks, class... KArgs, class... Args>
-static bool launch_over(MuonTable &t, Blocks blocks, void (*kernel)(KArgs...), Args... args) {
+// Numbers the CTAs (or tiles) of a launch over the matrices.
+template <class Blocks>
+static void number(MuonTable &t, Blocks blocks) {
   u64 n = 0;
   for (int i = 0; i < t.count; ++i) {
     t.mat[i].first = (unsigned)n;
     n += blocks(t.mat[i]);
   }
-  const cudaError_t e = launch_k(kernel, dim3((unsigned)n), dim3(kMuonThreads), 0, stream(), t, args...);
-  if (e != cudaSuccess) {
-    set_error(PLAST_B200_ERR_CUDA, "muon: %s", cudaGetErrorString(e));
-    return false;
+  t.total = (unsigned)n; // a group's scratch bounds it far below 2^32
+}
+static bool launched(cudaError_t e) {
+  if (e == cudaSuccess) {
+    count_launch();
+    return true;
   }
-  count_launch();
-  return true;
+  set_error(PLAST_B200_ERR_CUDA, "muon: %s", cudaGetErrorString(e));
+  return false;
+}
+template <class Blocks>
+static bool launch_over(MuonTable &t, Blocks blocks, void (*kernel)(const MuonTable)) {
+  number(t, blocks);
+  return launched(launch_k(kernel, dim3(t.total), dim3(kMuonThreads), 0, stream(), t));
+}
+template <int WHAT>
+static bool launch_product(MuonTable &t, int from, int last) {
+  number(t, [](const MuonMat &q) {
+    return (u64)panel_row_blocks(q.m) * panel_row_blocks(WHAT == kApply ? q.n : q.m);
+  });
+  const cudaError_t e = cudaFuncSetAttribute(muon_product_kernel<WHAT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem);
+  if (e != cudaSuccess) return launched(e);
+  const unsigned grid = t.total < (unsigned)sm_count() ? t.total : (unsigned)sm_count();
+  return launched(launch_k(muon_product_kernel<WHAT>, dim3(grid), dim3(kNsThreads), kNsSmem, stream(), t, from, last));
 }
 
 // One group of matrices whose scratch is `base`.
 static void run_group(MuonTable &t, char *base, int steps) {
   for (int i = 0; i < t.count; ++i) {
     MuonMat &q = t.mat[i];
-    for (int k = 0; k < 2; ++k) {
-      q.x[k] = (float *)base;
-      base += padded((u64)q.m * q.n * 4);
-    }
-    q.a = (float *)base;
-    base += padded((u64)q.m * q.m * 4);
-    q.b = (float *)base;
-    base += padded((u64)q.m * q.m * 4);
-    q.partial = (double *)base;
-    base += padded((u64)(q.chunks + 1) * 8);
+    auto take = [&](u64 bytes) {
+      char *p = base;
+      base += bytes;
+      return p;
+    };
+    q.x[0] = take(panel_bytes(q.m, q.n));
+    q.x[1] = take(panel_bytes(q.m, q.n));
+    q.a = take(panel_bytes(q.m, q.m));
+    q.b = take(panel_bytes(q.m, q.m));
+    q.partial = (double *)take(padded((u64)(q.chunks + 1) * 8));
   }
   auto chunks = [](const MuonMat &q) { return (u64)q.chunks; };
-  auto tiles = [](unsigned a, unsigned b, unsigned s) { return (u64)((a + s - 1) / s) * ((b + s - 1) / s); };
+  auto blocks = [](const MuonMat &q) { return (u64)panel_row_blocks(q.m) * panel_col_blocks(q.n); };
   if (!launch_over(t, chunks, muon_momentum_kernel)) return;
   if (!launch_over(t, [](const MuonMat &) { return (u64)1; }, muon_norm_kernel)) return;
-  if (!launch_over(t, [&](const MuonMat &q) { return tiles(q.rows, q.cols, 32); }, muon_load_kernel)) return;
-  int from = 0;
+  if (!launch_over(t, blocks, muon_load_kernel)) return;
   for (int s = 0; s < steps; ++s) {
-    const int last = s + 1 == steps;
-    if (!launch_over(t, [&](const MuonMat &q) { return tiles(q.m, q.m, 64); }, muon_product_kernel<kGram>, from, 0)) return;
-    if (!launch_over(t, [&](const MuonMat &q) { return tiles(q.m, q.m, 64); }, muon_product_kernel<kPolynomial>, from, 0)) return;
-    if (!launch_over(t, [&](const MuonMat &q) { return tiles(q.m, q.n, 64); }, muon_product_kernel<kApply>, from, last)) return;
-    from ^= 1;
+    const int from = s & 1, last = s + 1 == steps;
+    if (!launch_product<kGram>(t, from, 0) || !launch_product<kPolynomial>(t, from, 0) || !launch_product<kApply>(t, from, last))
+      return;
   }
-  if (steps == 0) launch_over(t, chunks, muon_store_kernel, 0);
+  if (steps == 0) launch_over(t, chunks, muon_store_kernel);
 }
 
 // All matrices, in groups that share one piece of scratch.
@@ -504,6 +709,18 @@ void plast_b200_orthogonalise(const Tensor **inputs, Tensor **outputs, int count
   } catch (...) {
     set_error(PLAST_B200_ERR_CUDA, "orthogonalise: out of host memory");
   }
+}
+
+int plast_b200_muon_status(void) {
+  begin_call();
+  unsigned status = 0;
+  PB_CUDA_RET(cudaStreamSynchronize(stream()), -1);
+  PB_CUDA_RET(cudaMemcpyFromSymbol(&status, g_ns_gave_up, sizeof status), -1);
+  if (status) {
+    const unsigned none = 0;
+    PB_CUDA_RET(cudaMemcpyToSymbol(g_ns_gave_up, &none, sizeof none), -1);
+  }
+  return (int)status;
 }
 
 void plast_b200_muon_state_release(Tensor **m) {
