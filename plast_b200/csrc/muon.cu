@@ -37,13 +37,17 @@ struct MuonMat {
   float keep, rate;
   unsigned rows, cols; // as stored
   unsigned m, n;       // m <= n
-  unsigned first;      // first CTA (or tile) of this matrix in the launch at hand
+  unsigned first;      // first CTA of this matrix in the launch at hand
+  unsigned first_tile[3]; // first tile of this matrix in the products gram, polynomial, apply
   unsigned chunks;
 };
 struct MuonTable {
   MuonMat mat[kMuonMax];
   int count;
-  unsigned total; // CTAs or tiles of the launch at hand
+  unsigned total;     // CTAs of the launch at hand
+  unsigned tiles[3];  // of each product
+  int narrow[3];      // tiles of 128 x 64 instead of 128 x 128
+  unsigned *arrived;  // grid barrier of the fused steps
   float mu, epsilon;
   int nesterov;
 };
@@ -103,7 +107,10 @@ __global__ void __launch_bounds__(kMuonThreads) muon_norm_kernel(const __grid_co
     if ((int)threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
     __syncthreads();
   }
-  if (threadIdx.x == 0) q.partial[0] = part[0];
+  if (threadIdx.x == 0) {
+    q.partial[0] = part[0];
+    if (blockIdx.x == 0) *t.arrived = 0; // for the grid barrier of the steps
+  }
 }
 
 // X = u / (|u| + eps), turned so that it has at most as many rows as columns, into its panel: one CTA
@@ -153,221 +160,457 @@ __global__ void __launch_bounds__(kMuonThreads) muon_load_kernel(const __grid_co
 // ---- the products --------------------------------------------------------------------------------------
 // Three kinds, all on panels of split fp16 numbers (split_gemm.cuh), all values scaled by 2^14:
 //   gram        A = X X^T          both operands X, K-major, K = n
-//   polynomial  B = b A + c A A    both operands A (symmetric), K-major, K = m
-//   apply       X = a X + B X      left B, K-major; right X, MN-major (its rows are K), K = m
-// A persistent CTA walks tiles of 128 x 128. One thread brings 64 KB stages (64 of K, hi and lo of
-// both operands) with bulk copies, one thread issues the twelve tcgen05.mma of a stage, small products
-// first, and eight warps drain the accumulators. Tensor-core accumulation truncates; every kNsChunk
-// stages the accumulator (one of two in tensor memory) is therefore added in fp32 registers, rounded
-// to nearest, while the next one fills.
+//   polynomial  B = b A + c A A    both operands A, K = m
+//   apply       X = a X + B X      left B; right X, MN-major (its rows are K), K = m
+// A and B are symmetric: only tiles on and above the diagonal are computed and stored. An operand
+// block below it is fetched as the block above it and read MN-major, which is its transpose.
+//
+// A persistent CTA walks tiles of 128 x 128 (or 128 x 64); a pair of CTAs (CTAS = 2) walks tiles of
+// 256 x 256, each CTA holding half of either operand. One thread brings 64 KB stages (64 of K, hi and
+// lo of both operands) with bulk copies, one thread (of the pair) issues the twelve tcgen05.mma of a
+// stage, small products first, and eight warps drain the accumulators. Tensor-core accumulation
+// truncates; every kNsChunk stages the accumulator (one of two in tensor memory) is therefore added in
+// fp32 registers, rounded to nearest, while the next one fills.
 enum MuonProduct { kGram = 0, kPolynomial = 1, kApply = 2 };
 constexpr int kNsStages = 3;
 constexpr unsigned kNsStageBytes = 4 * kPanelHalf; // left hi, left lo, right hi, right lo
 constexpr int kNsEpilogueWarps = 8, kNsThreads = (kNsEpilogueWarps + 2) * 32;
 #ifndef NS_CHUNK
-#define NS_CHUNK 4
+#define NS_CHUNK 2
 #endif
 constexpr int kNsChunk = NS_CHUNK;
-constexpr unsigned kNsSmem = kNsStages * kNsStageBytes + 1024;
+constexpr unsigned kNsTurnBytes = kNsEpilogueWarps * 32 * 33 * 4; // a 32 x 32 piece per warp, to store rows in order
+constexpr unsigned kNsSmem = kNsStages * kNsStageBytes + 1024 + kNsTurnBytes;
 
 __device__ unsigned g_ns_gave_up; // a wait ran out: results are NaN from then on, see plast_b200_muon_status
+
+// tiles along a side, and of a product; `wide`: columns of a tile (256, 128 or 64)
+__host__ __device__ inline unsigned ns_along(unsigned size, unsigned tile) { return (size + tile - 1) / tile; }
+template <int CTAS> __host__ __device__ inline unsigned ns_wide(bool narrow) { return narrow ? 64 : 128 * CTAS; }
+template <int CTAS> __host__ __device__ inline u64 ns_tiles_of(const MuonMat &q, int what, bool narrow) {
+  const u64 r = ns_along(q.m, 128 * CTAS), per_diagonal = 128 * CTAS / ns_wide<CTAS>(narrow);
+  const u64 c = ns_along(what == kApply ? q.n : q.m, ns_wide<CTAS>(narrow));
+  return what == kApply ? r * c : r * c - per_diagonal * (r * (r - 1) / 2); // row i starts at its diagonal block
+}
 
 struct NsTile {
   unsigned i, j, k_blocks; // tile row, tile column, K / 64
 };
-template <int WHAT>
+template <int CTAS, int WHAT>
 __device__ __forceinline__ const MuonMat &tile_at(const MuonTable &t, unsigned tile, NsTile &out) {
-  const MuonMat &q = t.mat[matrix_of(t, tile)];
-  const unsigned across = panel_row_blocks(WHAT == kApply ? q.n : q.m), at = tile - q.first;
-  out.i = at / across;
-  out.j = at % across;
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.mat[mid].first_tile[WHAT] <= tile) lo = mid; else hi = mid - 1;
+  }
+  const MuonMat &q = t.mat[lo];
+  const unsigned wide = ns_wide<CTAS>(t.narrow[WHAT]), across = ns_along(WHAT == kApply ? q.n : q.m, wide);
+  unsigned at = tile - q.first_tile[WHAT];
+  if (WHAT == kApply) {
+    out.i = at / across;
+    out.j = at % across;
+  } else { // rows of the upper triangle
+    const unsigned per_diagonal = 128 * CTAS / wide;
+    unsigned i = 0, length = across;
+    while (at >= length) {
+      at -= length;
+      length -= per_diagonal;
+      ++i;
+    }
+    out.i = i;
+    out.j = i * per_diagonal + at;
+  }
   out.k_blocks = panel_col_blocks(WHAT == kGram ? q.n : q.m);
   return q;
 }
 
-template <int WHAT>
-__global__ void __launch_bounds__(kNsThreads, 1) muon_product_kernel(const __grid_constant__ MuonTable t, int from, int last) {
-  extern __shared__ char dynamic_smem[];
-  __shared__ __align__(8) uint64_t full[kNsStages], empty[kNsStages], acc_full[2], acc_empty[2], drained;
-  __shared__ uint32_t tmem_base;
-  __shared__ volatile unsigned gave_up;
-  const uint32_t stages = (smem_address(dynamic_smem) + 1023) & ~1023u;
-  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr unsigned kColumns = 128; // of one accumulator
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kNsStages; ++s) {
-      barrier_init(smem_address(&full[s]), 1);
-      barrier_init(smem_address(&empty[s]), 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      barrier_init(smem_address(&acc_full[b]), 1);
-      barrier_init(smem_address(&acc_empty[b]), kNsEpilogueWarps);
-    }
-    barrier_init(smem_address(&drained), 1);
-    gave_up = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+// 128 rows (block row rb) by 64 of K (block kb) of a panel into `dst`: hi, then lo. `flip`: as the
+// transpose of the block above the diagonal, two pieces of 64 K rows by 64 columns each. `narrow`: 64
+// rows, rb counts in 64. Returns the bytes; what lies outside the panel is not fetched (it only feeds
+// results that are not stored).
+__device__ __forceinline__ unsigned operand_bytes(unsigned rb, unsigned row_blocks, unsigned col_blocks, bool flip, bool narrow) {
+  if (narrow) return (flip ? rb < col_blocks : rb / 2 < row_blocks) ? kPanelHalf : 0;
+  if (!flip) return rb < row_blocks ? 2 * kPanelHalf : 0;
+  return 2 * rb + 1 < col_blocks ? 2 * kPanelHalf : (2 * rb < col_blocks ? kPanelHalf : 0);
+}
+__device__ __forceinline__ void load_operand(uint32_t dst, const char *panel, unsigned rb, unsigned kb, unsigned row_blocks,
+                                             unsigned col_blocks, bool flip, bool narrow, uint32_t bar) {
+  constexpr unsigned kPiece = kPanelHalf / 2; // 64 rows
+  if (narrow) {
+    if (flip ? rb >= col_blocks : rb / 2 >= row_blocks) return;
+    const char *src = flip ? panel + panel_block(kb / 2, rb, col_blocks) + (kb & 1) * kPiece
+                           : panel + panel_block(rb / 2, kb, col_blocks) + (rb & 1) * kPiece;
+    bulk_load(dst, src, kPiece, bar);
+    bulk_load(dst + kPanelHalf, src + kPanelHalf, kPiece, bar);
+    return;
   }
-  if (warp == kNsEpilogueWarps + 1) tmem_alloc<1>(smem_address(&tmem_base), 2 * kColumns);
-  tmem_fence_before();
-  __syncthreads();
-  tmem_fence_after();
-  const uint32_t tmem = tmem_base;
-  pdl_wait();
-  pdl_launch_dependents();
+  if (!flip) {
+    if (rb < row_blocks) bulk_load(dst, panel + panel_block(rb, kb, col_blocks), 2 * kPanelHalf, bar);
+    return;
+  }
+#pragma unroll
+  for (unsigned c = 0; c < 2; ++c)
+    if (2 * rb + c < col_blocks) {
+      const char *src = panel + panel_block(kb / 2, 2 * rb + c, col_blocks) + (kb & 1) * kPiece;
+      bulk_load(dst + c * kPiece, src, kPiece, bar);
+      bulk_load(dst + kPanelHalf + c * kPiece, src + kPanelHalf, kPiece, bar);
+    }
+}
 
-  if (warp == kNsEpilogueWarps) { // ---- loads
-    if (lane == 0) {
-      asm volatile("fence.proxy.async;" ::: "memory"); // the panels were written with plain stores
-      unsigned it = 0;
-      bool ok = true;
-      for (unsigned tile = blockIdx.x; ok && tile < t.total; tile += gridDim.x) {
-        NsTile at;
-        const MuonMat &q = tile_at<WHAT>(t, tile, at);
-        const unsigned xcb = panel_col_blocks(q.n), mcb = panel_col_blocks(q.m);
-        const char *left = WHAT == kGram ? q.x[from] : WHAT == kPolynomial ? q.a : q.b;
-        const unsigned left_cb = WHAT == kGram ? xcb : mcb;
-        const char *right = WHAT == kApply ? q.x[from] : left;
-        for (unsigned k = 0; k < at.k_blocks; ++k, ++it) {
-          const unsigned s = it % kNsStages, phase = (it / kNsStages) & 1;
-          if (!(ok = barrier_wait(smem_address(&empty[s]), phase ^ 1, &gave_up))) break;
-          const uint32_t bar = smem_address(&full[s]), dst = stages + s * kNsStageBytes;
-          if (WHAT != kApply) {
-            barrier_expect(bar, kNsStageBytes);
-            bulk_load(dst, left + panel_block(at.i, k, left_cb), 2 * kPanelHalf, bar);
-            bulk_load(dst + 2 * kPanelHalf, right + panel_block(at.j, k, left_cb), 2 * kPanelHalf, bar);
-          } else {
-            // right: rows 64 k .. 64 k + 63 of two neighbouring blocks of X, the second of which may
-            // lie beyond its last column (then those columns of the tile are not stored)
-            const bool both = 2 * at.j + 1 < xcb;
-            barrier_expect(bar, 2 * kPanelHalf + (both ? 2 : 1) * kPanelHalf);
-            bulk_load(dst, left + panel_block(at.i, k, left_cb), 2 * kPanelHalf, bar);
-            for (unsigned c = 0; c < (both ? 2u : 1u); ++c) {
-              const char *src = right + panel_block(k / 2, 2 * at.j + c, xcb) + (k & 1) * (kPanelHalf / 2);
-              bulk_load(dst + 2 * kPanelHalf + c * (kPanelHalf / 2), src, kPanelHalf / 2, bar);
-              bulk_load(dst + 3 * kPanelHalf + c * (kPanelHalf / 2), src + kPanelHalf, kPanelHalf / 2, bar);
-            }
-          }
-        }
-      }
-      if (!ok) // copies in flight end before shared memory goes away
-        for (unsigned back = 1; back <= kNsStages && back <= it; ++back) {
-          const unsigned i = it - back, s = i % kNsStages, phase = (i / kNsStages) & 1;
-          const long long start = clock64();
-          while (!barrier_try(smem_address(&full[s]), phase) && clock64() - start < 10000000) {}
-        }
+struct NsShared {
+  uint64_t full[kNsStages], peer_full[kNsStages], empty[kNsStages], acc_full[2], acc_empty[2], drained;
+  uint32_t tmem;
+  volatile unsigned gave_up;
+};
+// A role's place in the rings of stages and accumulators, kept from one product to the next.
+struct NsRing {
+  uint32_t stages; // shared memory
+  unsigned rank;   // in the pair
+  unsigned it, round;
+};
+
+// ---- the thread that loads
+template <int CTAS, int WHAT>
+__device__ bool ns_load(const MuonTable &t, int from, NsShared &sh, NsRing &ring) {
+  const bool narrow = CTAS == 1 && t.narrow[WHAT];
+  for (unsigned tile = blockIdx.x / CTAS; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
+    NsTile at;
+    const MuonMat &q = tile_at<CTAS, WHAT>(t, tile, at);
+    const unsigned rows = panel_row_blocks(q.m), xcb = panel_col_blocks(q.n), mcb = panel_col_blocks(q.m);
+    const char *left = WHAT == kGram ? q.x[from] : WHAT == kPolynomial ? q.a : q.b;
+    const char *right = WHAT == kPolynomial ? q.a : q.x[from];
+    const unsigned left_cb = WHAT == kGram ? xcb : mcb, right_cb = WHAT == kPolynomial ? mcb : xcb;
+    const unsigned i = at.i * CTAS + ring.rank, j = at.j * CTAS + ring.rank;
+    const unsigned j_diagonal = narrow ? at.j / 2 : at.j;
+    for (unsigned k = 0; k < at.k_blocks; ++k, ++ring.it) {
+      const unsigned s = ring.it % kNsStages, phase = (ring.it / kNsStages) & 1;
+      const bool flip_left = WHAT != kGram && k / (2 * CTAS) < at.i;
+      const bool flip_right = WHAT == kApply || (WHAT == kPolynomial && k / (2 * CTAS) < j_diagonal);
+      if (!barrier_wait(smem_address(&sh.empty[s]), phase ^ 1, &sh.gave_up)) return false;
+      const uint32_t bar = smem_address(&sh.full[s]), dst = ring.stages + s * kNsStageBytes;
+      barrier_expect(bar, operand_bytes(i, rows, left_cb, flip_left, false) + operand_bytes(j, rows, right_cb, flip_right, narrow));
+      load_operand(dst, left, i, k, rows, left_cb, flip_left, false, bar);
+      load_operand(dst + 2 * kPanelHalf, right, j, k, rows, right_cb, flip_right, narrow, bar);
     }
-  } else if (warp == kNsEpilogueWarps + 1) { // ---- products
-    if (lane == 0) {
-      constexpr uint32_t desc = mma_desc(128, 128, false, WHAT == kApply);
-      unsigned it = 0, round = 0;
-      bool ok = true;
-      for (unsigned tile = blockIdx.x; ok && tile < t.total; tile += gridDim.x) {
-        NsTile at;
-        tile_at<WHAT>(t, tile, at);
-        for (unsigned k = 0; k < at.k_blocks; ++k, ++it) {
-          const unsigned s = it % kNsStages, phase = (it / kNsStages) & 1, buf = round & 1;
-          const bool first = k % kNsChunk == 0;
-          if (first && !(ok = barrier_wait(smem_address(&acc_empty[buf]), ((round >> 1) & 1) ^ 1, &gave_up))) break;
-          if (!(ok = barrier_wait(smem_address(&full[s]), phase, &gave_up))) break;
-          tmem_fence_after();
-          const uint32_t left = stages + s * kNsStageBytes, right = left + 2 * kPanelHalf;
-          const uint32_t acc = tmem + buf * kColumns;
-#pragma unroll
-          for (int part = 0; part < 3; ++part) { // lo hi, hi lo, hi hi
-            const uint32_t l = left + (part == 0 ? kPanelHalf : 0), r = right + (part == 1 ? kPanelHalf : 0);
-#pragma unroll
-            for (int step = 0; step < 4; ++step) { // 16 of K
-              const uint64_t da = operand_desc(l + step * 32, 16, 1024);
-              const uint64_t db = WHAT == kApply ? operand_desc(r + step * 2048, kPanelHalf / 2, 1024)
-                                                 : operand_desc(r + step * 32, 16, 1024);
-              mma_f16<1>(acc, da, db, desc, !(first && part == 0 && step == 0));
-            }
-          }
-          mma_commit<1>(smem_address(&empty[s]));
-          if (k % kNsChunk == kNsChunk - 1 || k + 1 == at.k_blocks) {
-            mma_commit<1>(smem_address(&acc_full[buf]));
-            ++round;
-          }
-        }
+  }
+  return true;
+}
+
+// ---- the thread that issues the products (in the second CTA of a pair: passes on that its half is there)
+template <int CTAS, int WHAT>
+__device__ bool ns_multiply(const MuonTable &t, NsShared &sh, NsRing &ring) {
+  constexpr unsigned kColumns = 128 * CTAS;
+  const bool narrow = CTAS == 1 && t.narrow[WHAT];
+  for (unsigned tile = blockIdx.x / CTAS; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
+    NsTile at;
+    tile_at<CTAS, WHAT>(t, tile, at);
+    const unsigned j_diagonal = narrow ? at.j / 2 : at.j;
+    for (unsigned k = 0; k < at.k_blocks; ++k, ++ring.it) {
+      const unsigned s = ring.it % kNsStages, phase = (ring.it / kNsStages) & 1, buf = ring.round & 1;
+      if (CTAS > 1 && ring.rank != 0) {
+        if (!barrier_wait(smem_address(&sh.full[s]), phase, &sh.gave_up)) return false;
+        barrier_arrive_at(smem_address(&sh.peer_full[s]), 0);
+        continue;
       }
-      if (!ok) {
-        mma_commit<1>(smem_address(&drained));
-        const long long start = clock64();
-        while (!barrier_try(smem_address(&drained), 0) && clock64() - start < 10000000) {}
+      const bool flip_left = WHAT != kGram && k / (2 * CTAS) < at.i;
+      const bool flip_right = WHAT == kApply || (WHAT == kPolynomial && k / (2 * CTAS) < j_diagonal);
+      const bool first = k % kNsChunk == 0;
+      if (first && !barrier_wait(smem_address(&sh.acc_empty[buf]), ((ring.round >> 1) & 1) ^ 1, &sh.gave_up)) return false;
+      if (!barrier_wait(smem_address(&sh.full[s]), phase, &sh.gave_up)) return false;
+      if (CTAS > 1 && !barrier_wait(smem_address(&sh.peer_full[s]), phase, &sh.gave_up)) return false;
+      tmem_fence_after();
+      const uint32_t left = ring.stages + s * kNsStageBytes, right = left + 2 * kPanelHalf;
+      const uint32_t acc = sh.tmem + buf * kColumns;
+      const uint32_t desc = mma_desc(128 * CTAS, ns_wide<CTAS>(narrow), flip_left, flip_right);
+      // 16 of K: 32 bytes along K-major rows, or 16 rows of 128 bytes
+      const unsigned left_step = flip_left ? 2048 : 32, right_step = flip_right ? 2048 : 32;
+#pragma unroll
+      for (int part = 0; part < 3; ++part) { // lo hi, hi lo, hi hi
+        const uint32_t l = left + (part == 0 ? kPanelHalf : 0), r = right + (part == 1 ? kPanelHalf : 0);
+#pragma unroll
+        for (int step = 0; step < 4; ++step)
+          mma_f16<CTAS>(acc, operand_desc(l + step * left_step, kPanelHalf / 2, 1024),
+                        operand_desc(r + step * right_step, kPanelHalf / 2, 1024), desc, !(first && part == 0 && step == 0));
+      }
+      mma_commit<CTAS>(smem_address(&sh.empty[s]));
+      if (k % kNsChunk == kNsChunk - 1 || k + 1 == at.k_blocks) {
+        mma_commit<CTAS>(smem_address(&sh.acc_full[buf]));
+        ++ring.round;
       }
     }
-  } else { // ---- accumulators to results: warp w takes rows 32 (w % 4) .. and columns 64 (w / 4) ..
-    const unsigned row_in_tile = (warp & 3) * 32 + lane, half = warp >> 2;
-    unsigned round = 0;
-    bool ok = true;
-    for (unsigned tile = blockIdx.x; ok && tile < t.total; tile += gridDim.x) {
-      NsTile at;
-      const MuonMat &q = tile_at<WHAT>(t, tile, at);
-      float acc[64];
-      const unsigned rounds = (at.k_blocks + kNsChunk - 1) / kNsChunk;
-      for (unsigned c = 0; c < rounds; ++c, ++round) {
-        const unsigned buf = round & 1;
-        ok = __all_sync(0xffffffffu, barrier_wait(smem_address(&acc_full[buf]), (round >> 1) & 1, &gave_up));
-        if (!ok) break;
-        tmem_fence_after();
+  }
+  return true;
+}
+
+// ---- the warps that drain: warp w takes rows 32 (w % 4) .. and half of the tile's columns
+template <int CTAS, int WHAT>
+__device__ bool ns_drain(const MuonTable &t, int from, bool last, NsShared &sh, NsRing &ring, float *turn) {
+  constexpr unsigned kColumns = 128 * CTAS;
+  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned row_in_tile = (warp & 3) * 32 + lane, half = warp >> 2;
+  const bool narrow = CTAS == 1 && t.narrow[WHAT];
+  const unsigned pieces = narrow ? 2 : 4 * CTAS; // of 16 columns
+  for (unsigned tile = blockIdx.x / CTAS; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
+    NsTile at;
+    const MuonMat &q = tile_at<CTAS, WHAT>(t, tile, at);
+    float acc[64 * CTAS];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float v[32];
-          tmem_load32(tmem + (((warp & 3) * 32) << 16) + buf * kColumns + half * 64 + h * 32, v);
+    for (int i = 0; i < 64 * CTAS; ++i) acc[i] = 0.0f;
+    const unsigned rounds = (at.k_blocks + kNsChunk - 1) / kNsChunk;
+#pragma unroll 1
+    for (unsigned c = 0; c < rounds; ++c, ++ring.round) {
+      const unsigned buf = ring.round & 1;
+      if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_full[buf]), (ring.round >> 1) & 1, &sh.gave_up))) return false;
+      tmem_fence_after();
+      const uint32_t columns = sh.tmem + (((warp & 3) * 32) << 16) + buf * kColumns + half * pieces * 16;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) acc[h * 32 + i] = c == 0 ? v[i] : acc[h * 32 + i] + v[i];
-        }
-        tmem_fence_before();
-        __syncwarp();
-        if (lane == 0) barrier_arrive(smem_address(&acc_empty[buf]));
+      for (int h = 0; h < 4 * CTAS; ++h) {
+        if (h >= pieces) continue;
+        float v[16];
+        tmem_load16(columns + h * 16, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[h * 16 + i] += v[i];
       }
-      if (!ok) break;
-      // the warp's 64 columns are one block column of the result
-      const unsigned width = WHAT == kApply ? q.n : q.m;
-      const unsigned col_blocks = panel_col_blocks(width), cb = 2 * at.j + half;
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (ring.rank == 0) barrier_arrive(smem_address(&sh.acc_empty[buf]));
+        else barrier_arrive_at(smem_address(&sh.acc_empty[buf]), 0);
+      }
+    }
+    const unsigned width = WHAT == kApply ? q.n : q.m, rb = at.i * CTAS + ring.rank;
+    const unsigned col_blocks = panel_col_blocks(width);
+    if (rb >= panel_row_blocks(q.m)) continue;
+    const char *old = WHAT == kPolynomial ? q.a : q.x[from]; // the linear term
+    char *out = WHAT == kGram ? q.a : WHAT == kPolynomial ? q.b : q.x[from ^ 1];
+    const unsigned row = rb * 128 + row_in_tile;
+    // 32 columns at a time: half of a block column. All its loads are issued before its stores: the
+    // compiler cannot move a load over a store that may alias it, and a load waits for L2.
+#pragma unroll
+    for (int g = 0; g < 2 * CTAS; ++g) {
+      if (g * 2 >= pieces) continue;
+      const unsigned col0 = at.j * ns_wide<CTAS>(narrow) + (half * pieces + g * 2) * 16;
+      const unsigned cb = col0 / kPanelCols, chunk0 = (col0 % kPanelCols) / 8;
       if (cb >= col_blocks) continue;
-      const u64 offset = panel_block(at.i, cb, col_blocks);
-      const char *old = WHAT == kPolynomial ? q.a : q.x[from]; // the linear term
-      char *out = WHAT == kGram ? q.a : WHAT == kPolynomial ? q.b : q.x[from ^ 1];
+      const u64 offset = panel_block(rb, cb, col_blocks);
+      float v[32];
 #pragma unroll
-      for (int chunk = 0; chunk < 8; ++chunk) {
-        const u64 here = offset + panel_chunk(row_in_tile, chunk);
-        float v[8];
+      for (int i = 0; i < 32; ++i) v[i] = acc[g * 32 + i] * kSplitUnscale;
+      if (WHAT != kGram) {
+        uint4 hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = acc[chunk * 8 + i] * kSplitUnscale;
-        if (WHAT != kGram) {
-          float z[8];
-          join8(*reinterpret_cast<const uint4 *>(old + here), *reinterpret_cast<const uint4 *>(old + here + kPanelHalf), z);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            v[i] = WHAT == kPolynomial ? __fmaf_rn(kNsB, z[i], kNsC * v[i]) : __fmaf_rn(kNsA, z[i], v[i]);
+        for (int c = 0; c < 4; ++c) {
+          const char *here = old + offset + panel_chunk(row_in_tile, chunk0 + c);
+          hi[c] = *reinterpret_cast<const uint4 *>(here);
+          lo[c] = *reinterpret_cast<const uint4 *>(here + kPanelHalf);
         }
-        if (WHAT != kApply || !last) {
-          uint4 hi, lo;
-          split8(v, hi, lo);
-          *reinterpret_cast<uint4 *>(out + here) = hi;
-          *reinterpret_cast<uint4 *>(out + here + kPanelHalf) = lo;
-        } else {
-          const unsigned row = at.i * 128 + row_in_tile;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float z[8];
+          join8(hi[c], lo[c], z);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const unsigned col = cb * kPanelCols + chunk * 8 + i;
-            if (row >= q.m || col >= q.n) continue;
-            float *w = q.w + (q.rows <= q.cols ? (u64)row * q.n + col : (u64)col * q.m + row);
-            const float x = g_ns_gave_up ? NAN : v[i] * kSplitUnscale;
-            *w = q.keep == 0.0f ? -q.rate * x : __fmaf_rn(-q.rate, x, q.keep * *w);
+            float &r = v[c * 8 + i];
+            r = WHAT == kPolynomial ? __fmaf_rn(kNsB, z[i], kNsC * r) : __fmaf_rn(kNsA, z[i], r);
           }
         }
       }
+      if (WHAT != kApply || !last) {
+        if (row >= q.m) { // padding stays zero (an operand read from beyond the panel may leave anything here)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint4 hi, lo;
+          split8(v + c * 8, hi, lo);
+          char *here = out + offset + panel_chunk(row_in_tile, chunk0 + c);
+          *reinterpret_cast<uint4 *>(here) = hi;
+          *reinterpret_cast<uint4 *>(here + kPanelHalf) = lo;
+        }
+        continue;
+      }
+      // the weights (or the output), 32 neighbours to an access: where the matrix was turned, the lanes'
+      // rows are neighbours as they are, else a piece is turned in shared memory first
+      const float scale = g_ns_gave_up ? NAN : kSplitUnscale * q.rate;
+      if (q.rows > q.cols) {
+        if (row < q.m)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (col0 + i < q.n) {
+              float *w = q.w + (u64)(col0 + i) * q.m + row;
+              *w = q.keep == 0.0f ? -scale * v[i] : __fmaf_rn(-scale, v[i], q.keep * *w);
+            }
+      } else {
+        float *mine = turn + warp * (32 * 33);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mine[lane * 33 + i] = v[i];
+        __syncwarp();
+        const unsigned row0 = rb * 128 + (warp & 3) * 32, col = col0 + lane;
+        if (col < q.n)
+#pragma unroll 8
+          for (int r = 0; r < 32; ++r)
+            if (row0 + r < q.m) {
+              float *w = q.w + (u64)(row0 + r) * q.n + col;
+              *w = q.keep == 0.0f ? -scale * mine[r * 33 + lane] : __fmaf_rn(-scale, mine[r * 33 + lane], q.keep * *w);
+            }
+        __syncwarp();
+      }
     }
   }
+  return true;
+}
+
+// Barriers and tensor memory at the start and end of a kernel of products.
+template <int CTAS>
+__device__ __forceinline__ void ns_begin(NsShared &sh) {
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kNsStages; ++s) {
+      barrier_init(smem_address(&sh.full[s]), 1);
+      barrier_init(smem_address(&sh.peer_full[s]), 1);
+      barrier_init(smem_address(&sh.empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      barrier_init(smem_address(&sh.acc_full[b]), 1);
+      barrier_init(smem_address(&sh.acc_empty[b]), kNsEpilogueWarps * CTAS);
+    }
+    barrier_init(smem_address(&sh.drained), 1);
+    sh.gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  if (threadIdx.x >> 5 == kNsEpilogueWarps + 1) tmem_alloc<CTAS>(smem_address(&sh.tmem), 2 * 128 * CTAS);
+  tmem_fence_before();
+  __syncthreads();
+  if (CTAS > 1) cluster_sync_all(); // the other CTA's barriers exist
+  tmem_fence_after();
+}
+template <int CTAS>
+__device__ __forceinline__ void ns_end(NsShared &sh) {
   __syncwarp();
   tmem_fence_before();
   __syncthreads();
+  if (CTAS > 1) cluster_sync_all(); // nothing of this CTA is used by the other one any more
   tmem_fence_after();
-  if (threadIdx.x == 0 && gave_up) atomicOr(&g_ns_gave_up, 1u);
-  if (warp == kNsEpilogueWarps + 1) tmem_free<1>(tmem, 2 * kColumns);
+  if (threadIdx.x == 0 && sh.gave_up) atomicOr(&g_ns_gave_up, 1u);
+  if (threadIdx.x >> 5 == kNsEpilogueWarps + 1) tmem_free<CTAS>(sh.tmem, 2 * 128 * CTAS);
+}
+// After a wait that ran out: copies (or products) in flight end before shared and tensor memory go away.
+__device__ __forceinline__ void ns_abandon_loads(NsShared &sh, const NsRing &ring) {
+  for (unsigned back = 1; back <= kNsStages && back <= ring.it; ++back) {
+    const unsigned i = ring.it - back, s = i % kNsStages, phase = (i / kNsStages) & 1;
+    const long long start = clock64();
+    while (!barrier_try(smem_address(&sh.full[s]), phase) && clock64() - start < 10000000) {}
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void ns_abandon_products(NsShared &sh) {
+  mma_commit<CTAS>(smem_address(&sh.drained));
+  const long long start = clock64();
+  while (!barrier_try(smem_address(&sh.drained), 0) && clock64() - start < 10000000) {}
+}
+
+// One product over all matrices.
+template <int CTAS, int WHAT>
+__global__ void __launch_bounds__(kNsThreads, 1) muon_product_kernel(const __grid_constant__ MuonTable t, int from, int last) {
+  extern __shared__ char dynamic_smem[];
+  __shared__ __align__(8) NsShared sh;
+  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  NsRing ring = {(smem_address(dynamic_smem) + 1023) & ~1023u, CTAS == 1 ? 0 : blockIdx.x % CTAS, 0, 0};
+  float *turn = reinterpret_cast<float *>(dynamic_smem + kNsStages * kNsStageBytes + 1024);
+  ns_begin<CTAS>(sh);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (warp == kNsEpilogueWarps) {
+    if (lane == 0) {
+      asm volatile("fence.proxy.async;" ::: "memory"); // the panels were written with plain stores
+      if (!ns_load<CTAS, WHAT>(t, from, sh, ring)) ns_abandon_loads(sh, ring);
+    }
+  } else if (warp == kNsEpilogueWarps + 1) {
+    if (lane == 0 && !ns_multiply<CTAS, WHAT>(t, sh, ring) && ring.rank == 0) ns_abandon_products<CTAS>(sh);
+  } else {
+    ns_drain<CTAS, WHAT>(t, from, last != 0, sh, ring, turn);
+  }
+  ns_end<CTAS>(sh);
+}
+
+// ---- all steps in one launch ---------------------------------------------------------------------------
+// For matrices whose products are short a launch per product is most of the time (measured: 10 to 13
+// us a product of 256 x 640). Here one cooperative grid goes through all of them; a product starts
+// when every CTA has stored its tiles of the one before (a counter in global memory).
+__device__ __forceinline__ void grid_arrive(unsigned *arrived) {
+  __threadfence();
+  asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(arrived) : "memory");
+}
+__device__ __forceinline__ bool grid_wait(const unsigned *arrived, unsigned target, volatile unsigned *gave_up) {
+  const long long start = clock64();
+  for (unsigned spins = 0;; ++spins) {
+    unsigned now;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(arrived) : "memory");
+    if (now >= target) return true;
+    if ((spins & 255) == 255) {
+      if (*gave_up) return false;
+      if (clock64() - start > kWaitCycles) {
+        *gave_up = 1;
+        return false;
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_constant__ MuonTable t, int steps) {
+  extern __shared__ char dynamic_smem[];
+  __shared__ __align__(8) NsShared sh;
+  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  NsRing ring = {(smem_address(dynamic_smem) + 1023) & ~1023u, 0, 0, 0};
+  float *turn = reinterpret_cast<float *>(dynamic_smem + kNsStages * kNsStageBytes + 1024);
+  ns_begin<1>(sh);
+  if (warp == kNsEpilogueWarps) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int s = 0; ok && s < steps; ++s) {
+        const int from = s & 1;
+        ok = grid_wait(t.arrived, 3 * s * gridDim.x, &sh.gave_up);
+        asm volatile("fence.proxy.async;" ::: "memory"); // panels are written with plain stores
+        ok = ok && ns_load<1, kGram>(t, from, sh, ring) && grid_wait(t.arrived, (3 * s + 1) * gridDim.x, &sh.gave_up);
+        asm volatile("fence.proxy.async;" ::: "memory");
+        ok = ok && ns_load<1, kPolynomial>(t, from, sh, ring) && grid_wait(t.arrived, (3 * s + 2) * gridDim.x, &sh.gave_up);
+        asm volatile("fence.proxy.async;" ::: "memory");
+        ok = ok && ns_load<1, kApply>(t, from, sh, ring);
+      }
+      if (!ok) ns_abandon_loads(sh, ring);
+    }
+  } else if (warp == kNsEpilogueWarps + 1) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int s = 0; ok && s < steps; ++s)
+        ok = ns_multiply<1, kGram>(t, sh, ring) && ns_multiply<1, kPolynomial>(t, sh, ring) && ns_multiply<1, kApply>(t, sh, ring);
+      if (!ok) ns_abandon_products<1>(sh);
+    }
+  } else {
+    // The draining warps read what other CTAs stored (the linear term), so they wait for the grid too.
+    // After a wait that ran out they go on through the block's barriers, all of them, without work.
+    auto live = [&] { return !__any_sync(0xffffffffu, sh.gave_up != 0); };
+    auto next = [&](unsigned product) {
+      asm volatile("fence.proxy.async;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"r"(kNsEpilogueWarps * 32) : "memory");
+      if (threadIdx.x == 0 && !sh.gave_up) {
+        grid_arrive(t.arrived);
+        grid_wait(t.arrived, product * gridDim.x, &sh.gave_up);
+      }
+      asm volatile("bar.sync 1, %0;" ::"r"(kNsEpilogueWarps * 32) : "memory");
+    };
+    for (int s = 0; s < steps; ++s) {
+      const int from = s & 1;
+      if (live()) ns_drain<1, kGram>(t, from, false, sh, ring, turn);
+      next(3 * s + 1);
+      if (live()) ns_drain<1, kPolynomial>(t, from, false, sh, ring, turn);
+      next(3 * s + 2);
+      if (live()) ns_drain<1, kApply>(t, from, s + 1 == steps, sh, ring, turn);
+      if (s + 1 < steps) next(3 * s + 3);
+    }
+  }
+  ns_end<1>(sh);
 }
 
 // steps == 0: X itself
@@ -420,43 +663,83 @@ static bool launch_over(MuonTable &t, Blocks blocks, void (*kernel)(const MuonTa
   number(t, blocks);
   return launched(launch_k(kernel, dim3(t.total), dim3(kMuonThreads), 0, stream(), t));
 }
-template <int WHAT>
+template <int CTAS> static void number_tiles(MuonTable &t) {
+  for (int what = kGram; what <= kApply; ++what) {
+    u64 n = 0;
+    for (int i = 0; i < t.count; ++i) {
+      t.mat[i].first_tile[what] = (unsigned)n;
+      n += ns_tiles_of<CTAS>(t.mat[i], what, t.narrow[what]);
+    }
+    t.tiles[what] = (unsigned)n;
+  }
+}
+template <int CTAS, int WHAT>
 static bool launch_product(MuonTable &t, int from, int last) {
-  number(t, [](const MuonMat &q) {
-    return (u64)panel_row_blocks(q.m) * panel_row_blocks(WHAT == kApply ? q.n : q.m);
-  });
-  const cudaError_t e = cudaFuncSetAttribute(muon_product_kernel<WHAT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem);
+  const auto kernel = muon_product_kernel<CTAS, WHAT>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem);
   if (e != cudaSuccess) return launched(e);
-  const unsigned grid = t.total < (unsigned)sm_count() ? t.total : (unsigned)sm_count();
-  return launched(launch_k(muon_product_kernel<WHAT>, dim3(grid), dim3(kNsThreads), kNsSmem, stream(), t, from, last));
+  const unsigned most = (unsigned)sm_count() / CTAS, grid = std::min(t.tiles[WHAT], most) * CTAS;
+  return launched(launch_kc(CTAS, kernel, dim3(grid), dim3(kNsThreads), kNsSmem, stream(), t, from, last));
+}
+// Tiles of 256 x 256 by pairs of CTAs, a launch per product.
+static void run_pairs(MuonTable &t, int steps) {
+  for (int &narrow : t.narrow) narrow = 0;
+  number_tiles<2>(t);
+  for (int s = 0; s < steps; ++s) {
+    const int from = s & 1;
+    if (!launch_product<2, kGram>(t, from, 0) || !launch_product<2, kPolynomial>(t, from, 0) ||
+        !launch_product<2, kApply>(t, from, s + 1 == steps))
+      return;
+  }
+}
+// Tiles of 128 x 128 (128 x 64 where that still leaves one each), all steps in one launch.
+static void run_fused(MuonTable &t, int steps) {
+  const unsigned sms = (unsigned)sm_count();
+  for (int what = kGram; what <= kApply; ++what) {
+    u64 n = 0;
+    for (int i = 0; i < t.count; ++i) n += ns_tiles_of<1>(t.mat[i], what, true);
+    t.narrow[what] = n <= sms;
+  }
+  number_tiles<1>(t);
+  const unsigned tiles = std::max(t.tiles[kGram], std::max(t.tiles[kPolynomial], t.tiles[kApply]));
+  cudaError_t e = cudaFuncSetAttribute(muon_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem);
+  if (e == cudaSuccess) {
+    void *args[] = {&t, &steps};
+    e = cudaLaunchCooperativeKernel((const void *)muon_steps_kernel, dim3(std::min(tiles, sms)), dim3(kNsThreads), args, kNsSmem, stream());
+  }
+  launched(e);
 }
 
 // One group of matrices whose scratch is `base`.
 static void run_group(MuonTable &t, char *base, int steps) {
+  auto take = [&](u64 bytes) {
+    char *p = base;
+    base += bytes;
+    return p;
+  };
   for (int i = 0; i < t.count; ++i) {
     MuonMat &q = t.mat[i];
-    auto take = [&](u64 bytes) {
-      char *p = base;
-      base += bytes;
-      return p;
-    };
     q.x[0] = take(panel_bytes(q.m, q.n));
     q.x[1] = take(panel_bytes(q.m, q.n));
     q.a = take(panel_bytes(q.m, q.m));
     q.b = take(panel_bytes(q.m, q.m));
     q.partial = (double *)take(padded((u64)(q.chunks + 1) * 8));
   }
+  t.arrived = (unsigned *)take(256);
   auto chunks = [](const MuonMat &q) { return (u64)q.chunks; };
   auto blocks = [](const MuonMat &q) { return (u64)panel_row_blocks(q.m) * panel_col_blocks(q.n); };
   if (!launch_over(t, chunks, muon_momentum_kernel)) return;
   if (!launch_over(t, [](const MuonMat &) { return (u64)1; }, muon_norm_kernel)) return;
   if (!launch_over(t, blocks, muon_load_kernel)) return;
-  for (int s = 0; s < steps; ++s) {
-    const int from = s & 1, last = s + 1 == steps;
-    if (!launch_product<kGram>(t, from, 0) || !launch_product<kPolynomial>(t, from, 0) || !launch_product<kApply>(t, from, last))
-      return;
+  if (steps > 0) {
+    u64 tiles = 0;
+    for (int i = 0; i < t.count; ++i) tiles += ns_tiles_of<2>(t.mat[i], kApply, false);
+    const bool pairs = tuned(kTuneMuonPairs) >= 0 ? tuned(kTuneMuonPairs) != 0 : tiles >= (u64)sm_count() / 2;
+    if (pairs) run_pairs(t, steps);
+    else run_fused(t, steps);
+    return;
   }
-  if (steps == 0) launch_over(t, chunks, muon_store_kernel);
+  launch_over(t, chunks, muon_store_kernel);
 }
 
 // All matrices, in groups that share one piece of scratch.
@@ -464,7 +747,7 @@ static void run_matrices(const std::vector<MuonMat> &mats, float mu, float epsil
   u64 largest = 0;
   std::vector<size_t> ends;
   for (size_t i = 0; i < mats.size();) {
-    u64 bytes = 0;
+    u64 bytes = 256; // the grid barrier
     size_t k = i;
     while (k < mats.size() && k - i < (size_t)kMuonMax && (k == i || bytes + scratch_bytes(mats[k]) <= kMuonScratch))
       bytes += scratch_bytes(mats[k++]);

@@ -13,6 +13,15 @@ pytestmark = pytest.mark.gpu
 U = R.U
 
 
+@pytest.fixture(autouse=True, params=["built_in", "fused", "pairs"])
+def route(request):
+    """Every test by the built-in choice, by the fused steps and by the pairs of CTAs."""
+    pb.lib.plast_b200_tune(12, {"built_in": -1, "fused": 0, "pairs": 1}[request.param])
+    yield request.param
+    pb.lib.plast_b200_tune(12, -1)
+    assert pb.lib.plast_b200_muon_status() == 0
+
+
 def tolerance(m, steps=5):
     """Frobenius error relative to the result's. A product whose terms carry 2^-22 adds at most about 20 * 2^-22 of
     |X|_F per step (3.4 + 4.8 * 1.45 + 2 * 2.03 * 2.1, times 1.2, rounded up); an error grows at most by
