@@ -23,7 +23,8 @@
 namespace pb {
 
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
-constexpr int kMuonMax = 32;                       // matrices per launch
+constexpr int kMuonMax = 32;                       // matrices per launch (256 bytes hold their counters)
+static_assert(kMuonMax * sizeof(unsigned) <= 256, "");
 constexpr u64 kMuonScratch = (u64)2 << 30;         // scratch of one group of matrices
 constexpr int kMuonThreads = 256;
 constexpr int kMuonChunk = kMuonThreads * 16;      // elements per CTA of the momentum pass
@@ -38,7 +39,7 @@ struct MuonMat {
   unsigned rows, cols; // as stored
   unsigned m, n;       // m <= n
   unsigned first;      // first CTA of this matrix in the launch at hand
-  unsigned first_tile[3]; // first tile of this matrix in the products gram, polynomial, apply
+  unsigned first_tile[3], tiles[3]; // of this matrix in the products gram, polynomial, apply
   unsigned chunks;
 };
 struct MuonTable {
@@ -47,7 +48,7 @@ struct MuonTable {
   unsigned total;     // CTAs of the launch at hand
   unsigned tiles[3];  // of each product
   int narrow[3];      // tiles of 128 x 64 instead of 128 x 128
-  unsigned *arrived;  // grid barrier of the fused steps
+  unsigned *stored;   // per matrix: warps that have stored their part of a tile, over all products so far
   float mu, epsilon;
   int nesterov;
 };
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(kMuonThreads) muon_norm_kernel(const __grid_co
   }
   if (threadIdx.x == 0) {
     q.partial[0] = part[0];
-    if (blockIdx.x == 0) *t.arrived = 0; // for the grid barrier of the steps
+    t.stored[blockIdx.x] = 0; // for the steps
   }
 }
 
@@ -165,12 +166,17 @@ __global__ void __launch_bounds__(kMuonThreads) muon_load_kernel(const __grid_co
 // A and B are symmetric: only tiles on and above the diagonal are computed and stored. An operand
 // block below it is fetched as the block above it and read MN-major, which is its transpose.
 //
-// A persistent CTA walks tiles of 128 x 128 (or 128 x 64); a pair of CTAs (CTAS = 2) walks tiles of
-// 256 x 256, each CTA holding half of either operand. One thread brings 64 KB stages (64 of K, hi and
-// lo of both operands) with bulk copies, one thread (of the pair) issues the twelve tcgen05.mma of a
-// stage, small products first, and eight warps drain the accumulators. Tensor-core accumulation
-// truncates; every kNsChunk stages the accumulator (one of two in tensor memory) is therefore added in
-// fp32 registers, rounded to nearest, while the next one fills.
+// One launch goes through all products of all matrices. A persistent CTA takes every gridDim-th tile,
+// of 128 x 128 (or 128 x 64); a pair of CTAs (CTAS = 2) tiles of 256 x 256, each CTA holding half of
+// either operand. One thread brings 64 KB stages (64 of K, hi and lo of both operands) with bulk
+// copies, one warp (of the pair) issues the twelve tcgen05.mma of a stage, small products first, and
+// eight warps drain the accumulators. Tensor-core accumulation truncates; every kNsChunk stages the
+// accumulator (one of two in tensor memory) is therefore added in fp32 registers, rounded to nearest,
+// while the next one fills.
+//
+// A product of a matrix starts when all tiles of its product before are stored, which a counter per
+// matrix in global memory tells; the tiles of other matrices do not wait. The grid is launched
+// cooperatively (all of it is resident, so the waits end) and every wait is limited.
 enum MuonProduct { kGram = 0, kPolynomial = 1, kApply = 2 };
 constexpr int kNsStages = 3;
 constexpr unsigned kNsStageBytes = 4 * kPanelHalf; // left hi, left lo, right hi, right lo
@@ -179,7 +185,7 @@ constexpr int kNsEpilogueWarps = 8, kNsThreads = (kNsEpilogueWarps + 2) * 32;
 #define NS_CHUNK 2
 #endif
 constexpr int kNsChunk = NS_CHUNK;
-constexpr unsigned kNsTurnBytes = kNsEpilogueWarps * 32 * 33 * 4; // a 32 x 32 piece per warp, to store rows in order
+constexpr unsigned kNsTurnBytes = kNsEpilogueWarps * 32 * 17 * 4; // a 32 x 16 piece per warp, to store rows in order
 constexpr unsigned kNsSmem = kNsStages * kNsStageBytes + 1024 + kNsTurnBytes;
 
 __device__ unsigned g_ns_gave_up; // a wait ran out: results are NaN from then on, see plast_b200_muon_status
@@ -198,7 +204,7 @@ struct NsTile {
 };
 template <int CTAS, int WHAT>
 __device__ __forceinline__ const MuonMat &tile_at(const MuonTable &t, unsigned tile, NsTile &out) {
-  int lo = 0, hi = t.count - 1;
+  int lo = 0, hi = t.count - 1; // the last matrix whose first tile is not beyond
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (t.mat[mid].first_tile[WHAT] <= tile) lo = mid; else hi = mid - 1;
@@ -261,21 +267,54 @@ struct NsShared {
   uint64_t full[kNsStages], peer_full[kNsStages], empty[kNsStages], acc_full[2], acc_empty[2], drained;
   uint32_t tmem;
   volatile unsigned gave_up;
+  MuonTable table; // a copy: the roles index it at every tile, which is slow in constant memory
 };
 // A role's place in the rings of stages and accumulators, kept from one product to the next.
 struct NsRing {
   uint32_t stages; // shared memory
   unsigned rank;   // in the pair
+  unsigned first;  // this CTA's (pair's) first tile of the product at hand
   unsigned it, round;
 };
 
+// Waits until matrix q's products up to this one (step s, product what) are stored. Relaxed polling, then
+// one fence: an acquiring load would fence at every turn.
+template <int CTAS, int WHAT>
+__device__ __forceinline__ bool ns_wait_stored(const MuonTable &t, const MuonMat &q, int s, volatile unsigned *gave_up) {
+  unsigned target = s * (q.tiles[0] + q.tiles[1] + q.tiles[2]);
+  if (WHAT > kGram) target += q.tiles[kGram];
+  if (WHAT > kPolynomial) target += q.tiles[kPolynomial];
+  target *= CTAS * kNsEpilogueWarps;
+  const unsigned *counter = t.stored + (&q - t.mat);
+  long long start = 0;
+  for (unsigned spins = 0;; ++spins) {
+    unsigned now;
+    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(counter) : "memory");
+    if (now >= target) break;
+    if (spins == 0) start = clock64();
+    if ((spins & 63) == 63) {
+      if (*gave_up) return false;
+      if (clock64() - start > kWaitCycles) {
+        *gave_up = 1;
+        return false;
+      }
+    }
+  }
+  asm volatile("fence.acq_rel.gpu;" ::: "memory");
+  return true;
+}
+
 // ---- the thread that loads
 template <int CTAS, int WHAT>
-__device__ bool ns_load(const MuonTable &t, int from, NsShared &sh, NsRing &ring) {
+__device__ bool ns_load(NsShared &sh, NsRing &ring, int s) {
+  const MuonTable &t = sh.table;
+  const int from = s & 1;
   const bool narrow = CTAS == 1 && t.narrow[WHAT];
-  for (unsigned tile = blockIdx.x / CTAS; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
+  for (unsigned tile = ring.first; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
     NsTile at;
     const MuonMat &q = tile_at<CTAS, WHAT>(t, tile, at);
+    if (!ns_wait_stored<CTAS, WHAT>(t, q, s, &sh.gave_up)) return false;
+    asm volatile("fence.proxy.async.global;" ::: "memory"); // panels are written with plain stores
     const unsigned rows = panel_row_blocks(q.m), xcb = panel_col_blocks(q.n), mcb = panel_col_blocks(q.m);
     const char *left = WHAT == kGram ? q.x[from] : WHAT == kPolynomial ? q.a : q.b;
     const char *right = WHAT == kPolynomial ? q.a : q.x[from];
@@ -283,11 +322,11 @@ __device__ bool ns_load(const MuonTable &t, int from, NsShared &sh, NsRing &ring
     const unsigned i = at.i * CTAS + ring.rank, j = at.j * CTAS + ring.rank;
     const unsigned j_diagonal = narrow ? at.j / 2 : at.j;
     for (unsigned k = 0; k < at.k_blocks; ++k, ++ring.it) {
-      const unsigned s = ring.it % kNsStages, phase = (ring.it / kNsStages) & 1;
+      const unsigned st = ring.it % kNsStages, phase = (ring.it / kNsStages) & 1;
       const bool flip_left = WHAT != kGram && k / (2 * CTAS) < at.i;
       const bool flip_right = WHAT == kApply || (WHAT == kPolynomial && k / (2 * CTAS) < j_diagonal);
-      if (!barrier_wait(smem_address(&sh.empty[s]), phase ^ 1, &sh.gave_up)) return false;
-      const uint32_t bar = smem_address(&sh.full[s]), dst = ring.stages + s * kNsStageBytes;
+      if (!barrier_wait(smem_address(&sh.empty[st]), phase ^ 1, &sh.gave_up)) return false;
+      const uint32_t bar = smem_address(&sh.full[st]), dst = ring.stages + st * kNsStageBytes;
       barrier_expect(bar, operand_bytes(i, rows, left_cb, flip_left, false) + operand_bytes(j, rows, right_cb, flip_right, narrow));
       load_operand(dst, left, i, k, rows, left_cb, flip_left, false, bar);
       load_operand(dst + 2 * kPanelHalf, right, j, k, rows, right_cb, flip_right, narrow, bar);
@@ -296,47 +335,54 @@ __device__ bool ns_load(const MuonTable &t, int from, NsShared &sh, NsRing &ring
   return true;
 }
 
-// ---- the thread that issues the products (in the second CTA of a pair: passes on that its half is there)
+// ---- the warp that issues the products (in the second CTA of a pair: passes on that its half is there).
+// All lanes walk the loops together, so that descriptors stay in uniform registers; one lane issues.
 template <int CTAS, int WHAT>
-__device__ bool ns_multiply(const MuonTable &t, NsShared &sh, NsRing &ring) {
+__device__ bool ns_multiply(NsShared &sh, NsRing &ring) {
   constexpr unsigned kColumns = 128 * CTAS;
+  const MuonTable &t = sh.table;
   const bool narrow = CTAS == 1 && t.narrow[WHAT];
-  for (unsigned tile = blockIdx.x / CTAS; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
+  const uint32_t tmem = sh.tmem;
+  for (unsigned tile = ring.first; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
     NsTile at;
     tile_at<CTAS, WHAT>(t, tile, at);
     const unsigned j_diagonal = narrow ? at.j / 2 : at.j;
     for (unsigned k = 0; k < at.k_blocks; ++k, ++ring.it) {
-      const unsigned s = ring.it % kNsStages, phase = (ring.it / kNsStages) & 1, buf = ring.round & 1;
+      const unsigned st = ring.it % kNsStages, phase = (ring.it / kNsStages) & 1, buf = ring.round & 1;
+      if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.full[st]), phase, &sh.gave_up))) return false;
       if (CTAS > 1 && ring.rank != 0) {
-        if (!barrier_wait(smem_address(&sh.full[s]), phase, &sh.gave_up)) return false;
-        barrier_arrive_at(smem_address(&sh.peer_full[s]), 0);
+        if (elect_one()) barrier_arrive_at(smem_address(&sh.peer_full[st]), 0);
+        __syncwarp();
         continue;
       }
+      const bool first = k % kNsChunk == 0;
+      if (first && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_empty[buf]), ((ring.round >> 1) & 1) ^ 1, &sh.gave_up)))
+        return false;
+      if (CTAS > 1 && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.peer_full[st]), phase, &sh.gave_up))) return false;
+      tmem_fence_after();
       const bool flip_left = WHAT != kGram && k / (2 * CTAS) < at.i;
       const bool flip_right = WHAT == kApply || (WHAT == kPolynomial && k / (2 * CTAS) < j_diagonal);
-      const bool first = k % kNsChunk == 0;
-      if (first && !barrier_wait(smem_address(&sh.acc_empty[buf]), ((ring.round >> 1) & 1) ^ 1, &sh.gave_up)) return false;
-      if (!barrier_wait(smem_address(&sh.full[s]), phase, &sh.gave_up)) return false;
-      if (CTAS > 1 && !barrier_wait(smem_address(&sh.peer_full[s]), phase, &sh.gave_up)) return false;
-      tmem_fence_after();
-      const uint32_t left = ring.stages + s * kNsStageBytes, right = left + 2 * kPanelHalf;
-      const uint32_t acc = sh.tmem + buf * kColumns;
+      const uint32_t stage = ring.stages + st * kNsStageBytes;
+      const uint64_t left = operand_desc(stage, kPanelHalf / 2, 1024);
+      const uint64_t right = operand_desc(stage + 2 * kPanelHalf, kPanelHalf / 2, 1024);
+      const uint32_t acc = tmem + buf * kColumns;
       const uint32_t desc = mma_desc(128 * CTAS, ns_wide<CTAS>(narrow), flip_left, flip_right);
-      // 16 of K: 32 bytes along K-major rows, or 16 rows of 128 bytes
-      const unsigned left_step = flip_left ? 2048 : 32, right_step = flip_right ? 2048 : 32;
+      // 16 of K: 32 bytes along K-major rows, or 16 rows of 128 bytes; descriptors count in 16 bytes
+      const unsigned left_step = flip_left ? 128 : 2, right_step = flip_right ? 128 : 2;
+      const bool last = k % kNsChunk == kNsChunk - 1 || k + 1 == at.k_blocks;
+      if (elect_one()) {
 #pragma unroll
-      for (int part = 0; part < 3; ++part) { // lo hi, hi lo, hi hi
-        const uint32_t l = left + (part == 0 ? kPanelHalf : 0), r = right + (part == 1 ? kPanelHalf : 0);
+        for (int part = 0; part < 3; ++part) { // lo hi, hi lo, hi hi
+          const uint64_t l = left + (part == 0 ? kPanelHalf >> 4 : 0), r = right + (part == 1 ? kPanelHalf >> 4 : 0);
 #pragma unroll
-        for (int step = 0; step < 4; ++step)
-          mma_f16<CTAS>(acc, operand_desc(l + step * left_step, kPanelHalf / 2, 1024),
-                        operand_desc(r + step * right_step, kPanelHalf / 2, 1024), desc, !(first && part == 0 && step == 0));
+          for (int step = 0; step < 4; ++step)
+            mma_f16<CTAS>(acc, l + step * left_step, r + step * right_step, desc, !(first && part == 0 && step == 0));
+        }
+        mma_commit<CTAS>(smem_address(&sh.empty[st]));
+        if (last) mma_commit<CTAS>(smem_address(&sh.acc_full[buf]));
       }
-      mma_commit<CTAS>(smem_address(&sh.empty[s]));
-      if (k % kNsChunk == kNsChunk - 1 || k + 1 == at.k_blocks) {
-        mma_commit<CTAS>(smem_address(&sh.acc_full[buf]));
-        ++ring.round;
-      }
+      __syncwarp();
+      if (last) ++ring.round;
     }
   }
   return true;
@@ -344,13 +390,15 @@ __device__ bool ns_multiply(const MuonTable &t, NsShared &sh, NsRing &ring) {
 
 // ---- the warps that drain: warp w takes rows 32 (w % 4) .. and half of the tile's columns
 template <int CTAS, int WHAT>
-__device__ bool ns_drain(const MuonTable &t, int from, bool last, NsShared &sh, NsRing &ring, float *turn) {
+__device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, bool last, float *turn) {
   constexpr unsigned kColumns = 128 * CTAS;
+  const MuonTable &t = sh.table;
+  const int from = s & 1;
   const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned row_in_tile = (warp & 3) * 32 + lane, half = warp >> 2;
   const bool narrow = CTAS == 1 && t.narrow[WHAT];
-  const unsigned pieces = narrow ? 2 : 4 * CTAS; // of 16 columns
-  for (unsigned tile = blockIdx.x / CTAS; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
+  const unsigned groups = narrow ? 1 : 2 * CTAS; // of 32 columns
+  for (unsigned tile = ring.first; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
     NsTile at;
     const MuonMat &q = tile_at<CTAS, WHAT>(t, tile, at);
     float acc[64 * CTAS];
@@ -362,14 +410,14 @@ __device__ bool ns_drain(const MuonTable &t, int from, bool last, NsShared &sh, 
       const unsigned buf = ring.round & 1;
       if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_full[buf]), (ring.round >> 1) & 1, &sh.gave_up))) return false;
       tmem_fence_after();
-      const uint32_t columns = sh.tmem + (((warp & 3) * 32) << 16) + buf * kColumns + half * pieces * 16;
+      const uint32_t columns = sh.tmem + (((warp & 3) * 32) << 16) + buf * kColumns + half * groups * 32;
 #pragma unroll
-      for (int h = 0; h < 4 * CTAS; ++h) {
-        if (h >= pieces) continue;
-        float v[16];
-        tmem_load16(columns + h * 16, v);
+      for (int g = 0; g < 2 * CTAS; ++g) {
+        if (g >= groups) continue;
+        float v[32];
+        tmem_load32(columns + g * 32, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[h * 16 + i] += v[i];
+        for (int i = 0; i < 32; ++i) acc[g * 32 + i] += v[i];
       }
       tmem_fence_before();
       __syncwarp();
@@ -379,17 +427,23 @@ __device__ bool ns_drain(const MuonTable &t, int from, bool last, NsShared &sh, 
       }
     }
     const unsigned width = WHAT == kApply ? q.n : q.m, rb = at.i * CTAS + ring.rank;
-    const unsigned col_blocks = panel_col_blocks(width);
-    if (rb >= panel_row_blocks(q.m)) continue;
+    const unsigned col_blocks = panel_col_blocks(width), row_blocks = panel_row_blocks(q.m);
     const char *old = WHAT == kPolynomial ? q.a : q.x[from]; // the linear term
     char *out = WHAT == kGram ? q.a : WHAT == kPolynomial ? q.b : q.x[from ^ 1];
     const unsigned row = rb * 128 + row_in_tile;
+    // The linear term is other CTAs' work; the accumulators came after it was stored (the loads waited),
+    // which orders it for the thread that loaded: this warp looks for itself.
+    if (WHAT != kGram) {
+      bool ok = true;
+      if (lane == 0) ok = ns_wait_stored<CTAS, WHAT>(t, q, s, &sh.gave_up);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+    }
     // 32 columns at a time: half of a block column. All its loads are issued before its stores: the
     // compiler cannot move a load over a store that may alias it, and a load waits for L2.
 #pragma unroll
     for (int g = 0; g < 2 * CTAS; ++g) {
-      if (g * 2 >= pieces) continue;
-      const unsigned col0 = at.j * ns_wide<CTAS>(narrow) + (half * pieces + g * 2) * 16;
+      if (g >= groups || rb >= row_blocks) continue;
+      const unsigned col0 = at.j * ns_wide<CTAS>(narrow) + (half * groups + g) * 32;
       const unsigned cb = col0 / kPanelCols, chunk0 = (col0 % kPanelCols) / 8;
       if (cb >= col_blocks) continue;
       const u64 offset = panel_block(rb, cb, col_blocks);
@@ -399,10 +453,10 @@ __device__ bool ns_drain(const MuonTable &t, int from, bool last, NsShared &sh, 
       if (WHAT != kGram) {
         uint4 hi[4], lo[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 4; ++c) { // past L1, which may hold an earlier step's values
           const char *here = old + offset + panel_chunk(row_in_tile, chunk0 + c);
-          hi[c] = *reinterpret_cast<const uint4 *>(here);
-          lo[c] = *reinterpret_cast<const uint4 *>(here + kPanelHalf);
+          hi[c] = __ldcg(reinterpret_cast<const uint4 *>(here));
+          lo[c] = __ldcg(reinterpret_cast<const uint4 *>(here + kPanelHalf));
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -439,31 +493,44 @@ __device__ bool ns_drain(const MuonTable &t, int from, bool last, NsShared &sh, 
           for (int i = 0; i < 32; ++i)
             if (col0 + i < q.n) {
               float *w = q.w + (u64)(col0 + i) * q.m + row;
-              *w = q.keep == 0.0f ? -scale * v[i] : __fmaf_rn(-scale, v[i], q.keep * *w);
+              *w = q.keep == 0.0f ? -scale * v[i] : q.keep * *w - scale * v[i];
             }
       } else {
-        float *mine = turn + warp * (32 * 33);
+        float *mine = turn + warp * (32 * 17);
+        const unsigned row0 = rb * 128 + (warp & 3) * 32 + (lane >> 4);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mine[lane * 33 + i] = v[i];
-        __syncwarp();
-        const unsigned row0 = rb * 128 + (warp & 3) * 32, col = col0 + lane;
-        if (col < q.n)
+        for (int piece = 0; piece < 2; ++piece) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mine[lane * 17 + i] = v[piece * 16 + i];
+          __syncwarp();
+          const unsigned col = col0 + piece * 16 + (lane & 15);
+          if (col < q.n)
 #pragma unroll 8
-          for (int r = 0; r < 32; ++r)
-            if (row0 + r < q.m) {
-              float *w = q.w + (u64)(row0 + r) * q.n + col;
-              *w = q.keep == 0.0f ? -scale * mine[r * 33 + lane] : __fmaf_rn(-scale, mine[r * 33 + lane], q.keep * *w);
-            }
-        __syncwarp();
+            for (int r = 0; r < 32; r += 2)
+              if (row0 + r < q.m) {
+                float *w = q.w + (u64)(row0 + r) * q.n + col;
+                const float x = scale * mine[(r + (lane >> 4)) * 17 + (lane & 15)];
+                *w = q.keep == 0.0f ? -x : q.keep * *w - x;
+              }
+          __syncwarp();
+        }
       }
     }
+    __syncwarp();
+    if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(t.stored + (&q - t.mat)) : "memory");
   }
   return true;
 }
 
-// Barriers and tensor memory at the start and end of a kernel of products.
 template <int CTAS>
-__device__ __forceinline__ void ns_begin(NsShared &sh) {
+__global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_constant__ MuonTable param, int steps) {
+  extern __shared__ char dynamic_smem[];
+  __shared__ __align__(16) NsShared sh;
+  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (unsigned i = threadIdx.x; i < sizeof(MuonTable) / 4; i += kNsThreads)
+    reinterpret_cast<unsigned *>(&sh.table)[i] = reinterpret_cast<const unsigned *>(&param)[i];
+  NsRing ring = {(smem_address(dynamic_smem) + 1023) & ~1023u, CTAS == 1 ? 0 : blockIdx.x % CTAS, 0, 0, 0};
+  float *turn = reinterpret_cast<float *>(dynamic_smem + kNsStages * kNsStageBytes + 1024);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kNsStages; ++s) {
       barrier_init(smem_address(&sh.full[s]), 1);
@@ -479,138 +546,77 @@ __device__ __forceinline__ void ns_begin(NsShared &sh) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
-  if (threadIdx.x >> 5 == kNsEpilogueWarps + 1) tmem_alloc<CTAS>(smem_address(&sh.tmem), 2 * 128 * CTAS);
+  if (warp == kNsEpilogueWarps + 1) tmem_alloc<CTAS>(smem_address(&sh.tmem), 2 * 128 * CTAS);
   tmem_fence_before();
   __syncthreads();
   if (CTAS > 1) cluster_sync_all(); // the other CTA's barriers exist
   tmem_fence_after();
-}
-template <int CTAS>
-__device__ __forceinline__ void ns_end(NsShared &sh) {
+
+  // Tiles are numbered through all products, so that a product that ends between two turns of the grid
+  // leaves the next one's first tiles to the CTAs that are free.
+  const MuonTable &t = sh.table;
+  const unsigned workers = gridDim.x / CTAS, me = blockIdx.x / CTAS;
+  unsigned before = 0; // tiles of the products so far, modulo the number of workers
+  auto advance = [&](int what) { before = (before + t.tiles[what]) % workers; };
+  auto begin = [&] { ring.first = (me + workers - before) % workers; };
+  bool ok = true;
+  if (warp == kNsEpilogueWarps) {
+    if (lane == 0) {
+      for (int s = 0; ok && s < steps; ++s) {
+        begin();
+        ok = ok && ns_load<CTAS, kGram>(sh, ring, s);
+        advance(kGram);
+        begin();
+        ok = ok && ns_load<CTAS, kPolynomial>(sh, ring, s);
+        advance(kPolynomial);
+        begin();
+        ok = ok && ns_load<CTAS, kApply>(sh, ring, s);
+        advance(kApply);
+      }
+      if (!ok) // copies in flight end before shared memory goes away
+        for (unsigned back = 1; back <= kNsStages && back <= ring.it; ++back) {
+          const unsigned i = ring.it - back, st = i % kNsStages, phase = (i / kNsStages) & 1;
+          const long long start = clock64();
+          while (!barrier_try(smem_address(&sh.full[st]), phase) && clock64() - start < 10000000) {}
+        }
+    }
+  } else if (warp == kNsEpilogueWarps + 1) {
+    for (int s = 0; ok && s < steps; ++s) {
+      begin();
+      ok = ok && ns_multiply<CTAS, kGram>(sh, ring);
+      advance(kGram);
+      begin();
+      ok = ok && ns_multiply<CTAS, kPolynomial>(sh, ring);
+      advance(kPolynomial);
+      begin();
+      ok = ok && ns_multiply<CTAS, kApply>(sh, ring);
+      advance(kApply);
+    }
+    if (!ok && ring.rank == 0 && lane == 0) { // products in flight end before tensor memory is freed
+      mma_commit<CTAS>(smem_address(&sh.drained));
+      const long long start = clock64();
+      while (!barrier_try(smem_address(&sh.drained), 0) && clock64() - start < 10000000) {}
+    }
+  } else {
+    for (int s = 0; ok && s < steps; ++s) {
+      begin();
+      ok = ok && ns_drain<CTAS, kGram>(sh, ring, s, false, turn);
+      advance(kGram);
+      begin();
+      ok = ok && ns_drain<CTAS, kPolynomial>(sh, ring, s, false, turn);
+      advance(kPolynomial);
+      begin();
+      ok = ok && ns_drain<CTAS, kApply>(sh, ring, s, s + 1 == steps, turn);
+      advance(kApply);
+    }
+  }
   __syncwarp();
   tmem_fence_before();
   __syncthreads();
   if (CTAS > 1) cluster_sync_all(); // nothing of this CTA is used by the other one any more
   tmem_fence_after();
   if (threadIdx.x == 0 && sh.gave_up) atomicOr(&g_ns_gave_up, 1u);
-  if (threadIdx.x >> 5 == kNsEpilogueWarps + 1) tmem_free<CTAS>(sh.tmem, 2 * 128 * CTAS);
-}
-// After a wait that ran out: copies (or products) in flight end before shared and tensor memory go away.
-__device__ __forceinline__ void ns_abandon_loads(NsShared &sh, const NsRing &ring) {
-  for (unsigned back = 1; back <= kNsStages && back <= ring.it; ++back) {
-    const unsigned i = ring.it - back, s = i % kNsStages, phase = (i / kNsStages) & 1;
-    const long long start = clock64();
-    while (!barrier_try(smem_address(&sh.full[s]), phase) && clock64() - start < 10000000) {}
-  }
-}
-template <int CTAS>
-__device__ __forceinline__ void ns_abandon_products(NsShared &sh) {
-  mma_commit<CTAS>(smem_address(&sh.drained));
-  const long long start = clock64();
-  while (!barrier_try(smem_address(&sh.drained), 0) && clock64() - start < 10000000) {}
-}
-
-// One product over all matrices.
-template <int CTAS, int WHAT>
-__global__ void __launch_bounds__(kNsThreads, 1) muon_product_kernel(const __grid_constant__ MuonTable t, int from, int last) {
-  extern __shared__ char dynamic_smem[];
-  __shared__ __align__(8) NsShared sh;
-  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  NsRing ring = {(smem_address(dynamic_smem) + 1023) & ~1023u, CTAS == 1 ? 0 : blockIdx.x % CTAS, 0, 0};
-  float *turn = reinterpret_cast<float *>(dynamic_smem + kNsStages * kNsStageBytes + 1024);
-  ns_begin<CTAS>(sh);
-  pdl_wait();
-  pdl_launch_dependents();
-  if (warp == kNsEpilogueWarps) {
-    if (lane == 0) {
-      asm volatile("fence.proxy.async;" ::: "memory"); // the panels were written with plain stores
-      if (!ns_load<CTAS, WHAT>(t, from, sh, ring)) ns_abandon_loads(sh, ring);
-    }
-  } else if (warp == kNsEpilogueWarps + 1) {
-    if (lane == 0 && !ns_multiply<CTAS, WHAT>(t, sh, ring) && ring.rank == 0) ns_abandon_products<CTAS>(sh);
-  } else {
-    ns_drain<CTAS, WHAT>(t, from, last != 0, sh, ring, turn);
-  }
-  ns_end<CTAS>(sh);
-}
-
-// ---- all steps in one launch ---------------------------------------------------------------------------
-// For matrices whose products are short a launch per product is most of the time (measured: 10 to 13
-// us a product of 256 x 640). Here one cooperative grid goes through all of them; a product starts
-// when every CTA has stored its tiles of the one before (a counter in global memory).
-__device__ __forceinline__ void grid_arrive(unsigned *arrived) {
-  __threadfence();
-  asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(arrived) : "memory");
-}
-__device__ __forceinline__ bool grid_wait(const unsigned *arrived, unsigned target, volatile unsigned *gave_up) {
-  const long long start = clock64();
-  for (unsigned spins = 0;; ++spins) {
-    unsigned now;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(arrived) : "memory");
-    if (now >= target) return true;
-    if ((spins & 255) == 255) {
-      if (*gave_up) return false;
-      if (clock64() - start > kWaitCycles) {
-        *gave_up = 1;
-        return false;
-      }
-    }
-  }
-}
-
-__global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_constant__ MuonTable t, int steps) {
-  extern __shared__ char dynamic_smem[];
-  __shared__ __align__(8) NsShared sh;
-  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  NsRing ring = {(smem_address(dynamic_smem) + 1023) & ~1023u, 0, 0, 0};
-  float *turn = reinterpret_cast<float *>(dynamic_smem + kNsStages * kNsStageBytes + 1024);
-  ns_begin<1>(sh);
-  if (warp == kNsEpilogueWarps) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int s = 0; ok && s < steps; ++s) {
-        const int from = s & 1;
-        ok = grid_wait(t.arrived, 3 * s * gridDim.x, &sh.gave_up);
-        asm volatile("fence.proxy.async;" ::: "memory"); // panels are written with plain stores
-        ok = ok && ns_load<1, kGram>(t, from, sh, ring) && grid_wait(t.arrived, (3 * s + 1) * gridDim.x, &sh.gave_up);
-        asm volatile("fence.proxy.async;" ::: "memory");
-        ok = ok && ns_load<1, kPolynomial>(t, from, sh, ring) && grid_wait(t.arrived, (3 * s + 2) * gridDim.x, &sh.gave_up);
-        asm volatile("fence.proxy.async;" ::: "memory");
-        ok = ok && ns_load<1, kApply>(t, from, sh, ring);
-      }
-      if (!ok) ns_abandon_loads(sh, ring);
-    }
-  } else if (warp == kNsEpilogueWarps + 1) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int s = 0; ok && s < steps; ++s)
-        ok = ns_multiply<1, kGram>(t, sh, ring) && ns_multiply<1, kPolynomial>(t, sh, ring) && ns_multiply<1, kApply>(t, sh, ring);
-      if (!ok) ns_abandon_products<1>(sh);
-    }
-  } else {
-    // The draining warps read what other CTAs stored (the linear term), so they wait for the grid too.
-    // After a wait that ran out they go on through the block's barriers, all of them, without work.
-    auto live = [&] { return !__any_sync(0xffffffffu, sh.gave_up != 0); };
-    auto next = [&](unsigned product) {
-      asm volatile("fence.proxy.async;" ::: "memory");
-      asm volatile("bar.sync 1, %0;" ::"r"(kNsEpilogueWarps * 32) : "memory");
-      if (threadIdx.x == 0 && !sh.gave_up) {
-        grid_arrive(t.arrived);
-        grid_wait(t.arrived, product * gridDim.x, &sh.gave_up);
-      }
-      asm volatile("bar.sync 1, %0;" ::"r"(kNsEpilogueWarps * 32) : "memory");
-    };
-    for (int s = 0; s < steps; ++s) {
-      const int from = s & 1;
-      if (live()) ns_drain<1, kGram>(t, from, false, sh, ring, turn);
-      next(3 * s + 1);
-      if (live()) ns_drain<1, kPolynomial>(t, from, false, sh, ring, turn);
-      next(3 * s + 2);
-      if (live()) ns_drain<1, kApply>(t, from, s + 1 == steps, sh, ring, turn);
-      if (s + 1 < steps) next(3 * s + 3);
-    }
-  }
-  ns_end<1>(sh);
+  if (warp == kNsEpilogueWarps + 1) tmem_free<CTAS>(sh.tmem, 2 * 128 * CTAS);
 }
 
 // steps == 0: X itself
@@ -650,64 +656,64 @@ static void number(MuonTable &t, Blocks blocks) {
   }
   t.total = (unsigned)n; // a group's scratch bounds it far below 2^32
 }
-static bool launched(cudaError_t e) {
-  if (e == cudaSuccess) {
-    count_launch();
-    return true;
-  }
+static bool check_cuda(cudaError_t e) {
+  if (e == cudaSuccess) return true;
+  cudaGetLastError();
   set_error(PLAST_B200_ERR_CUDA, "muon: %s", cudaGetErrorString(e));
   return false;
 }
 template <class Blocks>
 static bool launch_over(MuonTable &t, Blocks blocks, void (*kernel)(const MuonTable)) {
   number(t, blocks);
-  return launched(launch_k(kernel, dim3(t.total), dim3(kMuonThreads), 0, stream(), t));
+  if (!check_cuda(launch_k(kernel, dim3(t.total), dim3(kMuonThreads), 0, stream(), t))) return false;
+  count_launch();
+  return true;
 }
-template <int CTAS> static void number_tiles(MuonTable &t) {
+template <int CTAS>
+static void run_steps(MuonTable &t, int steps) {
   for (int what = kGram; what <= kApply; ++what) {
+    // tiles of 128 x 64 where the GPU has an SM for each
     u64 n = 0;
+    for (int i = 0; i < t.count; ++i) n += ns_tiles_of<1>(t.mat[i], what, true);
+    t.narrow[what] = CTAS == 1 && n <= (u64)sm_count();
+    n = 0;
     for (int i = 0; i < t.count; ++i) {
-      t.mat[i].first_tile[what] = (unsigned)n;
-      n += ns_tiles_of<CTAS>(t.mat[i], what, t.narrow[what]);
+      MuonMat &q = t.mat[i];
+      q.first_tile[what] = (unsigned)n;
+      q.tiles[what] = (unsigned)ns_tiles_of<CTAS>(q, what, t.narrow[what]);
+      n += q.tiles[what];
     }
     t.tiles[what] = (unsigned)n;
   }
-}
-template <int CTAS, int WHAT>
-static bool launch_product(MuonTable &t, int from, int last) {
-  const auto kernel = muon_product_kernel<CTAS, WHAT>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem);
-  if (e != cudaSuccess) return launched(e);
-  const unsigned most = (unsigned)sm_count() / CTAS, grid = std::min(t.tiles[WHAT], most) * CTAS;
-  return launched(launch_kc(CTAS, kernel, dim3(grid), dim3(kNsThreads), kNsSmem, stream(), t, from, last));
-}
-// Tiles of 256 x 256 by pairs of CTAs, a launch per product.
-static void run_pairs(MuonTable &t, int steps) {
-  for (int &narrow : t.narrow) narrow = 0;
-  number_tiles<2>(t);
-  for (int s = 0; s < steps; ++s) {
-    const int from = s & 1;
-    if (!launch_product<2, kGram>(t, from, 0) || !launch_product<2, kPolynomial>(t, from, 0) ||
-        !launch_product<2, kApply>(t, from, s + 1 == steps))
-      return;
+  const auto kernel = muon_steps_kernel<CTAS>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kNsThreads);
+  cfg.dynamicSmemBytes = kNsSmem;
+  cfg.stream = stream();
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CTAS;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CTAS > 1 ? 2 : 1;
+  if (!check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem))) return;
+  // what is resident at once: one CTA per SM, pairs where a GPU partition has two SMs for them
+  unsigned most = (unsigned)sm_count();
+  if (CTAS > 1) {
+    int clusters = 0;
+    cfg.gridDim = dim3(CTAS);
+    cfg.numAttrs = 1;
+    cfg.attrs = attr + 1;
+    if (!check_cuda(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg))) return;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    most = (unsigned)clusters;
   }
-}
-// Tiles of 128 x 128 (128 x 64 where that still leaves one each), all steps in one launch.
-static void run_fused(MuonTable &t, int steps) {
-  const unsigned sms = (unsigned)sm_count();
-  for (int what = kGram; what <= kApply; ++what) {
-    u64 n = 0;
-    for (int i = 0; i < t.count; ++i) n += ns_tiles_of<1>(t.mat[i], what, true);
-    t.narrow[what] = n <= sms;
-  }
-  number_tiles<1>(t);
   const unsigned tiles = std::max(t.tiles[kGram], std::max(t.tiles[kPolynomial], t.tiles[kApply]));
-  cudaError_t e = cudaFuncSetAttribute(muon_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNsSmem);
-  if (e == cudaSuccess) {
-    void *args[] = {&t, &steps};
-    e = cudaLaunchCooperativeKernel((const void *)muon_steps_kernel, dim3(std::min(tiles, sms)), dim3(kNsThreads), args, kNsSmem, stream());
-  }
-  launched(e);
+  cfg.gridDim = dim3(std::min(tiles, most) * CTAS);
+  if (check_cuda(cudaLaunchKernelEx(&cfg, kernel, t, steps))) count_launch();
 }
 
 // One group of matrices whose scratch is `base`.
@@ -725,7 +731,7 @@ static void run_group(MuonTable &t, char *base, int steps) {
     q.b = take(panel_bytes(q.m, q.m));
     q.partial = (double *)take(padded((u64)(q.chunks + 1) * 8));
   }
-  t.arrived = (unsigned *)take(256);
+  t.stored = (unsigned *)take(256);
   auto chunks = [](const MuonMat &q) { return (u64)q.chunks; };
   auto blocks = [](const MuonMat &q) { return (u64)panel_row_blocks(q.m) * panel_col_blocks(q.n); };
   if (!launch_over(t, chunks, muon_momentum_kernel)) return;
@@ -735,8 +741,8 @@ static void run_group(MuonTable &t, char *base, int steps) {
     u64 tiles = 0;
     for (int i = 0; i < t.count; ++i) tiles += ns_tiles_of<2>(t.mat[i], kApply, false);
     const bool pairs = tuned(kTuneMuonPairs) >= 0 ? tuned(kTuneMuonPairs) != 0 : tiles >= (u64)sm_count() / 2;
-    if (pairs) run_pairs(t, steps);
-    else run_fused(t, steps);
+    if (pairs) run_steps<2>(t, steps);
+    else run_steps<1>(t, steps);
     return;
   }
   launch_over(t, chunks, muon_store_kernel);
@@ -747,7 +753,7 @@ static void run_matrices(const std::vector<MuonMat> &mats, float mu, float epsil
   u64 largest = 0;
   std::vector<size_t> ends;
   for (size_t i = 0; i < mats.size();) {
-    u64 bytes = 256; // the grid barrier
+    u64 bytes = 256; // the counters of stored tiles
     size_t k = i;
     while (k < mats.size() && k - i < (size_t)kMuonMax && (k == i || bytes + scratch_bytes(mats[k]) <= kMuonScratch))
       bytes += scratch_bytes(mats[k++]);
