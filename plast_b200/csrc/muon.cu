@@ -39,15 +39,12 @@ struct MuonMat {
   unsigned rows, cols; // as stored
   unsigned m, n;       // m <= n
   unsigned first;      // first CTA of this matrix in the launch at hand
-  unsigned first_tile[3], tiles[3]; // of this matrix in the products gram, polynomial, apply
   unsigned chunks;
 };
 struct MuonTable {
   MuonMat mat[kMuonMax];
   int count;
   unsigned total;     // CTAs of the launch at hand
-  unsigned tiles[3];  // of each product
-  int narrow[3];      // tiles of 128 x 64 instead of 128 x 128
   unsigned *stored;   // per matrix: warps that have stored their part of a tile, over all products so far
   float mu, epsilon;
   int nesterov;
@@ -185,34 +182,49 @@ constexpr int kNsEpilogueWarps = 8, kNsThreads = (kNsEpilogueWarps + 2) * 32;
 #define NS_CHUNK 2
 #endif
 constexpr int kNsChunk = NS_CHUNK;
-constexpr unsigned kNsTurnBytes = kNsEpilogueWarps * 32 * 17 * 4; // a 32 x 16 piece per warp, to store rows in order
-constexpr unsigned kNsSmem = kNsStages * kNsStageBytes + 1024 + kNsTurnBytes;
+constexpr unsigned kNsPieceBytes = 4096; // per draining warp: its 32 rows of a block's hi or lo, or 32 x 32 floats
+
+struct NsMat {
+  char *x[2], *a, *b;
+  float *w;
+  float keep, rate;
+  unsigned m, n;
+  unsigned first_tile[3], tiles[3];
+  unsigned turned; // stored as n x m
+};
+struct NsTable {
+  NsMat mat[kMuonMax];
+  unsigned *stored;
+  unsigned tiles[3]; // of each product
+  int narrow[3];     // tiles of 128 x 64 instead of 128 x 128
+  int count;
+};
 
 __device__ unsigned g_ns_gave_up; // a wait ran out: results are NaN from then on, see plast_b200_muon_status
 
 // tiles along a side, and of a product; `wide`: columns of a tile (256, 128 or 64)
 __host__ __device__ inline unsigned ns_along(unsigned size, unsigned tile) { return (size + tile - 1) / tile; }
 template <int CTAS> __host__ __device__ inline unsigned ns_wide(bool narrow) { return narrow ? 64 : 128 * CTAS; }
-template <int CTAS> __host__ __device__ inline u64 ns_tiles_of(const MuonMat &q, int what, bool narrow) {
-  const u64 r = ns_along(q.m, 128 * CTAS), per_diagonal = 128 * CTAS / ns_wide<CTAS>(narrow);
-  const u64 c = ns_along(what == kApply ? q.n : q.m, ns_wide<CTAS>(narrow));
+template <int CTAS> inline u64 ns_tiles_of(unsigned m, unsigned n, int what, bool narrow) {
+  const u64 r = ns_along(m, 128 * CTAS), per_diagonal = 128 * CTAS / ns_wide<CTAS>(narrow);
+  const u64 c = ns_along(what == kApply ? n : m, ns_wide<CTAS>(narrow));
   return what == kApply ? r * c : r * c - per_diagonal * (r * (r - 1) / 2); // row i starts at its diagonal block
 }
 
 struct NsTile {
   unsigned i, j, k_blocks; // tile row, tile column, K / 64
 };
-template <int CTAS, int WHAT>
-__device__ __forceinline__ const MuonMat &tile_at(const MuonTable &t, unsigned tile, NsTile &out) {
+template <int CTAS>
+__device__ __forceinline__ const NsMat &tile_at(const NsTable &t, int what, unsigned tile, NsTile &out) {
   int lo = 0, hi = t.count - 1; // the last matrix whose first tile is not beyond
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (t.mat[mid].first_tile[WHAT] <= tile) lo = mid; else hi = mid - 1;
+    if (t.mat[mid].first_tile[what] <= tile) lo = mid; else hi = mid - 1;
   }
-  const MuonMat &q = t.mat[lo];
-  const unsigned wide = ns_wide<CTAS>(t.narrow[WHAT]), across = ns_along(WHAT == kApply ? q.n : q.m, wide);
-  unsigned at = tile - q.first_tile[WHAT];
-  if (WHAT == kApply) {
+  const NsMat &q = t.mat[lo];
+  const unsigned wide = ns_wide<CTAS>(t.narrow[what]), across = ns_along(what == kApply ? q.n : q.m, wide);
+  unsigned at = tile - q.first_tile[what];
+  if (what == kApply) {
     out.i = at / across;
     out.j = at % across;
   } else { // rows of the upper triangle
@@ -226,64 +238,94 @@ __device__ __forceinline__ const MuonMat &tile_at(const MuonTable &t, unsigned t
     out.i = i;
     out.j = i * per_diagonal + at;
   }
-  out.k_blocks = panel_col_blocks(WHAT == kGram ? q.n : q.m);
+  out.k_blocks = panel_col_blocks(what == kGram ? q.n : q.m);
   return q;
 }
 
-// 128 rows (block row rb) by 64 of K (block kb) of a panel into `dst`: hi, then lo. `flip`: as the
-// transpose of the block above the diagonal, two pieces of 64 K rows by 64 columns each. `narrow`: 64
-// rows, rb counts in 64. Returns the bytes; what lies outside the panel is not fetched (it only feeds
-// results that are not stored).
-__device__ __forceinline__ unsigned operand_bytes(unsigned rb, unsigned row_blocks, unsigned col_blocks, bool flip, bool narrow) {
-  if (narrow) return (flip ? rb < col_blocks : rb / 2 < row_blocks) ? kPanelHalf : 0;
-  if (!flip) return rb < row_blocks ? 2 * kPanelHalf : 0;
-  return 2 * rb + 1 < col_blocks ? 2 * kPanelHalf : (2 * rb < col_blocks ? kPanelHalf : 0);
+// One operand of a tile: 128 rows (64 where narrow) by 64 of K per stage. `plain`: the block in block
+// row rb, 32 KB at once. `flip`: read MN-major from the blocks above the diagonal (or, for X, always),
+// pieces of 64 K rows by 64 columns, 8 KB of hi and of lo each. What lies outside the panel is not
+// fetched (it only feeds results that are not stored).
+struct NsOperand {
+  const char *plain, *flip;   // of K block 0; the flipped one moves on every second block
+  u64 flip_step;              // bytes from one block row to the next
+  unsigned plain_bytes, flip_bytes; // per stage
+  bool narrow;
+};
+__device__ __forceinline__ NsOperand operand_of(const char *panel, unsigned rb, unsigned row_blocks, unsigned col_blocks, bool narrow) {
+  NsOperand o;
+  o.narrow = narrow;
+  o.flip_step = panel_block(1, 0, col_blocks);
+  if (narrow) { // rb counts in 64
+    o.plain = panel + panel_block(rb / 2, 0, col_blocks) + (rb & 1) * (kPanelHalf / 2);
+    o.flip = panel + panel_block(0, rb, col_blocks);
+    o.plain_bytes = rb / 2 < row_blocks ? kPanelHalf : 0;
+    o.flip_bytes = rb < col_blocks ? kPanelHalf : 0;
+  } else {
+    o.plain = panel + panel_block(rb, 0, col_blocks);
+    o.flip = panel + panel_block(0, 2 * rb, col_blocks);
+    o.plain_bytes = rb < row_blocks ? 2 * kPanelHalf : 0;
+    o.flip_bytes = 2 * rb + 1 < col_blocks ? 2 * kPanelHalf : (2 * rb < col_blocks ? kPanelHalf : 0);
+  }
+  return o;
 }
-__device__ __forceinline__ void load_operand(uint32_t dst, const char *panel, unsigned rb, unsigned kb, unsigned row_blocks,
-                                             unsigned col_blocks, bool flip, bool narrow, uint32_t bar) {
+__device__ __forceinline__ void load_operand(const NsOperand &o, uint32_t dst, unsigned k, bool flip, uint32_t bar) {
   constexpr unsigned kPiece = kPanelHalf / 2; // 64 rows
-  if (narrow) {
-    if (flip ? rb >= col_blocks : rb / 2 >= row_blocks) return;
-    const char *src = flip ? panel + panel_block(kb / 2, rb, col_blocks) + (kb & 1) * kPiece
-                           : panel + panel_block(rb / 2, kb, col_blocks) + (rb & 1) * kPiece;
-    bulk_load(dst, src, kPiece, bar);
-    bulk_load(dst + kPanelHalf, src + kPanelHalf, kPiece, bar);
-    return;
-  }
   if (!flip) {
-    if (rb < row_blocks) bulk_load(dst, panel + panel_block(rb, kb, col_blocks), 2 * kPanelHalf, bar);
+    if (!o.plain_bytes) return;
+    const char *src = o.plain + (u64)k * (2 * kPanelHalf);
+    if (!o.narrow) bulk_load(dst, src, 2 * kPanelHalf, bar);
+    else {
+      bulk_load(dst, src, kPiece, bar);
+      bulk_load(dst + kPanelHalf, src + kPanelHalf, kPiece, bar);
+    }
     return;
   }
-#pragma unroll
-  for (unsigned c = 0; c < 2; ++c)
-    if (2 * rb + c < col_blocks) {
-      const char *src = panel + panel_block(kb / 2, 2 * rb + c, col_blocks) + (kb & 1) * kPiece;
-      bulk_load(dst + c * kPiece, src, kPiece, bar);
-      bulk_load(dst + kPanelHalf + c * kPiece, src + kPanelHalf, kPiece, bar);
-    }
+  if (!o.flip_bytes) return;
+  const char *src = o.flip + (k >> 1) * o.flip_step + (k & 1) * kPiece;
+  bulk_load(dst, src, kPiece, bar);
+  bulk_load(dst + kPanelHalf, src + kPanelHalf, kPiece, bar);
+  if (o.flip_bytes == 2 * kPanelHalf) { // the neighbouring block column
+    src += 2 * kPanelHalf;
+    bulk_load(dst + kPiece, src, kPiece, bar);
+    bulk_load(dst + kPanelHalf + kPiece, src + kPanelHalf, kPiece, bar);
+  }
 }
 
 struct NsShared {
   uint64_t full[kNsStages], peer_full[kNsStages], empty[kNsStages], acc_full[2], acc_empty[2], drained;
+  NsTable table; // a copy: the roles index it at every tile, which is slow in constant memory
   uint32_t tmem;
   volatile unsigned gave_up;
-  MuonTable table; // a copy: the roles index it at every tile, which is slow in constant memory
 };
+constexpr unsigned kNsSmem = kNsStages * kNsStageBytes + kNsEpilogueWarps * kNsPieceBytes + sizeof(NsShared);
+static_assert(kNsSmem <= 232448, "227 KB of shared memory per CTA");
+
 // A role's place in the rings of stages and accumulators, kept from one product to the next.
 struct NsRing {
-  uint32_t stages; // shared memory
-  unsigned rank;   // in the pair
-  unsigned first;  // this CTA's (pair's) first tile of the product at hand
-  unsigned it, round;
+  uint32_t stages;      // shared memory
+  unsigned rank;        // in the pair
+  unsigned first;       // this CTA's (pair's) first tile of the product at hand
+  unsigned stage, phase; // of the next stage
+  unsigned buf, turn;   // of the next accumulator
+  __device__ __forceinline__ void next_stage() {
+    if (++stage == kNsStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+  __device__ __forceinline__ void next_accumulator() {
+    buf ^= 1;
+    turn ^= buf == 0;
+  }
 };
 
 // Waits until matrix q's products up to this one (step s, product what) are stored. Relaxed polling, then
 // one fence: an acquiring load would fence at every turn.
-template <int CTAS, int WHAT>
-__device__ __forceinline__ bool ns_wait_stored(const MuonTable &t, const MuonMat &q, int s, volatile unsigned *gave_up) {
+template <int CTAS>
+__device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, int s, int what, volatile unsigned *gave_up) {
   unsigned target = s * (q.tiles[0] + q.tiles[1] + q.tiles[2]);
-  if (WHAT > kGram) target += q.tiles[kGram];
-  if (WHAT > kPolynomial) target += q.tiles[kPolynomial];
+  for (int w = 0; w < what; ++w) target += q.tiles[w];
   target *= CTAS * kNsEpilogueWarps;
   const unsigned *counter = t.stored + (&q - t.mat);
   long long start = 0;
@@ -304,32 +346,37 @@ __device__ __forceinline__ bool ns_wait_stored(const MuonTable &t, const MuonMat
   return true;
 }
 
+// The roles below take the product as an argument, not as a template: three copies of each do not fit
+// the instruction cache, and a tile of a small matrix runs its code once (measured with three copies,
+// 180 KB: 2,400 cycles to store a tile of 128 x 64, all of it fetching instructions).
+
 // ---- the thread that loads
-template <int CTAS, int WHAT>
-__device__ bool ns_load(NsShared &sh, NsRing &ring, int s) {
-  const MuonTable &t = sh.table;
+template <int CTAS>
+__device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
+  const NsTable &t = sh.table;
   const int from = s & 1;
-  const bool narrow = CTAS == 1 && t.narrow[WHAT];
-  for (unsigned tile = ring.first; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
+  const bool narrow = CTAS == 1 && t.narrow[what];
+  for (unsigned tile = ring.first; tile < t.tiles[what]; tile += gridDim.x / CTAS) {
     NsTile at;
-    const MuonMat &q = tile_at<CTAS, WHAT>(t, tile, at);
-    if (!ns_wait_stored<CTAS, WHAT>(t, q, s, &sh.gave_up)) return false;
-    asm volatile("fence.proxy.async.global;" ::: "memory"); // panels are written with plain stores
+    const NsMat &q = tile_at<CTAS>(t, what, tile, at);
     const unsigned rows = panel_row_blocks(q.m), xcb = panel_col_blocks(q.n), mcb = panel_col_blocks(q.m);
-    const char *left = WHAT == kGram ? q.x[from] : WHAT == kPolynomial ? q.a : q.b;
-    const char *right = WHAT == kPolynomial ? q.a : q.x[from];
-    const unsigned left_cb = WHAT == kGram ? xcb : mcb, right_cb = WHAT == kPolynomial ? mcb : xcb;
-    const unsigned i = at.i * CTAS + ring.rank, j = at.j * CTAS + ring.rank;
-    const unsigned j_diagonal = narrow ? at.j / 2 : at.j;
-    for (unsigned k = 0; k < at.k_blocks; ++k, ++ring.it) {
-      const unsigned st = ring.it % kNsStages, phase = (ring.it / kNsStages) & 1;
-      const bool flip_left = WHAT != kGram && k / (2 * CTAS) < at.i;
-      const bool flip_right = WHAT == kApply || (WHAT == kPolynomial && k / (2 * CTAS) < j_diagonal);
-      if (!barrier_wait(smem_address(&sh.empty[st]), phase ^ 1, &sh.gave_up)) return false;
-      const uint32_t bar = smem_address(&sh.full[st]), dst = ring.stages + st * kNsStageBytes;
-      barrier_expect(bar, operand_bytes(i, rows, left_cb, flip_left, false) + operand_bytes(j, rows, right_cb, flip_right, narrow));
-      load_operand(dst, left, i, k, rows, left_cb, flip_left, false, bar);
-      load_operand(dst + 2 * kPanelHalf, right, j, k, rows, right_cb, flip_right, narrow, bar);
+    const NsOperand left = operand_of(what == kGram ? q.x[from] : what == kPolynomial ? q.a : q.b, at.i * CTAS + ring.rank, rows,
+                                      what == kGram ? xcb : mcb, false);
+    const NsOperand right = operand_of(what == kPolynomial ? q.a : q.x[from], at.j * CTAS + ring.rank, rows,
+                                       what == kPolynomial ? mcb : xcb, narrow);
+    // K blocks before these are above the diagonal
+    const unsigned flip_left = what == kGram ? 0 : 2 * CTAS * at.i;
+    const unsigned flip_right = what == kGram ? 0 : what == kApply ? at.k_blocks : 2 * CTAS * (narrow ? at.j / 2 : at.j);
+    if (!ns_wait_stored<CTAS>(t, q, s, what, &sh.gave_up)) return false;
+    asm volatile("fence.proxy.async.global;" ::: "memory"); // panels are written with plain stores
+    for (unsigned k = 0; k < at.k_blocks; ++k) {
+      if (!barrier_wait(smem_address(&sh.empty[ring.stage]), ring.phase ^ 1, &sh.gave_up)) return false;
+      const uint32_t bar = smem_address(&sh.full[ring.stage]), dst = ring.stages + ring.stage * kNsStageBytes;
+      const bool fl = k < flip_left, fr = k < flip_right;
+      barrier_expect(bar, (fl ? left.flip_bytes : left.plain_bytes) + (fr ? right.flip_bytes : right.plain_bytes));
+      load_operand(left, dst, k, fl, bar);
+      load_operand(right, dst + 2 * kPanelHalf, k, fr, bar);
+      ring.next_stage();
     }
   }
   return true;
@@ -337,39 +384,39 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s) {
 
 // ---- the warp that issues the products (in the second CTA of a pair: passes on that its half is there).
 // All lanes walk the loops together, so that descriptors stay in uniform registers; one lane issues.
-template <int CTAS, int WHAT>
-__device__ bool ns_multiply(NsShared &sh, NsRing &ring) {
+template <int CTAS>
+__device__ bool ns_multiply(NsShared &sh, NsRing &ring, int what) {
   constexpr unsigned kColumns = 128 * CTAS;
-  const MuonTable &t = sh.table;
-  const bool narrow = CTAS == 1 && t.narrow[WHAT];
+  const NsTable &t = sh.table;
+  const bool narrow = CTAS == 1 && t.narrow[what];
   const uint32_t tmem = sh.tmem;
-  for (unsigned tile = ring.first; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
+  for (unsigned tile = ring.first; tile < t.tiles[what]; tile += gridDim.x / CTAS) {
     NsTile at;
-    tile_at<CTAS, WHAT>(t, tile, at);
-    const unsigned j_diagonal = narrow ? at.j / 2 : at.j;
-    for (unsigned k = 0; k < at.k_blocks; ++k, ++ring.it) {
-      const unsigned st = ring.it % kNsStages, phase = (ring.it / kNsStages) & 1, buf = ring.round & 1;
-      if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.full[st]), phase, &sh.gave_up))) return false;
+    tile_at<CTAS>(t, what, tile, at);
+    const unsigned flip_left = what == kGram ? 0 : 2 * CTAS * at.i;
+    const unsigned flip_right = what == kGram ? 0 : what == kApply ? at.k_blocks : 2 * CTAS * (narrow ? at.j / 2 : at.j);
+    for (unsigned k = 0; k < at.k_blocks; ++k, ring.next_stage()) {
+      const uint32_t full = smem_address(&sh.full[ring.stage]);
+      if (!__all_sync(0xffffffffu, barrier_wait(full, ring.phase, &sh.gave_up))) return false;
       if (CTAS > 1 && ring.rank != 0) {
-        if (elect_one()) barrier_arrive_at(smem_address(&sh.peer_full[st]), 0);
+        if (elect_one()) barrier_arrive_at(smem_address(&sh.peer_full[ring.stage]), 0);
         __syncwarp();
         continue;
       }
-      const bool first = k % kNsChunk == 0;
-      if (first && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_empty[buf]), ((ring.round >> 1) & 1) ^ 1, &sh.gave_up)))
+      const bool first = k % kNsChunk == 0, last = k % kNsChunk == kNsChunk - 1 || k + 1 == at.k_blocks;
+      if (first && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_empty[ring.buf]), ring.turn ^ 1, &sh.gave_up)))
         return false;
-      if (CTAS > 1 && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.peer_full[st]), phase, &sh.gave_up))) return false;
+      if (CTAS > 1 && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.peer_full[ring.stage]), ring.phase, &sh.gave_up)))
+        return false;
       tmem_fence_after();
-      const bool flip_left = WHAT != kGram && k / (2 * CTAS) < at.i;
-      const bool flip_right = WHAT == kApply || (WHAT == kPolynomial && k / (2 * CTAS) < j_diagonal);
-      const uint32_t stage = ring.stages + st * kNsStageBytes;
+      const bool fl = k < flip_left, fr = k < flip_right;
+      const uint32_t stage = ring.stages + ring.stage * kNsStageBytes;
       const uint64_t left = operand_desc(stage, kPanelHalf / 2, 1024);
       const uint64_t right = operand_desc(stage + 2 * kPanelHalf, kPanelHalf / 2, 1024);
-      const uint32_t acc = tmem + buf * kColumns;
-      const uint32_t desc = mma_desc(128 * CTAS, ns_wide<CTAS>(narrow), flip_left, flip_right);
+      const uint32_t acc = tmem + ring.buf * kColumns;
+      const uint32_t desc = mma_desc(128 * CTAS, ns_wide<CTAS>(narrow), fl, fr);
       // 16 of K: 32 bytes along K-major rows, or 16 rows of 128 bytes; descriptors count in 16 bytes
-      const unsigned left_step = flip_left ? 128 : 2, right_step = flip_right ? 128 : 2;
-      const bool last = k % kNsChunk == kNsChunk - 1 || k + 1 == at.k_blocks;
+      const unsigned left_step = fl ? 128 : 2, right_step = fr ? 128 : 2;
       if (elect_one()) {
 #pragma unroll
         for (int part = 0; part < 3; ++part) { // lo hi, hi lo, hi hi
@@ -378,42 +425,94 @@ __device__ bool ns_multiply(NsShared &sh, NsRing &ring) {
           for (int step = 0; step < 4; ++step)
             mma_f16<CTAS>(acc, l + step * left_step, r + step * right_step, desc, !(first && part == 0 && step == 0));
         }
-        mma_commit<CTAS>(smem_address(&sh.empty[st]));
-        if (last) mma_commit<CTAS>(smem_address(&sh.acc_full[buf]));
+        mma_commit<CTAS>(smem_address(&sh.empty[ring.stage]));
+        if (last) mma_commit<CTAS>(smem_address(&sh.acc_full[ring.buf]));
       }
       __syncwarp();
-      if (last) ++ring.round;
+      if (last) ring.next_accumulator();
     }
   }
   return true;
 }
 
-// ---- the warps that drain: warp w takes rows 32 (w % 4) .. and half of the tile's columns
-template <int CTAS, int WHAT>
-__device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, bool last, float *turn) {
+// ---- the warps that drain: warp w takes rows 32 (w % 4) .. and half of the tile's columns, in groups of
+// 64 (one block column; 32 of one where narrow).
+//
+// A lane holds a row, so it would touch 32 different lines per access to a panel; the warp's 32 rows of
+// a block lie in 4 KB without gaps, so they go through shared memory instead and a warp's access covers
+// four whole lines. The linear term (b A or a X) starts the sum: it is fetched while the first products
+// run.
+template <int CTAS>
+__device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last, char *piece) {
   constexpr unsigned kColumns = 128 * CTAS;
-  const MuonTable &t = sh.table;
+  const float init = what == kPolynomial ? kNsB / kNsC * kSplitScale : kNsA * kSplitScale;
+  const float finish = what == kPolynomial ? kNsC * kSplitUnscale : kSplitUnscale;
+  const NsTable &t = sh.table;
   const int from = s & 1;
-  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned row_in_tile = (warp & 3) * 32 + lane, half = warp >> 2;
-  const bool narrow = CTAS == 1 && t.narrow[WHAT];
-  const unsigned groups = narrow ? 1 : 2 * CTAS; // of 32 columns
-  for (unsigned tile = ring.first; tile < t.tiles[WHAT]; tile += gridDim.x / CTAS) {
+  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
+  const unsigned row_in_tile = (warp & 3) * 32 + lane;
+  const bool narrow = CTAS == 1 && t.narrow[what];
+  // a warp's pass over its rows of a group: `chunks` 16-byte pieces per row, 32 pieces at a time
+  const unsigned chunks = narrow ? 4 : 8, shift = narrow ? 2 : 3;
+  for (unsigned tile = ring.first; tile < t.tiles[what]; tile += gridDim.x / CTAS) {
     NsTile at;
-    const MuonMat &q = tile_at<CTAS, WHAT>(t, tile, at);
+    const NsMat &q = tile_at<CTAS>(t, what, tile, at);
+    const unsigned rb = at.i * CTAS + ring.rank, col_blocks = panel_col_blocks(what == kApply ? q.n : q.m);
+    const bool rows_exist = rb < panel_row_blocks(q.m);
+    // the group's block column and its first chunk there
+    const unsigned cb0 = narrow ? at.j : (at.j * 2 + half) * CTAS, chunk0 = narrow ? half * 4 : 0;
     float acc[64 * CTAS];
 #pragma unroll
     for (int i = 0; i < 64 * CTAS; ++i) acc[i] = 0.0f;
+    if (what != kGram) {
+      // other CTAs' work: the warp looks for itself that it is stored
+      bool ok = true;
+      if (lane == 0) ok = ns_wait_stored<CTAS>(t, q, s, what, &sh.gave_up);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      const char *old = what == kPolynomial ? q.a : q.x[from];
+#pragma unroll
+      for (int b = 0; b < CTAS; ++b) {
+        if (!rows_exist || cb0 + b >= col_blocks) continue;
+        const char *block = old + panel_block(rb, cb0 + b, col_blocks) + (warp & 3) * 4096;
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part, block += kPanelHalf) { // past L1, which may hold an earlier step's values
+          uint4 v[8];
+#pragma unroll
+          for (unsigned c = 0; c < 8; ++c) {
+            const unsigned item = c * 32 + lane;
+            if (c < chunks) v[c] = __ldcg(reinterpret_cast<const uint4 *>(block + panel_chunk(item >> shift, chunk0 + (item & (chunks - 1)))));
+          }
+#pragma unroll
+          for (unsigned c = 0; c < 8; ++c) {
+            const unsigned item = c * 32 + lane;
+            if (c < chunks) *reinterpret_cast<uint4 *>(piece + panel_chunk(item >> shift, chunk0 + (item & (chunks - 1)))) = v[c];
+          }
+          __syncwarp();
+#pragma unroll
+          for (unsigned c = 0; c < 8; ++c) {
+            if (c >= chunks) continue;
+            const uint4 h = *reinterpret_cast<const uint4 *>(piece + panel_chunk(lane, chunk0 + c));
+            const unsigned w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+              acc[b * 64 + c * 8 + 2 * i] = __fmaf_rn(f.x, init, acc[b * 64 + c * 8 + 2 * i]);
+              acc[b * 64 + c * 8 + 2 * i + 1] = __fmaf_rn(f.y, init, acc[b * 64 + c * 8 + 2 * i + 1]);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
     const unsigned rounds = (at.k_blocks + kNsChunk - 1) / kNsChunk;
 #pragma unroll 1
-    for (unsigned c = 0; c < rounds; ++c, ++ring.round) {
-      const unsigned buf = ring.round & 1;
-      if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_full[buf]), (ring.round >> 1) & 1, &sh.gave_up))) return false;
+    for (unsigned c = 0; c < rounds; ++c) {
+      if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_full[ring.buf]), ring.turn, &sh.gave_up))) return false;
       tmem_fence_after();
-      const uint32_t columns = sh.tmem + (((warp & 3) * 32) << 16) + buf * kColumns + half * groups * 32;
+      const uint32_t columns = sh.tmem + (((warp & 3) * 32) << 16) + ring.buf * kColumns + half * (narrow ? 32 : 64 * CTAS);
 #pragma unroll
       for (int g = 0; g < 2 * CTAS; ++g) {
-        if (g >= groups) continue;
+        if (g > 0 && narrow) continue;
         float v[32];
         tmem_load32(columns + g * 32, v);
 #pragma unroll
@@ -422,98 +521,80 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, bool last, float *tu
       tmem_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if (ring.rank == 0) barrier_arrive(smem_address(&sh.acc_empty[buf]));
-        else barrier_arrive_at(smem_address(&sh.acc_empty[buf]), 0);
+        if (ring.rank == 0) barrier_arrive(smem_address(&sh.acc_empty[ring.buf]));
+        else barrier_arrive_at(smem_address(&sh.acc_empty[ring.buf]), 0);
       }
+      ring.next_accumulator();
     }
-    const unsigned width = WHAT == kApply ? q.n : q.m, rb = at.i * CTAS + ring.rank;
-    const unsigned col_blocks = panel_col_blocks(width), row_blocks = panel_row_blocks(q.m);
-    const char *old = WHAT == kPolynomial ? q.a : q.x[from]; // the linear term
-    char *out = WHAT == kGram ? q.a : WHAT == kPolynomial ? q.b : q.x[from ^ 1];
+    char *out = what == kGram ? q.a : what == kPolynomial ? q.b : q.x[from ^ 1];
     const unsigned row = rb * 128 + row_in_tile;
-    // The linear term is other CTAs' work; the accumulators came after it was stored (the loads waited),
-    // which orders it for the thread that loaded: this warp looks for itself.
-    if (WHAT != kGram) {
-      bool ok = true;
-      if (lane == 0) ok = ns_wait_stored<CTAS, WHAT>(t, q, s, &sh.gave_up);
-      if (!__all_sync(0xffffffffu, ok)) return false;
-    }
-    // 32 columns at a time: half of a block column. All its loads are issued before its stores: the
-    // compiler cannot move a load over a store that may alias it, and a load waits for L2.
+    const bool weights = what == kApply && last;
 #pragma unroll
-    for (int g = 0; g < 2 * CTAS; ++g) {
-      if (g >= groups || rb >= row_blocks) continue;
-      const unsigned col0 = at.j * ns_wide<CTAS>(narrow) + (half * groups + g) * 32;
-      const unsigned cb = col0 / kPanelCols, chunk0 = (col0 % kPanelCols) / 8;
-      if (cb >= col_blocks) continue;
-      const u64 offset = panel_block(rb, cb, col_blocks);
-      float v[32];
+    for (int b = 0; b < CTAS; ++b) {
+      if (!rows_exist || cb0 + b >= col_blocks) continue;
+      if (!weights) {
+        char *block = out + panel_block(rb, cb0 + b, col_blocks) + (warp & 3) * 4096;
+        unsigned lo[32];
+        // hi goes out while lo waits in registers; padding stays zero (an operand read from beyond the
+        // panel may leave anything in the sums)
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = acc[g * 32 + i] * kSplitUnscale;
-      if (WHAT != kGram) {
-        uint4 hi[4], lo[4];
+        for (int c = 0; c < 8; ++c) {
+          unsigned hi[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) { // past L1, which may hold an earlier step's values
-          const char *here = old + offset + panel_chunk(row_in_tile, chunk0 + c);
-          hi[c] = __ldcg(reinterpret_cast<const uint4 *>(here));
-          lo[c] = __ldcg(reinterpret_cast<const uint4 *>(here + kPanelHalf));
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float z[8];
-          join8(hi[c], lo[c], z);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float &r = v[c * 8 + i];
-            r = WHAT == kPolynomial ? __fmaf_rn(kNsB, z[i], kNsC * r) : __fmaf_rn(kNsA, z[i], r);
+          for (int i = 0; i < 4; ++i) {
+            float x = acc[b * 64 + c * 8 + 2 * i] * finish, y = acc[b * 64 + c * 8 + 2 * i + 1] * finish;
+            if (row >= q.m) x = y = 0.0f;
+            const __half2 h = __floats2half2_rn(x, y);
+            const float2 f = __half22float2(h);
+            const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+            hi[i] = *reinterpret_cast<const unsigned *>(&h);
+            lo[c * 4 + i] = *reinterpret_cast<const unsigned *>(&l);
           }
+          if (c < chunks) *reinterpret_cast<uint4 *>(piece + panel_chunk(lane, chunk0 + c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         }
-      }
-      if (WHAT != kApply || !last) {
-        if (row >= q.m) { // padding stays zero (an operand read from beyond the panel may leave anything here)
+        __syncwarp();
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part, block += kPanelHalf) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-        }
+          for (unsigned c = 0; c < 8; ++c) {
+            if (c >= chunks) continue;
+            const unsigned item = c * 32 + lane, o = panel_chunk(item >> shift, chunk0 + (item & (chunks - 1)));
+            *reinterpret_cast<uint4 *>(block + o) = *reinterpret_cast<const uint4 *>(piece + o);
+          }
+          __syncwarp();
+          if (part == 1) break;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint4 hi, lo;
-          split8(v + c * 8, hi, lo);
-          char *here = out + offset + panel_chunk(row_in_tile, chunk0 + c);
-          *reinterpret_cast<uint4 *>(here) = hi;
-          *reinterpret_cast<uint4 *>(here + kPanelHalf) = lo;
+          for (unsigned c = 0; c < 8; ++c)
+            if (c < chunks)
+              *reinterpret_cast<uint4 *>(piece + panel_chunk(lane, chunk0 + c)) =
+                  make_uint4(lo[c * 4], lo[c * 4 + 1], lo[c * 4 + 2], lo[c * 4 + 3]);
+          __syncwarp();
         }
         continue;
       }
-      // the weights (or the output), 32 neighbours to an access: where the matrix was turned, the lanes'
-      // rows are neighbours as they are, else a piece is turned in shared memory first
-      const float scale = g_ns_gave_up ? NAN : kSplitUnscale * q.rate;
-      if (q.rows > q.cols) {
-        if (row < q.m)
+      // the weights (or the output): 32 x 32 through shared memory, then 32 neighbours to an access, along
+      // the matrix's rows as they are stored
+      const float scale = g_ns_gave_up ? NAN : finish * kSplitUnscale * q.rate;
+      float *mine = reinterpret_cast<float *>(piece);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (col0 + i < q.n) {
-              float *w = q.w + (u64)(col0 + i) * q.m + row;
-              *w = q.keep == 0.0f ? -scale * v[i] : q.keep * *w - scale * v[i];
-            }
-      } else {
-        float *mine = turn + warp * (32 * 17);
-        const unsigned row0 = rb * 128 + (warp & 3) * 32 + (lane >> 4);
+      for (int g = 0; g < 2; ++g) {
+        if (g > 0 && narrow) continue;
 #pragma unroll
-        for (int piece = 0; piece < 2; ++piece) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mine[lane * 17 + i] = v[piece * 16 + i];
-          __syncwarp();
-          const unsigned col = col0 + piece * 16 + (lane & 15);
-          if (col < q.n)
-#pragma unroll 8
-            for (int r = 0; r < 32; r += 2)
-              if (row0 + r < q.m) {
-                float *w = q.w + (u64)(row0 + r) * q.n + col;
-                const float x = scale * mine[(r + (lane >> 4)) * 17 + (lane & 15)];
-                *w = q.keep == 0.0f ? -x : q.keep * *w - x;
-              }
-          __syncwarp();
+        for (int i = 0; i < 32; ++i) mine[lane * 32 + (i ^ lane)] = acc[b * 64 + g * 32 + i];
+        __syncwarp();
+        const unsigned row0 = rb * 128 + (warp & 3) * 32, col0 = (cb0 + b) * kPanelCols + chunk0 * 8 + g * 32;
+        const unsigned outer0 = q.turned ? col0 : row0, inner = (q.turned ? row0 : col0) + lane;
+        const unsigned outer_end = q.turned ? q.n : q.m, inner_end = q.turned ? q.m : q.n;
+        if (inner < inner_end) {
+          float *w = q.w + (u64)outer0 * inner_end + inner;
+          const unsigned count = outer_end > outer0 ? (outer_end - outer0 < 32 ? outer_end - outer0 : 32) : 0;
+#pragma unroll 4
+          for (unsigned r = 0; r < count; ++r, w += inner_end) {
+            const float x = scale * mine[q.turned ? lane * 32 + (r ^ lane) : r * 32 + (lane ^ r)];
+            *w = q.keep == 0.0f ? -x : q.keep * *w - x;
+          }
         }
+        __syncwarp();
       }
     }
     __syncwarp();
@@ -523,14 +604,13 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, bool last, float *tu
 }
 
 template <int CTAS>
-__global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_constant__ MuonTable param, int steps) {
-  extern __shared__ char dynamic_smem[];
-  __shared__ __align__(16) NsShared sh;
+__global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_constant__ NsTable param, int steps) {
+  extern __shared__ __align__(1024) char dynamic_smem[];
+  NsShared &sh = *reinterpret_cast<NsShared *>(dynamic_smem + kNsStages * kNsStageBytes + kNsEpilogueWarps * kNsPieceBytes);
   const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (unsigned i = threadIdx.x; i < sizeof(MuonTable) / 4; i += kNsThreads)
+  for (unsigned i = threadIdx.x; i < sizeof(NsTable) / 4; i += kNsThreads)
     reinterpret_cast<unsigned *>(&sh.table)[i] = reinterpret_cast<const unsigned *>(&param)[i];
-  NsRing ring = {(smem_address(dynamic_smem) + 1023) & ~1023u, CTAS == 1 ? 0 : blockIdx.x % CTAS, 0, 0, 0};
-  float *turn = reinterpret_cast<float *>(dynamic_smem + kNsStages * kNsStageBytes + 1024);
+  NsRing ring = {smem_address(dynamic_smem), CTAS == 1 ? 0 : blockIdx.x % CTAS, 0, 0, 0, 0, 0};
   if (threadIdx.x == 0) {
     for (int s = 0; s < kNsStages; ++s) {
       barrier_init(smem_address(&sh.full[s]), 1);
@@ -554,60 +634,31 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
 
   // Tiles are numbered through all products, so that a product that ends between two turns of the grid
   // leaves the next one's first tiles to the CTAs that are free.
-  const MuonTable &t = sh.table;
+  const NsTable &t = sh.table;
   const unsigned workers = gridDim.x / CTAS, me = blockIdx.x / CTAS;
+  char *piece = dynamic_smem + kNsStages * kNsStageBytes + warp * kNsPieceBytes;
   unsigned before = 0; // tiles of the products so far, modulo the number of workers
-  auto advance = [&](int what) { before = (before + t.tiles[what]) % workers; };
-  auto begin = [&] { ring.first = (me + workers - before) % workers; };
   bool ok = true;
-  if (warp == kNsEpilogueWarps) {
-    if (lane == 0) {
-      for (int s = 0; ok && s < steps; ++s) {
-        begin();
-        ok = ok && ns_load<CTAS, kGram>(sh, ring, s);
-        advance(kGram);
-        begin();
-        ok = ok && ns_load<CTAS, kPolynomial>(sh, ring, s);
-        advance(kPolynomial);
-        begin();
-        ok = ok && ns_load<CTAS, kApply>(sh, ring, s);
-        advance(kApply);
+#pragma unroll 1
+  for (int product = 0; ok && product < 3 * steps; ++product) {
+    const int s = product / 3, what = product - 3 * s;
+    ring.first = (me + workers - before) % workers;
+    if (warp < kNsEpilogueWarps) ok = ns_drain<CTAS>(sh, ring, s, what, s + 1 == steps, piece);
+    else if (warp == kNsEpilogueWarps + 1) ok = ns_multiply<CTAS>(sh, ring, what);
+    else if (lane == 0) ok = ns_load<CTAS>(sh, ring, s, what);
+    before = (before + t.tiles[what]) % workers;
+  }
+  if (!ok && lane == 0) { // after a wait that ran out: what is in flight ends before its memory goes away
+    const long long start = clock64();
+    if (warp == kNsEpilogueWarps)
+      for (int st = 0; st < kNsStages; ++st) {
+        // the phase of this stage's last copy: the current one where the ring has passed it
+        const unsigned phase = (unsigned)st < ring.stage ? ring.phase : ring.phase ^ 1;
+        while (!barrier_try(smem_address(&sh.full[st]), phase) && clock64() - start < 10000000) {}
       }
-      if (!ok) // copies in flight end before shared memory goes away
-        for (unsigned back = 1; back <= kNsStages && back <= ring.it; ++back) {
-          const unsigned i = ring.it - back, st = i % kNsStages, phase = (i / kNsStages) & 1;
-          const long long start = clock64();
-          while (!barrier_try(smem_address(&sh.full[st]), phase) && clock64() - start < 10000000) {}
-        }
-    }
-  } else if (warp == kNsEpilogueWarps + 1) {
-    for (int s = 0; ok && s < steps; ++s) {
-      begin();
-      ok = ok && ns_multiply<CTAS, kGram>(sh, ring);
-      advance(kGram);
-      begin();
-      ok = ok && ns_multiply<CTAS, kPolynomial>(sh, ring);
-      advance(kPolynomial);
-      begin();
-      ok = ok && ns_multiply<CTAS, kApply>(sh, ring);
-      advance(kApply);
-    }
-    if (!ok && ring.rank == 0 && lane == 0) { // products in flight end before tensor memory is freed
+    if (warp == kNsEpilogueWarps + 1 && ring.rank == 0) {
       mma_commit<CTAS>(smem_address(&sh.drained));
-      const long long start = clock64();
       while (!barrier_try(smem_address(&sh.drained), 0) && clock64() - start < 10000000) {}
-    }
-  } else {
-    for (int s = 0; ok && s < steps; ++s) {
-      begin();
-      ok = ok && ns_drain<CTAS, kGram>(sh, ring, s, false, turn);
-      advance(kGram);
-      begin();
-      ok = ok && ns_drain<CTAS, kPolynomial>(sh, ring, s, false, turn);
-      advance(kPolynomial);
-      begin();
-      ok = ok && ns_drain<CTAS, kApply>(sh, ring, s, s + 1 == steps, turn);
-      advance(kApply);
     }
   }
   __syncwarp();
@@ -670,17 +721,34 @@ static bool launch_over(MuonTable &t, Blocks blocks, void (*kernel)(const MuonTa
   return true;
 }
 template <int CTAS>
-static void run_steps(MuonTable &t, int steps) {
+static void run_steps(const MuonTable &mt, int steps) {
+  NsTable t = {};
+  t.count = mt.count;
+  t.stored = mt.stored;
+  for (int i = 0; i < mt.count; ++i) {
+    const MuonMat &q = mt.mat[i];
+    NsMat &d = t.mat[i];
+    d.x[0] = q.x[0];
+    d.x[1] = q.x[1];
+    d.a = q.a;
+    d.b = q.b;
+    d.w = q.w;
+    d.keep = q.keep;
+    d.rate = q.rate;
+    d.m = q.m;
+    d.n = q.n;
+    d.turned = q.rows > q.cols;
+  }
   for (int what = kGram; what <= kApply; ++what) {
     // tiles of 128 x 64 where the GPU has an SM for each
     u64 n = 0;
-    for (int i = 0; i < t.count; ++i) n += ns_tiles_of<1>(t.mat[i], what, true);
+    for (int i = 0; i < t.count; ++i) n += ns_tiles_of<1>(t.mat[i].m, t.mat[i].n, what, true);
     t.narrow[what] = CTAS == 1 && n <= (u64)sm_count();
     n = 0;
     for (int i = 0; i < t.count; ++i) {
-      MuonMat &q = t.mat[i];
+      NsMat &q = t.mat[i];
       q.first_tile[what] = (unsigned)n;
-      q.tiles[what] = (unsigned)ns_tiles_of<CTAS>(q, what, t.narrow[what]);
+      q.tiles[what] = (unsigned)ns_tiles_of<CTAS>(q.m, q.n, what, t.narrow[what]);
       n += q.tiles[what];
     }
     t.tiles[what] = (unsigned)n;
@@ -739,7 +807,7 @@ static void run_group(MuonTable &t, char *base, int steps) {
   if (!launch_over(t, blocks, muon_load_kernel)) return;
   if (steps > 0) {
     u64 tiles = 0;
-    for (int i = 0; i < t.count; ++i) tiles += ns_tiles_of<2>(t.mat[i], kApply, false);
+    for (int i = 0; i < t.count; ++i) tiles += ns_tiles_of<2>(t.mat[i].m, t.mat[i].n, kApply, false);
     const bool pairs = tuned(kTuneMuonPairs) >= 0 ? tuned(kTuneMuonPairs) != 0 : tiles >= (u64)sm_count() / 2;
     if (pairs) run_steps<2>(t, steps);
     else run_steps<1>(t, steps);

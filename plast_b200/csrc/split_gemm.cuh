@@ -98,8 +98,7 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, unsigned parity) {
 // A wait that always ends: after about two seconds, or when another role of the CTA has given up, it
 // raises `*gave_up` (shared memory) and returns false; the caller then leaves its loop.
 constexpr long long kWaitCycles = 4000000000ll;
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, unsigned parity, volatile unsigned *gave_up) {
-  if (barrier_try(bar, parity)) return true;
+__device__ __noinline__ bool barrier_wait_long(uint32_t bar, unsigned parity, volatile unsigned *gave_up) {
   const long long start = clock64();
   for (;;) {
     for (int i = 0; i < 64; ++i)
@@ -110,6 +109,10 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, unsigned parity, vola
       return false;
     }
   }
+}
+
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, unsigned parity, volatile unsigned *gave_up) {
+  return barrier_try(bar, parity) || barrier_wait_long(bar, parity, gave_up);
 }
 
 // ---- copies and tensor core ----------------------------------------------------------------------------
