@@ -131,13 +131,14 @@ def _load() -> C.CDLL:
             f"{LIB_PATH} is missing: build it with `python -m plast_b200.build` "
             "(there is no CPU fallback for the CUDA path)")
     lib = C.CDLL(str(LIB_PATH))
+    # `inputs` as an address: any array of Tensor pointers, or of their addresses (see _addresses)
     for op in FORWARD_OPS:
         fn = getattr(lib, f"{op}_cuda_forward")
-        fn.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(CTensor), KernelParams]
+        fn.argtypes = [C.c_void_p, C.POINTER(CTensor), KernelParams]
         fn.restype = None
     for op in BACKWARD_OPS:
         fn = getattr(lib, f"{op}_cuda_backward")
-        fn.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(CTensor), KernelParams]
+        fn.argtypes = [C.c_void_p, C.POINTER(CTensor), KernelParams]
         fn.restype = None
     lib.sum_axis0_noalloc_cuda_forward.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(CTensor), KernelParams]
     lib.sum_axis0_noalloc_cuda_forward.restype = None
@@ -392,6 +393,16 @@ def _ptr_array(tensors):
     return arr
 
 
+_ADDRESSES = [C.c_void_p * n for n in range(9)]
+
+
+def _addresses(tensors):
+    """Tensor** as an array of addresses: a fifth of the time of an array of pointer objects, which is most of what a
+    call on a small tensor costs. The caller's list keeps the structs alive."""
+    n = len(tensors)
+    return (_ADDRESSES[n] if n < 9 else C.c_void_p * n)(*[C.addressof(t.c) for t in tensors])
+
+
 def check_error():
     code = lib.plast_b200_last_error()
     if code != 0:
@@ -401,8 +412,7 @@ def check_error():
 def forward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fval: float = 0.0,
             check: bool = True):
     """``<op>_cuda_forward(inputs, output, params)``; raises :class:`PlastError` on failure."""
-    getattr(lib, f"{op}_cuda_forward")(_ptr_array(inputs), C.byref(output.c),
-                                       KernelParams(dim, keepdim, fval))
+    getattr(lib, f"{op}_cuda_forward")(_addresses(inputs), C.byref(output.c), KernelParams(dim, keepdim, fval))
     if check:
         check_error()
     return output
@@ -411,8 +421,7 @@ def forward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fva
 def backward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fval: float = 0.0,
              check: bool = True):
     """``<op>_cuda_backward(inputs, output, params)``: accumulates into inputs[i].grad."""
-    getattr(lib, f"{op}_cuda_backward")(_ptr_array(inputs), C.byref(output.c),
-                                        KernelParams(dim, keepdim, fval))
+    getattr(lib, f"{op}_cuda_backward")(_addresses(inputs), C.byref(output.c), KernelParams(dim, keepdim, fval))
     if check:
         check_error()
 

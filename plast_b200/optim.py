@@ -52,14 +52,13 @@ assert C.sizeof(SGD) == 4 and C.sizeof(Adam) == 56 and C.sizeof(AdamW) == 56
 assert Adam.t.offset == 16 and Adam.m.offset == 24 and AdamW.t.offset == 20 and AdamW.m.offset == 24
 
 for _name, _struct in (("sgd_step_cuda", SGD), ("adam_step_cuda", Adam), ("adamw_step_cuda", AdamW), ("muon_step_cuda", Muon)):
-    getattr(lib, _name).argtypes = [C.POINTER(_struct), C.POINTER(C.POINTER(CTensor)), C.c_int]
+    getattr(lib, _name).argtypes = [C.POINTER(_struct), C.c_void_p, C.c_int]   # any array of Tensor pointers or addresses
     getattr(lib, _name).restype = None
 lib.plast_b200_adam_state_release.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(C.POINTER(CTensor))]
 lib.plast_b200_adam_state_release.restype = None
 lib.plast_b200_muon_state_release.argtypes = [C.POINTER(C.POINTER(CTensor))]
 lib.plast_b200_muon_state_release.restype = None
-lib.plast_b200_orthogonalise.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(C.POINTER(CTensor)), C.c_int, C.c_int,
-                                         C.c_float]
+lib.plast_b200_orthogonalise.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_float]
 lib.plast_b200_orthogonalise.restype = None
 
 
@@ -72,11 +71,16 @@ def param_array(params):
     return arr
 
 
+def _address_array(params):
+    """param_array() as plain addresses, for the length of one call."""
+    return (C.c_void_p * max(len(params), 1))(*[None if p is None else C.addressof(p.c) for p in params])
+
+
 def step(optimizer, params) -> None:
     """One optimiser step on the GPU over a list of parameters (Tensor objects with .grad)."""
     fn = {SGD: lib.sgd_step_cuda, Adam: lib.adam_step_cuda, AdamW: lib.adamw_step_cuda,
           Muon: lib.muon_step_cuda}[type(optimizer)]
-    fn(C.byref(optimizer), param_array(params), len(params))
+    fn(C.byref(optimizer), _address_array(params), len(params))
     check_error()
 
 
@@ -84,7 +88,7 @@ def orthogonalise(inputs, outputs, steps: int = 5, epsilon: float = 1e-7) -> Non
     """outputs[i] = the Newton-Schulz orthogonalisation of inputs[i], all matrices at once."""
     if len(inputs) != len(outputs):
         raise ValueError("as many outputs as inputs")
-    lib.plast_b200_orthogonalise(param_array(inputs), param_array(outputs), len(inputs), steps, epsilon)
+    lib.plast_b200_orthogonalise(_address_array(inputs), _address_array(outputs), len(inputs), steps, epsilon)
     check_error()
 
 
