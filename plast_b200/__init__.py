@@ -409,10 +409,19 @@ def check_error():
         raise PlastError(code, lib.plast_b200_last_error_message().decode())
 
 
+_ENTRY = {}                                          # (direction, op) -> the entry point, looked up once
+
+
+def _entry(direction: str, op: str):
+    fn = _ENTRY[direction, op] = getattr(lib, f"{op}_cuda_{direction}")
+    return fn
+
+
 def forward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fval: float = 0.0,
             check: bool = True):
     """``<op>_cuda_forward(inputs, output, params)``; raises :class:`PlastError` on failure."""
-    getattr(lib, f"{op}_cuda_forward")(_addresses(inputs), C.byref(output.c), KernelParams(dim, keepdim, fval))
+    fn = _ENTRY.get(("forward", op)) or _entry("forward", op)
+    fn(_addresses(inputs), C.byref(output.c), KernelParams(dim, keepdim, fval))
     if check:
         check_error()
     return output
@@ -421,7 +430,8 @@ def forward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fva
 def backward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fval: float = 0.0,
              check: bool = True):
     """``<op>_cuda_backward(inputs, output, params)``: accumulates into inputs[i].grad."""
-    getattr(lib, f"{op}_cuda_backward")(_addresses(inputs), C.byref(output.c), KernelParams(dim, keepdim, fval))
+    fn = _ENTRY.get(("backward", op)) or _entry("backward", op)
+    fn(_addresses(inputs), C.byref(output.c), KernelParams(dim, keepdim, fval))
     if check:
         check_error()
 
