@@ -45,7 +45,7 @@ struct MuonTable {
   MuonMat mat[kMuonMax];
   int count;
   unsigned total;     // CTAs of the launch at hand
-  unsigned *stored;   // per matrix: warps that have stored their part of a tile, over all products so far
+  unsigned *stored;   // per matrix: CTAs that have stored their part of a tile, over all products so far
   float mu, epsilon;
   int nesterov;
 };
@@ -163,11 +163,14 @@ __global__ void __launch_bounds__(kMuonThreads) muon_load_kernel(const __grid_co
 // A and B are symmetric: only tiles on and above the diagonal are computed and stored. An operand
 // block below it is fetched as the block above it and read MN-major, which is its transpose.
 //
+// (Folding the linear terms into the operands' diagonals would save the epilogues a read, but rounds a
+// number near 3.4 to 22 bits where b A + c A A is small: 3 to 6e-6 off instead of 1.1 to 1.5e-6.)
+//
 // One launch goes through all products of all matrices. A persistent CTA takes every gridDim-th tile,
 // of 128 x 128 (or 128 x 64); a pair of CTAs (CTAS = 2) tiles of 256 x 256, each CTA holding half of
 // either operand. One thread brings 64 KB stages (64 of K, hi and lo of both operands) with bulk
 // copies, one warp (of the pair) issues the twelve tcgen05.mma of a stage, small products first, and
-// eight warps drain the accumulators. Tensor-core accumulation truncates; every kNsChunk stages the
+// sixteen warps drain the accumulators. Tensor-core accumulation truncates; every kNsChunk stages the
 // accumulator (one of two in tensor memory) is therefore added in fp32 registers, rounded to nearest,
 // while the next one fills.
 //
@@ -177,12 +180,12 @@ __global__ void __launch_bounds__(kMuonThreads) muon_load_kernel(const __grid_co
 enum MuonProduct { kGram = 0, kPolynomial = 1, kApply = 2 };
 constexpr int kNsStages = 3;
 constexpr unsigned kNsStageBytes = 4 * kPanelHalf; // left hi, left lo, right hi, right lo
-constexpr int kNsEpilogueWarps = 8, kNsThreads = (kNsEpilogueWarps + 2) * 32;
+constexpr int kNsEpilogueWarps = 16, kNsThreads = (kNsEpilogueWarps + 3) * 32;
 #ifndef NS_CHUNK
 #define NS_CHUNK 2
 #endif
 constexpr int kNsChunk = NS_CHUNK;
-constexpr unsigned kNsPieceBytes = 4096; // per draining warp: its 32 rows of a block's hi or lo, or 32 x 32 floats
+constexpr unsigned kNsPieceBytes = 2048; // per draining warp: 32 rows of 32 columns of hi or lo, or 32 x 16 floats
 
 struct NsMat {
   char *x[2], *a, *b;
@@ -242,6 +245,10 @@ __device__ __forceinline__ const NsMat &tile_at(const NsTable &t, int what, unsi
   return q;
 }
 
+// The linear term of a tile comes through the same ring of stages, after the first four K blocks (or
+// after the last): by then the draining warps are done with the tile before and take it at once.
+__device__ __forceinline__ unsigned ns_linear_after(const NsTile &at, int what) { return at.k_blocks < 4 ? at.k_blocks : 4; }
+
 // One operand of a tile: 128 rows (64 where narrow) by 64 of K per stage. `plain`: the block in block
 // row rb, 32 KB at once. `flip`: read MN-major from the blocks above the diagonal (or, for X, always),
 // pieces of 64 K rows by 64 columns, 8 KB of hi and of lo each. What lies outside the panel is not
@@ -297,10 +304,16 @@ struct NsShared {
   NsTable table; // a copy: the roles index it at every tile, which is slow in constant memory
   uint32_t tmem;
   volatile unsigned gave_up;
+  unsigned written;     // draining warps that have written their part of a tile, over all tiles
+  unsigned linear_read[2]; // draining warps that have read their part of a linear term's stage, over all tiles
 };
 constexpr unsigned kNsSmem = kNsStages * kNsStageBytes + kNsEpilogueWarps * kNsPieceBytes + sizeof(NsShared);
 static_assert(kNsSmem <= 232448, "227 KB of shared memory per CTA");
 
+// a stage as an address for plain loads
+__device__ __forceinline__ const char *dynamic_stage(uint32_t stages, unsigned stage) {
+  return reinterpret_cast<const char *>(__cvta_shared_to_generic(stages + stage * kNsStageBytes));
+}
 // A role's place in the rings of stages and accumulators, kept from one product to the next.
 struct NsRing {
   uint32_t stages;      // shared memory
@@ -308,6 +321,12 @@ struct NsRing {
   unsigned first;       // this CTA's (pair's) first tile of the product at hand
   unsigned stage, phase; // of the next stage
   unsigned buf, turn;   // of the next accumulator
+  unsigned tiles;       // so far
+  __device__ __forceinline__ void skip_stages(unsigned n) {
+    stage += n;
+    phase ^= (stage / kNsStages) & 1;
+    stage %= kNsStages;
+  }
   __device__ __forceinline__ void next_stage() {
     if (++stage == kNsStages) {
       stage = 0;
@@ -326,7 +345,7 @@ template <int CTAS>
 __device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, int s, int what, volatile unsigned *gave_up) {
   unsigned target = s * (q.tiles[0] + q.tiles[1] + q.tiles[2]);
   for (int w = 0; w < what; ++w) target += q.tiles[w];
-  target *= CTAS * kNsEpilogueWarps;
+  target *= CTAS;
   const unsigned *counter = t.stored + (&q - t.mat);
   long long start = 0;
   for (unsigned spins = 0;; ++spins) {
@@ -343,6 +362,21 @@ __device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, in
     }
   }
   asm volatile("fence.acq_rel.gpu;" ::: "memory");
+  return true;
+}
+
+// The same for a counter in shared memory.
+__device__ __noinline__ bool ns_wait_counter(const volatile unsigned *counter, unsigned target, volatile unsigned *gave_up) {
+  const long long start = clock64();
+  for (unsigned spins = 0; *counter < target; ++spins)
+    if ((spins & 63) == 63) {
+      if (*gave_up) return false;
+      if (clock64() - start > kWaitCycles) {
+        *gave_up = 1;
+        return false;
+      }
+    }
+  __threadfence_block();
   return true;
 }
 
@@ -369,7 +403,25 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
     const unsigned flip_right = what == kGram ? 0 : what == kApply ? at.k_blocks : 2 * CTAS * (narrow ? at.j / 2 : at.j);
     if (!ns_wait_stored<CTAS>(t, q, s, what, &sh.gave_up)) return false;
     asm volatile("fence.proxy.async.global;" ::: "memory"); // panels are written with plain stores
-    for (unsigned k = 0; k < at.k_blocks; ++k) {
+    const unsigned k_linear = ns_linear_after(at, what);
+    for (unsigned k = 0; k <= at.k_blocks; ++k) {
+      if (k == k_linear && what != kGram) {
+        // the linear term, b A or a X: two block columns of this CTA's rows to a stage
+        const char *old = what == kPolynomial ? q.a : q.x[from];
+        const unsigned rb = at.i * CTAS + ring.rank, cbs = what == kPolynomial ? mcb : xcb;
+        const unsigned cb0 = narrow ? at.j : at.j * 2 * CTAS, cb_end = cb0 + (narrow ? 1 : 2 * CTAS);
+        for (unsigned c = 0; c < CTAS; ++c, ring.next_stage()) {
+          if (!barrier_wait(smem_address(&sh.empty[ring.stage]), ring.phase ^ 1, &sh.gave_up)) return false;
+          const uint32_t bar = smem_address(&sh.full[ring.stage]), dst = ring.stages + ring.stage * kNsStageBytes;
+          const unsigned first = cb0 + 2 * c;
+          unsigned n = 0; // block columns that exist
+          if (rb < rows)
+            while (n < 2 && first + n < cb_end && first + n < cbs) ++n;
+          barrier_expect(bar, n * 2 * kPanelHalf);
+          if (n) bulk_load(dst, old + panel_block(rb, first, cbs), n * 2 * kPanelHalf, bar); // neighbours in memory
+        }
+      }
+      if (k == at.k_blocks) break;
       if (!barrier_wait(smem_address(&sh.empty[ring.stage]), ring.phase ^ 1, &sh.gave_up)) return false;
       const uint32_t bar = smem_address(&sh.full[ring.stage]), dst = ring.stages + ring.stage * kNsStageBytes;
       const bool fl = k < flip_left, fr = k < flip_right;
@@ -395,7 +447,19 @@ __device__ bool ns_multiply(NsShared &sh, NsRing &ring, int what) {
     tile_at<CTAS>(t, what, tile, at);
     const unsigned flip_left = what == kGram ? 0 : 2 * CTAS * at.i;
     const unsigned flip_right = what == kGram ? 0 : what == kApply ? at.k_blocks : 2 * CTAS * (narrow ? at.j / 2 : at.j);
-    for (unsigned k = 0; k < at.k_blocks; ++k, ring.next_stage()) {
+    const unsigned k_linear = what == kGram ? ~0u : ns_linear_after(at, what);
+    for (unsigned k = 0; k <= at.k_blocks; ++k, ring.next_stage()) {
+      if (k == k_linear) {
+        // not for the tensor cores; but the second CTA's messages count every turn of the ring
+        if (CTAS > 1 && ring.rank != 0) {
+          for (int c = 0; c < CTAS; ++c, ring.next_stage()) {
+            if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.full[ring.stage]), ring.phase, &sh.gave_up))) return false;
+            if (elect_one()) barrier_arrive_at(smem_address(&sh.peer_full[ring.stage]), 0);
+            __syncwarp();
+          }
+        } else ring.skip_stages(CTAS);
+      }
+      if (k == at.k_blocks) break;
       const uint32_t full = smem_address(&sh.full[ring.stage]);
       if (!__all_sync(0xffffffffu, barrier_wait(full, ring.phase, &sh.gave_up))) return false;
       if (CTAS > 1 && ring.rank != 0) {
@@ -435,88 +499,82 @@ __device__ bool ns_multiply(NsShared &sh, NsRing &ring, int what) {
   return true;
 }
 
-// ---- the warps that drain: warp w takes rows 32 (w % 4) .. and half of the tile's columns, in groups of
-// 64 (one block column; 32 of one where narrow).
+// ---- the warps that drain: warp w takes rows 32 (w % 4) .. and a quarter of the tile's columns (64, 32 or
+// 16), 32 at a time.
 //
-// A lane holds a row, so it would touch 32 different lines per access to a panel; the warp's 32 rows of
-// a block lie in 4 KB without gaps, so they go through shared memory instead and a warp's access covers
-// four whole lines. The linear term (b A or a X) starts the sum: it is fetched while the first products
-// run.
+// A lane holds a row, so it would touch 32 different lines per access to a panel; the rows go through
+// shared memory instead and a warp's access covers whole 64-byte pieces of eight rows.
 template <int CTAS>
 __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last, char *piece) {
   constexpr unsigned kColumns = 128 * CTAS;
-  const float init = what == kPolynomial ? kNsB / kNsC * kSplitScale : kNsA * kSplitScale;
-  const float finish = what == kPolynomial ? kNsC * kSplitUnscale : kSplitUnscale;
+  constexpr int kGroups = 2 * CTAS; // of 16 columns
   const NsTable &t = sh.table;
-  const int from = s & 1;
-  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
+  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp >> 2;
   const unsigned row_in_tile = (warp & 3) * 32 + lane;
   const bool narrow = CTAS == 1 && t.narrow[what];
-  // a warp's pass over its rows of a group: `chunks` 16-byte pieces per row, 32 pieces at a time
-  const unsigned chunks = narrow ? 4 : 8, shift = narrow ? 2 : 3;
+  const unsigned columns = narrow ? 16 : 32 * CTAS;
+  const float init = what == kPolynomial ? kNsB / kNsC * kSplitScale : kNsA * kSplitScale;
+  const float finish = what == kPolynomial ? kNsC * kSplitUnscale : kSplitUnscale;
+  // a group's 32 columns: four 16-byte chunks of a row (two where narrow)
+  const unsigned shift = narrow ? 1 : 2, mask = (1u << shift) - 1;
   for (unsigned tile = ring.first; tile < t.tiles[what]; tile += gridDim.x / CTAS) {
     NsTile at;
     const NsMat &q = tile_at<CTAS>(t, what, tile, at);
     const unsigned rb = at.i * CTAS + ring.rank, col_blocks = panel_col_blocks(what == kApply ? q.n : q.m);
+    const unsigned col0 = at.j * ns_wide<CTAS>(narrow) + quarter * columns; // first column of the warp
+    const unsigned row = rb * 128 + row_in_tile;
     const bool rows_exist = rb < panel_row_blocks(q.m);
-    // the group's block column and its first chunk there
-    const unsigned cb0 = narrow ? at.j : (at.j * 2 + half) * CTAS, chunk0 = narrow ? half * 4 : 0;
-    float acc[64 * CTAS];
+    float acc[16 * kGroups];
 #pragma unroll
-    for (int i = 0; i < 64 * CTAS; ++i) acc[i] = 0.0f;
-    if (what != kGram) {
-      // other CTAs' work: the warp looks for itself that it is stored
-      bool ok = true;
-      if (lane == 0) ok = ns_wait_stored<CTAS>(t, q, s, what, &sh.gave_up);
-      if (!__all_sync(0xffffffffu, ok)) return false;
-      const char *old = what == kPolynomial ? q.a : q.x[from];
-#pragma unroll
-      for (int b = 0; b < CTAS; ++b) {
-        if (!rows_exist || cb0 + b >= col_blocks) continue;
-        const char *block = old + panel_block(rb, cb0 + b, col_blocks) + (warp & 3) * 4096;
+    for (int i = 0; i < 16 * kGroups; ++i) acc[i] = 0.0f;
+    const unsigned rounds = (at.k_blocks + kNsChunk - 1) / kNsChunk;
+    const unsigned k_linear = ns_linear_after(at, what);
 #pragma unroll 1
-        for (int part = 0; part < 2; ++part, block += kPanelHalf) { // past L1, which may hold an earlier step's values
-          uint4 v[8];
+    for (unsigned c = 0; c <= rounds; ++c) {
+      if (what != kGram && c == (k_linear + kNsChunk - 1) / kNsChunk) {
+        // the lane's row of the linear term, from the stage that holds the warp's block column
+        NsRing here = ring;
+        here.skip_stages(k_linear + (CTAS > 1 ? quarter / 2 : 0));
+        if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.full[here.stage]), here.phase, &sh.gave_up))) return false;
+        const unsigned block = CTAS > 1 ? (quarter & 1) : narrow ? 0 : quarter / 2;
+        const unsigned chunk0 = CTAS > 1 ? 0 : narrow ? quarter * 2 : (quarter & 1) * 4;
+        const char *old = dynamic_stage(ring.stages, here.stage) + block * (2 * kPanelHalf);
+        if (rows_exist && col0 / kPanelCols < col_blocks) {
 #pragma unroll
-          for (unsigned c = 0; c < 8; ++c) {
-            const unsigned item = c * 32 + lane;
-            if (c < chunks) v[c] = __ldcg(reinterpret_cast<const uint4 *>(block + panel_chunk(item >> shift, chunk0 + (item & (chunks - 1)))));
-          }
+          for (int part = 0; part < 2; ++part)
 #pragma unroll
-          for (unsigned c = 0; c < 8; ++c) {
-            const unsigned item = c * 32 + lane;
-            if (c < chunks) *reinterpret_cast<uint4 *>(piece + panel_chunk(item >> shift, chunk0 + (item & (chunks - 1)))) = v[c];
-          }
-          __syncwarp();
+            for (int k = 0; k < 2 * kGroups; ++k) {
+              if (k >= 2 && narrow) continue;
+              const uint4 h = *reinterpret_cast<const uint4 *>(old + part * kPanelHalf + panel_chunk(row_in_tile, chunk0 + k));
+              const unsigned w[4] = {h.x, h.y, h.z, h.w};
 #pragma unroll
-          for (unsigned c = 0; c < 8; ++c) {
-            if (c >= chunks) continue;
-            const uint4 h = *reinterpret_cast<const uint4 *>(piece + panel_chunk(lane, chunk0 + c));
-            const unsigned w[4] = {h.x, h.y, h.z, h.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-              acc[b * 64 + c * 8 + 2 * i] = __fmaf_rn(f.x, init, acc[b * 64 + c * 8 + 2 * i]);
-              acc[b * 64 + c * 8 + 2 * i + 1] = __fmaf_rn(f.y, init, acc[b * 64 + c * 8 + 2 * i + 1]);
+              for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                float &x = acc[k * 8 + 2 * i], &y = acc[k * 8 + 2 * i + 1];
+                x = __fmaf_rn(f.x, init, x);
+                y = __fmaf_rn(f.y, init, y);
+              }
             }
-          }
-          __syncwarp();
+        }
+        // the last of the warps that share the stage gives it back
+        __syncwarp();
+        if (lane == 0) {
+          __threadfence_block();
+          const unsigned mine = CTAS > 1 ? quarter / 2 : 0, share = kNsEpilogueWarps / CTAS;
+          if (atomicAdd(&sh.linear_read[mine], 1u) % share == share - 1) barrier_arrive(smem_address(&sh.empty[here.stage]));
         }
       }
-    }
-    const unsigned rounds = (at.k_blocks + kNsChunk - 1) / kNsChunk;
-#pragma unroll 1
-    for (unsigned c = 0; c < rounds; ++c) {
+      if (c == rounds) break;
       if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_full[ring.buf]), ring.turn, &sh.gave_up))) return false;
       tmem_fence_after();
-      const uint32_t columns = sh.tmem + (((warp & 3) * 32) << 16) + ring.buf * kColumns + half * (narrow ? 32 : 64 * CTAS);
+      const uint32_t from = sh.tmem + (((warp & 3) * 32) << 16) + ring.buf * kColumns + quarter * columns;
 #pragma unroll
-      for (int g = 0; g < 2 * CTAS; ++g) {
+      for (int g = 0; g < kGroups; ++g) {
         if (g > 0 && narrow) continue;
-        float v[32];
-        tmem_load32(columns + g * 32, v);
+        float v[16];
+        tmem_load16(from + g * 16, v);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[g * 32 + i] += v[i];
+        for (int i = 0; i < 16; ++i) acc[g * 16 + i] += v[i];
       }
       tmem_fence_before();
       __syncwarp();
@@ -526,79 +584,100 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
       }
       ring.next_accumulator();
     }
-    char *out = what == kGram ? q.a : what == kPolynomial ? q.b : q.x[from ^ 1];
-    const unsigned row = rb * 128 + row_in_tile;
-    const bool weights = what == kApply && last;
+    ring.skip_stages(at.k_blocks + (what == kGram ? 0 : CTAS));
+    if (rows_exist) {
+      if (what != kApply || !last) {
+        char *out = what == kGram ? q.a : what == kPolynomial ? q.b : q.x[(s & 1) ^ 1];
 #pragma unroll
-    for (int b = 0; b < CTAS; ++b) {
-      if (!rows_exist || cb0 + b >= col_blocks) continue;
-      if (!weights) {
-        char *block = out + panel_block(rb, cb0 + b, col_blocks) + (warp & 3) * 4096;
-        unsigned lo[32];
-        // hi goes out while lo waits in registers; padding stays zero (an operand read from beyond the
-        // panel may leave anything in the sums)
+        for (int u = 0; u < CTAS; ++u) { // 32 columns
+          const unsigned col = col0 + u * 32, cb = col / kPanelCols, chunk0 = (col % kPanelCols) / 8;
+          if (cb >= col_blocks) continue;
+          char *block = out + panel_block(rb, cb, col_blocks);
+          unsigned hi[16], lo[16];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          unsigned hi[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = acc[b * 64 + c * 8 + 2 * i] * finish, y = acc[b * 64 + c * 8 + 2 * i + 1] * finish;
+          for (int i = 0; i < 16; ++i) {
+            float x = acc[u * 32 + 2 * i] * finish, y = acc[u * 32 + 2 * i + 1] * finish;
+            // padding stays zero (an operand read from beyond the panel may leave anything in the sums)
             if (row >= q.m) x = y = 0.0f;
             const __half2 h = __floats2half2_rn(x, y);
             const float2 f = __half22float2(h);
             const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
             hi[i] = *reinterpret_cast<const unsigned *>(&h);
-            lo[c * 4 + i] = *reinterpret_cast<const unsigned *>(&l);
+            lo[i] = *reinterpret_cast<const unsigned *>(&l);
           }
-          if (c < chunks) *reinterpret_cast<uint4 *>(piece + panel_chunk(lane, chunk0 + c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        }
-        __syncwarp();
-#pragma unroll 1
-        for (int part = 0; part < 2; ++part, block += kPanelHalf) {
 #pragma unroll
-          for (unsigned c = 0; c < 8; ++c) {
-            if (c >= chunks) continue;
-            const unsigned item = c * 32 + lane, o = panel_chunk(item >> shift, chunk0 + (item & (chunks - 1)));
-            *reinterpret_cast<uint4 *>(block + o) = *reinterpret_cast<const uint4 *>(piece + o);
+          for (int part = 0; part < 2; ++part, block += kPanelHalf) {
+#pragma unroll
+            for (unsigned c = 0; c < 4; ++c) {
+              const unsigned *w = (part ? lo : hi) + c * 4;
+              if (c <= mask) *reinterpret_cast<uint4 *>(piece + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (unsigned k = 0; k < 4; ++k) {
+              const unsigned item = k * 32 + lane, r = item >> shift, c = item & mask;
+              if (k <= mask)
+                *reinterpret_cast<uint4 *>(block + panel_chunk((warp & 3) * 32 + r, chunk0 + c)) =
+                    *reinterpret_cast<const uint4 *>(piece + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+            }
+            __syncwarp();
           }
-          __syncwarp();
-          if (part == 1) break;
-#pragma unroll
-          for (unsigned c = 0; c < 8; ++c)
-            if (c < chunks)
-              *reinterpret_cast<uint4 *>(piece + panel_chunk(lane, chunk0 + c)) =
-                  make_uint4(lo[c * 4], lo[c * 4 + 1], lo[c * 4 + 2], lo[c * 4 + 3]);
-          __syncwarp();
         }
-        continue;
-      }
-      // the weights (or the output): 32 x 32 through shared memory, then 32 neighbours to an access, along
-      // the matrix's rows as they are stored
-      const float scale = g_ns_gave_up ? NAN : finish * kSplitUnscale * q.rate;
-      float *mine = reinterpret_cast<float *>(piece);
+      } else {
+        // the weights (or the output), along the matrix's rows as they are stored: the lanes' rows where it
+        // was turned, else 16 columns of two rows through shared memory
+        const float scale = g_ns_gave_up ? NAN : finish * kSplitUnscale * q.rate;
+        float *mine = reinterpret_cast<float *>(piece);
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (g > 0 && narrow) continue;
+        for (int g = 0; g < kGroups; ++g) {
+          if (g > 0 && narrow) continue;
+          const unsigned c0 = col0 + g * 16;
+          if (q.turned) {
+            float *w = q.w + (u64)c0 * q.m + row;
+            if (row < q.m)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mine[lane * 32 + (i ^ lane)] = acc[b * 64 + g * 32 + i];
-        __syncwarp();
-        const unsigned row0 = rb * 128 + (warp & 3) * 32, col0 = (cb0 + b) * kPanelCols + chunk0 * 8 + g * 32;
-        const unsigned outer0 = q.turned ? col0 : row0, inner = (q.turned ? row0 : col0) + lane;
-        const unsigned outer_end = q.turned ? q.n : q.m, inner_end = q.turned ? q.m : q.n;
-        if (inner < inner_end) {
-          float *w = q.w + (u64)outer0 * inner_end + inner;
-          const unsigned count = outer_end > outer0 ? (outer_end - outer0 < 32 ? outer_end - outer0 : 32) : 0;
+              for (int i = 0; i < 16; ++i, w += q.m)
+                if (c0 + i < q.n) {
+                  const float x = scale * acc[g * 16 + i];
+                  *w = q.keep == 0.0f ? -x : q.keep * *w - x;
+                }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mine[lane * 16 + (i ^ (lane & 15))] = acc[g * 16 + i];
+            __syncwarp();
+            const unsigned col = c0 + (lane & 15), r0 = lane >> 4, row0 = rb * 128 + (warp & 3) * 32;
+            float *w = q.w + (u64)(row0 + r0) * q.n + col;
+            if (col < q.n)
 #pragma unroll 4
-          for (unsigned r = 0; r < count; ++r, w += inner_end) {
-            const float x = scale * mine[q.turned ? lane * 32 + (r ^ lane) : r * 32 + (lane ^ r)];
-            *w = q.keep == 0.0f ? -x : q.keep * *w - x;
+              for (unsigned r = r0; r < 32; r += 2, w += 2 * (u64)q.n)
+                if (row0 + r < q.m) {
+                  const float x = scale * mine[r * 16 + ((lane & 15) ^ (r & 15))];
+                  *w = q.keep == 0.0f ? -x : q.keep * *w - x;
+                }
+            __syncwarp();
           }
         }
-        __syncwarp();
       }
     }
     __syncwarp();
-    if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(t.stored + (&q - t.mat)) : "memory");
+    if (lane == 0) {
+      __threadfence_block();
+      atomicAdd(&sh.written, 1u);
+    }
+  }
+  return true;
+}
+
+// ---- the thread that tells the other CTAs: its fence waits for the stores of the draining warps, which go
+// on to their next tile meanwhile (a release of their own cost each of them 1,500 to 2,000 cycles a tile)
+template <int CTAS>
+__device__ bool ns_publish(NsShared &sh, NsRing &ring, int what) {
+  const NsTable &t = sh.table;
+  for (unsigned tile = ring.first; tile < t.tiles[what]; tile += gridDim.x / CTAS) {
+    NsTile at;
+    const NsMat &q = tile_at<CTAS>(t, what, tile, at);
+    if (!ns_wait_counter(&sh.written, ++ring.tiles * kNsEpilogueWarps, &sh.gave_up)) return false;
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(t.stored + (&q - t.mat)) : "memory");
   }
   return true;
 }
@@ -610,7 +689,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
   const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (unsigned i = threadIdx.x; i < sizeof(NsTable) / 4; i += kNsThreads)
     reinterpret_cast<unsigned *>(&sh.table)[i] = reinterpret_cast<const unsigned *>(&param)[i];
-  NsRing ring = {smem_address(dynamic_smem), CTAS == 1 ? 0 : blockIdx.x % CTAS, 0, 0, 0, 0, 0};
+  NsRing ring = {smem_address(dynamic_smem), CTAS == 1 ? 0 : blockIdx.x % CTAS, 0, 0, 0, 0, 0, 0};
   if (threadIdx.x == 0) {
     for (int s = 0; s < kNsStages; ++s) {
       barrier_init(smem_address(&sh.full[s]), 1);
@@ -622,7 +701,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
       barrier_init(smem_address(&sh.acc_empty[b]), kNsEpilogueWarps * CTAS);
     }
     barrier_init(smem_address(&sh.drained), 1);
-    sh.gave_up = 0;
+    sh.gave_up = sh.written = sh.linear_read[0] = sh.linear_read[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
@@ -645,7 +724,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
     ring.first = (me + workers - before) % workers;
     if (warp < kNsEpilogueWarps) ok = ns_drain<CTAS>(sh, ring, s, what, s + 1 == steps, piece);
     else if (warp == kNsEpilogueWarps + 1) ok = ns_multiply<CTAS>(sh, ring, what);
-    else if (lane == 0) ok = ns_load<CTAS>(sh, ring, s, what);
+    else if (lane == 0) ok = warp == kNsEpilogueWarps ? ns_load<CTAS>(sh, ring, s, what) : ns_publish<CTAS>(sh, ring, what);
     before = (before + t.tiles[what]) % workers;
   }
   if (!ok && lane == 0) { // after a wait that ran out: what is in flight ends before its memory goes away

@@ -56,17 +56,6 @@ __device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
   hi = make_uint4(h[0], h[1], h[2], h[3]);
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
-__device__ __forceinline__ void join8(const uint4 &hi, const uint4 &lo, float *v) {
-  const unsigned h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&l[i]));
-    v[2 * i] = a.x + b.x;
-    v[2 * i + 1] = a.y + b.y;
-  }
-}
-
 // ---- barriers ----------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t smem_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void barrier_init(uint32_t bar, unsigned count) {
@@ -174,17 +163,14 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, unsigned columns) { // 
 }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// 32 columns of the warp's 32 lanes (the wait belongs to the load: nothing may use the values before)
-__device__ __forceinline__ void tmem_load32(uint32_t tmem, float (&v)[32]) {
+// 16 columns of the warp's 32 lanes (the wait belongs to the load: nothing may use the values before)
+__device__ __forceinline__ void tmem_load16(uint32_t tmem, float (&v)[16]) {
   uint32_t *r = reinterpret_cast<uint32_t *>(v);
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-               "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
                "tcgen05.wait::ld.sync.aligned;"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-                 "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-                 "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                : "r"(tmem)
                : "memory");
 }
