@@ -588,38 +588,46 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
     if (rows_exist) {
       if (what != kApply || !last) {
         char *out = what == kGram ? q.a : what == kPolynomial ? q.b : q.x[(s & 1) ^ 1];
+        if (rb * 128 + 128 > q.m && row >= q.m) {
+          // padding stays zero (an operand read from beyond the panel may leave anything in the sums)
+#pragma unroll
+          for (int i = 0; i < 16 * kGroups; ++i) acc[i] = 0.0f;
+        }
 #pragma unroll
         for (int u = 0; u < CTAS; ++u) { // 32 columns
           const unsigned col = col0 + u * 32, cb = col / kPanelCols, chunk0 = (col % kPanelCols) / 8;
           if (cb >= col_blocks) continue;
-          char *block = out + panel_block(rb, cb, col_blocks);
-          unsigned hi[16], lo[16];
+          // where the lane writes and reads the piece, and its first line in the panel; the k-th of its up to
+          // four 16-byte chunks lies k * 32 / chunks rows on
+          char *const mine = piece + lane * 64, *const theirs = piece + (lane >> shift) * 64 +
+                                                                (((lane & mask) ^ ((lane >> (shift + 1)) & 3)) << 4);
+          char *line = out + panel_block(rb, cb, col_blocks) + panel_chunk((warp & 3) * 32 + (lane >> shift), chunk0 + (lane & mask));
+          const unsigned piece_step = narrow ? 1024 : 512, line_step = 2 * piece_step;
+          unsigned lo[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float x = acc[u * 32 + 2 * i] * finish, y = acc[u * 32 + 2 * i + 1] * finish;
-            // padding stays zero (an operand read from beyond the panel may leave anything in the sums)
-            if (row >= q.m) x = y = 0.0f;
-            const __half2 h = __floats2half2_rn(x, y);
-            const float2 f = __half22float2(h);
-            const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-            hi[i] = *reinterpret_cast<const unsigned *>(&h);
-            lo[i] = *reinterpret_cast<const unsigned *>(&l);
-          }
-#pragma unroll
-          for (int part = 0; part < 2; ++part, block += kPanelHalf) {
+          for (int part = 0; part < 2; ++part, line += kPanelHalf) {
 #pragma unroll
             for (unsigned c = 0; c < 4; ++c) {
-              const unsigned *w = (part ? lo : hi) + c * 4;
-              if (c <= mask) *reinterpret_cast<uint4 *>(piece + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              if (c > mask) continue;
+              unsigned w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (part == 0) {
+                  const float x = acc[u * 32 + c * 8 + 2 * i] * finish, y = acc[u * 32 + c * 8 + 2 * i + 1] * finish;
+                  const __half2 h = __floats2half2_rn(x, y);
+                  const float2 f = __half22float2(h);
+                  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+                  w[i] = *reinterpret_cast<const unsigned *>(&h);
+                  lo[c * 4 + i] = *reinterpret_cast<const unsigned *>(&l);
+                } else w[i] = lo[c * 4 + i];
+              }
+              *reinterpret_cast<uint4 *>(mine + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             __syncwarp();
 #pragma unroll
-            for (unsigned k = 0; k < 4; ++k) {
-              const unsigned item = k * 32 + lane, r = item >> shift, c = item & mask;
+            for (unsigned k = 0; k < 4; ++k)
               if (k <= mask)
-                *reinterpret_cast<uint4 *>(block + panel_chunk((warp & 3) * 32 + r, chunk0 + c)) =
-                    *reinterpret_cast<const uint4 *>(piece + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-            }
+                *reinterpret_cast<uint4 *>(line + k * line_step) = *reinterpret_cast<const uint4 *>(theirs + k * piece_step);
             __syncwarp();
           }
         }
