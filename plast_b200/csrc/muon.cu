@@ -45,7 +45,9 @@ struct MuonTable {
   MuonMat mat[kMuonMax];
   int count;
   unsigned total;     // CTAs of the launch at hand
-  unsigned *stored;   // per matrix: CTAs that have stored their part of a tile, over all products so far
+  unsigned *tickets, ticket_count; // see NsTable
+  float4 *parts;
+  unsigned *stored;   // per matrix: draining warps that have stored their part of a tile, over all products so far
   float mu, epsilon;
   int nesterov;
 };
@@ -99,6 +101,8 @@ __global__ void __launch_bounds__(kMuonThreads) muon_norm_kernel(const __grid_co
   __shared__ double part[kMuonThreads];
   double sum = 0.0;
   for (unsigned i = threadIdx.x; i < q.chunks; i += kMuonThreads) sum += q.partial[1 + i];
+  if (blockIdx.x == 0)
+    for (unsigned i = threadIdx.x; i < t.ticket_count; i += kMuonThreads) t.tickets[i] = 0;
   part[threadIdx.x] = sum;
   __syncthreads();
   for (int o = kMuonThreads / 2; o; o >>= 1) {
@@ -163,14 +167,18 @@ __global__ void __launch_bounds__(kMuonThreads) muon_load_kernel(const __grid_co
 // A and B are symmetric: only tiles on and above the diagonal are computed and stored. An operand
 // block below it is fetched as the block above it and read MN-major, which is its transpose.
 //
-// (Folding the linear terms into the operands' diagonals would save the epilogues a read, but rounds a
-// number near 3.4 to 22 bits where b A + c A A is small: 3 to 6e-6 off instead of 1.1 to 1.5e-6.)
+// What is kept of A and B is moved towards 0 along the diagonal, S = A - T I and Q = B + s I:
+//   c A A + b A = c S S + (b + 2 c T) S + ((b + 2 c T) T - c T^2) I,   X = (a - s) X + Q X
+// With singular values of X near 1, A is near I and B near -2.74 I, and a X + B X would lose two bits to
+// cancellation, of numbers that have 22: 2e-6 off on 64 x 1000, 6e-7 with T = 0.7, s = 2.3 (plain fp32:
+// 1.3e-6). All the way (T = -b / 2c, s = a: no linear terms) A and B start near -1.2 I and 3.4 I
+// instead, and their rounding hurts: 3 to 6e-6.
 //
 // One launch goes through all products of all matrices. A persistent CTA takes every gridDim-th tile,
 // of 128 x 128 (or 128 x 64); a pair of CTAs (CTAS = 2) tiles of 256 x 256, each CTA holding half of
 // either operand. One thread brings 64 KB stages (64 of K, hi and lo of both operands) with bulk
 // copies, one warp (of the pair) issues the twelve tcgen05.mma of a stage, small products first, and
-// sixteen warps drain the accumulators. Tensor-core accumulation truncates; every kNsChunk stages the
+// sixteen warps drain the accumulators. Tensor-core accumulation truncates; every one or two stages the
 // accumulator (one of two in tensor memory) is therefore added in fp32 registers, rounded to nearest,
 // while the next one fills.
 //
@@ -181,10 +189,15 @@ enum MuonProduct { kGram = 0, kPolynomial = 1, kApply = 2 };
 constexpr int kNsStages = 3;
 constexpr unsigned kNsStageBytes = 4 * kPanelHalf; // left hi, left lo, right hi, right lo
 constexpr int kNsEpilogueWarps = 16, kNsThreads = (kNsEpilogueWarps + 3) * 32;
-#ifndef NS_CHUNK
-#define NS_CHUNK 2
-#endif
-constexpr int kNsChunk = NS_CHUNK;
+// Stages summed in tensor memory before they are added in registers (for pairs one costs 15 %).
+template <int CTAS> constexpr int kNsChunk = CTAS == 1 ? 1 : 2;
+// The truncation of such a sum shortens it by about one (single) to three units of 2^-23 on average,
+// which the addition in registers puts back: it multiplies by this.
+template <int CTAS> constexpr float kNsRaise = 1.0f + (CTAS == 1 ? 1 : 3) / 8388608.0f;
+// What the diagonals of A and B are moved by, see above, and what follows for the linear terms.
+constexpr double kNsT = 0.7, kNsS = 2.3;
+constexpr double kNsLinear = (double)kNsB + 2.0 * kNsC * kNsT; // of B in A - T
+constexpr unsigned kNsMostParts = 8;   // of a split K
 constexpr unsigned kNsPieceBytes = 2048; // per draining warp: 32 rows of 32 columns of hi or lo, or 32 x 16 floats
 
 struct NsMat {
@@ -192,12 +205,16 @@ struct NsMat {
   float *w;
   float keep, rate;
   unsigned m, n;
-  unsigned first_tile[3], tiles[3];
-  unsigned turned; // stored as n x m
+  unsigned first_tile[3], tiles[3]; // a tile whose K is split counts once for each part
+  unsigned char splits[3];
+  bool turned; // stored as n x m
 };
 struct NsTable {
   NsMat mat[kMuonMax];
   unsigned *stored;
+  unsigned *tickets; // of tiles whose K is split: per draining warp, how many parts are there
+  float4 *parts;     // their sums
+  unsigned room;     // tiles, per product
   unsigned tiles[3]; // of each product
   int narrow[3];     // tiles of 128 x 64 instead of 128 x 128
   int count;
@@ -214,8 +231,15 @@ template <int CTAS> inline u64 ns_tiles_of(unsigned m, unsigned n, int what, boo
   return what == kApply ? r * c : r * c - per_diagonal * (r * (r - 1) / 2); // row i starts at its diagonal block
 }
 
+// K blocks of one part (single CTAs only)
+__host__ __device__ inline unsigned ns_part_blocks(unsigned k_blocks, unsigned parts) {
+  return (k_blocks + parts - 1) / parts;
+}
+
 struct NsTile {
-  unsigned i, j, k_blocks; // tile row, tile column, K / 64
+  unsigned i, j;         // tile row, tile column
+  unsigned k0, k_blocks; // first K block (of 64) and their number
+  unsigned part, parts;  // of K
 };
 template <int CTAS>
 __device__ __forceinline__ const NsMat &tile_at(const NsTable &t, int what, unsigned tile, NsTile &out) {
@@ -227,6 +251,18 @@ __device__ __forceinline__ const NsMat &tile_at(const NsTable &t, int what, unsi
   const NsMat &q = t.mat[lo];
   const unsigned wide = ns_wide<CTAS>(t.narrow[what]), across = ns_along(what == kApply ? q.n : q.m, wide);
   unsigned at = tile - q.first_tile[what];
+  const unsigned k_all = panel_col_blocks(what == kGram ? q.n : q.m);
+  out.parts = CTAS == 1 ? q.splits[what] : 1;
+  out.part = 0;
+  out.k0 = 0;
+  out.k_blocks = k_all;
+  if (CTAS == 1 && out.parts > 1) {
+    out.part = at % out.parts;
+    at /= out.parts;
+    const unsigned each = ns_part_blocks(k_all, out.parts);
+    out.k0 = out.part * each;
+    out.k_blocks = k_all - out.k0 < each ? k_all - out.k0 : each;
+  }
   if (what == kApply) {
     out.i = at / across;
     out.j = at % across;
@@ -241,13 +277,16 @@ __device__ __forceinline__ const NsMat &tile_at(const NsTable &t, int what, unsi
     out.i = i;
     out.j = i * per_diagonal + at;
   }
-  out.k_blocks = panel_col_blocks(what == kGram ? q.n : q.m);
   return q;
 }
 
 // The linear term of a tile comes through the same ring of stages, after the first four K blocks (or
-// after the last): by then the draining warps are done with the tile before and take it at once.
-__device__ __forceinline__ unsigned ns_linear_after(const NsTile &at, int what) { return at.k_blocks < 4 ? at.k_blocks : 4; }
+// after the last): by then the draining warps are done with the tile before and take it at once. The
+// gram matrix has none, nor have the other parts of a split K.
+__device__ __forceinline__ unsigned ns_linear_after(const NsTile &at, int what) {
+  if (what == kGram || at.part != 0) return ~0u;
+  return at.k_blocks < 4 ? at.k_blocks : 4;
+}
 
 // One operand of a tile: 128 rows (64 where narrow) by 64 of K per stage. `plain`: the block in block
 // row rb, 32 KB at once. `flip`: read MN-major from the blocks above the diagonal (or, for X, always),
@@ -343,9 +382,9 @@ struct NsRing {
 // one fence: an acquiring load would fence at every turn.
 template <int CTAS>
 __device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, int s, int what, volatile unsigned *gave_up) {
-  unsigned target = s * (q.tiles[0] + q.tiles[1] + q.tiles[2]);
-  for (int w = 0; w < what; ++w) target += q.tiles[w];
-  target *= CTAS;
+  unsigned target = 0;
+  for (int w = 0; w < 3; ++w) target += q.tiles[w] / q.splits[w] * (s + (w < what));
+  target *= CTAS * kNsEpilogueWarps;
   const unsigned *counter = t.stored + (&q - t.mat);
   long long start = 0;
   for (unsigned spins = 0;; ++spins) {
@@ -400,12 +439,12 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
                                        what == kPolynomial ? mcb : xcb, narrow);
     // K blocks before these are above the diagonal
     const unsigned flip_left = what == kGram ? 0 : 2 * CTAS * at.i;
-    const unsigned flip_right = what == kGram ? 0 : what == kApply ? at.k_blocks : 2 * CTAS * (narrow ? at.j / 2 : at.j);
+    const unsigned flip_right = what == kGram ? 0 : what == kApply ? ~0u : 2 * CTAS * (narrow ? at.j / 2 : at.j);
     if (!ns_wait_stored<CTAS>(t, q, s, what, &sh.gave_up)) return false;
     asm volatile("fence.proxy.async.global;" ::: "memory"); // panels are written with plain stores
     const unsigned k_linear = ns_linear_after(at, what);
     for (unsigned k = 0; k <= at.k_blocks; ++k) {
-      if (k == k_linear && what != kGram) {
+      if (k == k_linear) {
         // the linear term, b A or a X: two block columns of this CTA's rows to a stage
         const char *old = what == kPolynomial ? q.a : q.x[from];
         const unsigned rb = at.i * CTAS + ring.rank, cbs = what == kPolynomial ? mcb : xcb;
@@ -424,10 +463,11 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
       if (k == at.k_blocks) break;
       if (!barrier_wait(smem_address(&sh.empty[ring.stage]), ring.phase ^ 1, &sh.gave_up)) return false;
       const uint32_t bar = smem_address(&sh.full[ring.stage]), dst = ring.stages + ring.stage * kNsStageBytes;
-      const bool fl = k < flip_left, fr = k < flip_right;
+      const unsigned kb = at.k0 + k;
+      const bool fl = kb < flip_left, fr = kb < flip_right;
       barrier_expect(bar, (fl ? left.flip_bytes : left.plain_bytes) + (fr ? right.flip_bytes : right.plain_bytes));
-      load_operand(left, dst, k, fl, bar);
-      load_operand(right, dst + 2 * kPanelHalf, k, fr, bar);
+      load_operand(left, dst, kb, fl, bar);
+      load_operand(right, dst + 2 * kPanelHalf, kb, fr, bar);
       ring.next_stage();
     }
   }
@@ -446,8 +486,8 @@ __device__ bool ns_multiply(NsShared &sh, NsRing &ring, int what) {
     NsTile at;
     tile_at<CTAS>(t, what, tile, at);
     const unsigned flip_left = what == kGram ? 0 : 2 * CTAS * at.i;
-    const unsigned flip_right = what == kGram ? 0 : what == kApply ? at.k_blocks : 2 * CTAS * (narrow ? at.j / 2 : at.j);
-    const unsigned k_linear = what == kGram ? ~0u : ns_linear_after(at, what);
+    const unsigned flip_right = what == kGram ? 0 : what == kApply ? ~0u : 2 * CTAS * (narrow ? at.j / 2 : at.j);
+    const unsigned k_linear = ns_linear_after(at, what);
     for (unsigned k = 0; k <= at.k_blocks; ++k, ring.next_stage()) {
       if (k == k_linear) {
         // not for the tensor cores; but the second CTA's messages count every turn of the ring
@@ -467,13 +507,13 @@ __device__ bool ns_multiply(NsShared &sh, NsRing &ring, int what) {
         __syncwarp();
         continue;
       }
-      const bool first = k % kNsChunk == 0, last = k % kNsChunk == kNsChunk - 1 || k + 1 == at.k_blocks;
+      const bool first = k % kNsChunk<CTAS> == 0, last = k % kNsChunk<CTAS> == kNsChunk<CTAS> - 1 || k + 1 == at.k_blocks;
       if (first && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_empty[ring.buf]), ring.turn ^ 1, &sh.gave_up)))
         return false;
       if (CTAS > 1 && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.peer_full[ring.stage]), ring.phase, &sh.gave_up)))
         return false;
       tmem_fence_after();
-      const bool fl = k < flip_left, fr = k < flip_right;
+      const bool fl = at.k0 + k < flip_left, fr = at.k0 + k < flip_right;
       const uint32_t stage = ring.stages + ring.stage * kNsStageBytes;
       const uint64_t left = operand_desc(stage, kPanelHalf / 2, 1024);
       const uint64_t right = operand_desc(stage + 2 * kPanelHalf, kPanelHalf / 2, 1024);
@@ -513,7 +553,8 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
   const unsigned row_in_tile = (warp & 3) * 32 + lane;
   const bool narrow = CTAS == 1 && t.narrow[what];
   const unsigned columns = narrow ? 16 : 32 * CTAS;
-  const float init = what == kPolynomial ? kNsB / kNsC * kSplitScale : kNsA * kSplitScale;
+  const float init = (float)(what == kPolynomial ? kNsLinear / kNsC : (double)kNsA - kNsS) * kSplitScale;
+  const float diagonal = (float)(what == kGram ? -kNsT : what == kPolynomial ? kNsLinear * kNsT - kNsC * kNsT * kNsT + kNsS : 0.0) * kSplitScale;
   const float finish = what == kPolynomial ? kNsC * kSplitUnscale : kSplitUnscale;
   // a group's 32 columns: four 16-byte chunks of a row (two where narrow)
   const unsigned shift = narrow ? 1 : 2, mask = (1u << shift) - 1;
@@ -527,11 +568,11 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
     float acc[16 * kGroups];
 #pragma unroll
     for (int i = 0; i < 16 * kGroups; ++i) acc[i] = 0.0f;
-    const unsigned rounds = (at.k_blocks + kNsChunk - 1) / kNsChunk;
+    const unsigned rounds = (at.k_blocks + kNsChunk<CTAS> - 1) / kNsChunk<CTAS>;
     const unsigned k_linear = ns_linear_after(at, what);
 #pragma unroll 1
     for (unsigned c = 0; c <= rounds; ++c) {
-      if (what != kGram && c == (k_linear + kNsChunk - 1) / kNsChunk) {
+      if (k_linear != ~0u && c == (k_linear + kNsChunk<CTAS> - 1) / kNsChunk<CTAS>) {
         // the lane's row of the linear term, from the stage that holds the warp's block column
         NsRing here = ring;
         here.skip_stages(k_linear + (CTAS > 1 ? quarter / 2 : 0));
@@ -574,7 +615,7 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
         float v[16];
         tmem_load16(from + g * 16, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[g * 16 + i] += v[i];
+        for (int i = 0; i < 16; ++i) acc[g * 16 + i] = __fmaf_rn(v[i], kNsRaise<CTAS>, acc[g * 16 + i]);
       }
       tmem_fence_before();
       __syncwarp();
@@ -584,8 +625,48 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
       }
       ring.next_accumulator();
     }
-    ring.skip_stages(at.k_blocks + (what == kGram ? 0 : CTAS));
-    if (rows_exist) {
+    ring.skip_stages(at.k_blocks + (k_linear == ~0u ? 0 : CTAS));
+    bool mine = true; // this warp stores its part of the tile
+    if (CTAS == 1 && at.parts > 1) {
+      // The warp's sums go to memory; the last of the parts' warps (a ticket) adds all of them up, always in
+      // the same order. Each product has its own room, where a place belongs to one matrix: another matrix
+      // may be ahead by any number of products.
+      const unsigned whole = ((what * t.room + tile - at.part)) * kNsEpilogueWarps + warp; // the tile's first part
+      float4 *out = t.parts + ((u64)whole + at.part * kNsEpilogueWarps) * (8 * 32) + lane;
+#pragma unroll
+      for (int i = 0; i < 4 * kGroups; ++i)
+        if (i < 4 || !narrow) out[i * 32] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+      __syncwarp();
+      unsigned before = 0;
+      if (lane == 0) {
+        asm volatile("fence.acq_rel.gpu;" ::: "memory");
+        before = atomicAdd(t.tickets + whole, 1u);
+        if (before == at.parts - 1) t.tickets[whole] = 0; // for the next product
+        asm volatile("fence.acq_rel.gpu;" ::: "memory");
+      }
+      mine = __shfl_sync(0xffffffffu, before, 0) == at.parts - 1;
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < 16 * kGroups; ++i) acc[i] = 0.0f;
+        const float4 *in = t.parts + (u64)whole * (8 * 32) + lane;
+#pragma unroll 1
+        for (unsigned part = 0; part < at.parts; ++part, in += kNsEpilogueWarps * 8 * 32) {
+          float4 v[4 * kGroups];
+#pragma unroll
+          for (int i = 0; i < 4 * kGroups; ++i)
+            if (i < 4 || !narrow) v[i] = __ldcg(in + i * 32);
+#pragma unroll
+          for (int i = 0; i < 4 * kGroups; ++i)
+            if (i < 4 || !narrow) {
+              acc[4 * i] += v[i].x;
+              acc[4 * i + 1] += v[i].y;
+              acc[4 * i + 2] += v[i].z;
+              acc[4 * i + 3] += v[i].w;
+            }
+        }
+      }
+    }
+    if (rows_exist && mine) {
       if (what != kApply || !last) {
         char *out = what == kGram ? q.a : what == kPolynomial ? q.b : q.x[(s & 1) ^ 1];
         if (rb * 128 + 128 > q.m && row >= q.m) {
@@ -603,6 +684,7 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
                                                                 (((lane & mask) ^ ((lane >> (shift + 1)) & 3)) << 4);
           char *line = out + panel_block(rb, cb, col_blocks) + panel_chunk((warp & 3) * 32 + (lane >> shift), chunk0 + (lane & mask));
           const unsigned piece_step = narrow ? 1024 : 512, line_step = 2 * piece_step;
+          const bool on_diagonal = what != kApply && col / 32 == row / 32;
           unsigned lo[16];
 #pragma unroll
           for (int part = 0; part < 2; ++part, line += kPanelHalf) {
@@ -613,7 +695,11 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 if (part == 0) {
-                  const float x = acc[u * 32 + c * 8 + 2 * i] * finish, y = acc[u * 32 + c * 8 + 2 * i + 1] * finish;
+                  float x = acc[u * 32 + c * 8 + 2 * i] * finish, y = acc[u * 32 + c * 8 + 2 * i + 1] * finish;
+                  if (on_diagonal) {
+                    if (col + c * 8 + 2 * i == row && row < q.m) x += diagonal;
+                    if (col + c * 8 + 2 * i + 1 == row && row < q.m) y += diagonal;
+                  }
                   const __half2 h = __floats2half2_rn(x, y);
                   const float2 f = __half22float2(h);
                   const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
@@ -669,6 +755,9 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
     }
     __syncwarp();
     if (lane == 0) {
+      if (CTAS == 1 && at.parts > 1) { // parts of one tile end in different CTAs: every warp tells for itself
+        if (mine) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(t.stored + (&q - t.mat)) : "memory");
+      }
       __threadfence_block();
       atomicAdd(&sh.written, 1u);
     }
@@ -685,7 +774,8 @@ __device__ bool ns_publish(NsShared &sh, NsRing &ring, int what) {
     NsTile at;
     const NsMat &q = tile_at<CTAS>(t, what, tile, at);
     if (!ns_wait_counter(&sh.written, ++ring.tiles * kNsEpilogueWarps, &sh.gave_up)) return false;
-    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(t.stored + (&q - t.mat)) : "memory");
+    if (at.parts == 1)
+      asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(t.stored + (&q - t.mat)), "n"(kNsEpilogueWarps) : "memory");
   }
   return true;
 }
@@ -784,7 +874,11 @@ static u64 scratch_bytes(const MuonMat &q) {
   return 2 * panel_bytes(q.m, q.n) + 2 * panel_bytes(q.m, q.m) + padded((u64)(q.chunks + 1) * 8);
 }
 
-// Numbers the CTAs (or tiles) of a launch over the matrices.
+// Tickets and sums of the tiles whose K is split: at most one turn of the GPU, for each product.
+static u64 ns_ticket_bytes() { return padded((u64)3 * sm_count() * kNsEpilogueWarps * sizeof(unsigned)); }
+static u64 ns_parts_bytes() { return padded((u64)3 * sm_count() * kNsEpilogueWarps * 8 * 32 * sizeof(float4)); }
+
+// Numbers the CTAs of a launch over the matrices.
 template <class Blocks>
 static void number(MuonTable &t, Blocks blocks) {
   u64 n = 0;
@@ -807,11 +901,55 @@ static bool launch_over(MuonTable &t, Blocks blocks, void (*kernel)(const MuonTa
   count_launch();
   return true;
 }
+// What a product over all matrices costs, in thousands of SM cycles as traced on a B200, for tiles and K
+// parts of one kind: K blocks of 64 take 1.7 (pairs, 256 x 256), 1.25 (128 x 128) or 1.05 (128 x 64); a
+// tile ends with 3 that its CTA's next one does not hide, a split one with 14; the product as a whole
+// starts and ends with 9 (20 for pairs).
 template <int CTAS>
-static void run_steps(const MuonTable &mt, int steps) {
+static double ns_cost(const NsTable &t, int what, bool narrow, unsigned part_blocks, u64 *units) {
+  const double per_block = CTAS == 2 ? 1.7 : narrow ? 1.05 : 1.25;
+  double total = 0.0, longest = 0.0;
+  *units = 0;
+  for (int i = 0; i < t.count; ++i) {
+    const unsigned k_blocks = panel_col_blocks(what == kGram ? t.mat[i].n : t.mat[i].m), parts = ns_along(k_blocks, part_blocks);
+    const double one = std::min(k_blocks, part_blocks) * per_block + (parts > 1 ? 14.0 : 3.0);
+    const u64 n = ns_tiles_of<CTAS>(t.mat[i].m, t.mat[i].n, what, narrow) * parts;
+    *units += n;
+    total += (double)n * one;
+    longest = std::max(longest, one);
+  }
+  const double workers = (double)(sm_count() / CTAS), turns = ceil((double)*units / workers);
+  return std::max(longest, turns * total / (double)*units) + (CTAS == 2 ? 20.0 : 9.0);
+}
+// Chooses the tiles and K parts of a product; returns its cost.
+template <int CTAS>
+static double ns_shape(NsTable &t, int what, unsigned *part_blocks) {
+  unsigned longest = 0;
+  for (int i = 0; i < t.count; ++i) longest = std::max(longest, panel_col_blocks(what == kGram ? t.mat[i].n : t.mat[i].m));
+  u64 units = 0;
+  t.narrow[what] = 0;
+  *part_blocks = longest;
+  double best = ns_cost<CTAS>(t, what, false, longest, &units);
+  for (int narrow = 0; narrow < (CTAS == 1 ? 2 : 0); ++narrow)
+    for (unsigned parts = 1; parts <= kNsMostParts; ++parts) {
+      const unsigned blocks = parts == 1 ? longest : ns_part_blocks(longest, parts);
+      const double cost = ns_cost<CTAS>(t, what, narrow != 0, blocks, &units);
+      if (cost < best && (parts == 1 || units <= (u64)sm_count())) { // the parts' sums have room for one turn
+        best = cost;
+        t.narrow[what] = narrow;
+        *part_blocks = blocks;
+      }
+    }
+  return best;
+}
+
+static NsTable steps_table(const MuonTable &mt) {
   NsTable t = {};
   t.count = mt.count;
   t.stored = mt.stored;
+  t.tickets = mt.tickets;
+  t.parts = mt.parts;
+  t.room = (unsigned)sm_count();
   for (int i = 0; i < mt.count; ++i) {
     const MuonMat &q = mt.mat[i];
     NsMat &d = t.mat[i];
@@ -826,16 +964,21 @@ static void run_steps(const MuonTable &mt, int steps) {
     d.n = q.n;
     d.turned = q.rows > q.cols;
   }
+  return t;
+}
+
+template <int CTAS>
+static void run_steps(NsTable &t, int steps) {
   for (int what = kGram; what <= kApply; ++what) {
-    // tiles of 128 x 64 where the GPU has an SM for each
+    unsigned part_blocks = 0;
+    ns_shape<CTAS>(t, what, &part_blocks);
     u64 n = 0;
-    for (int i = 0; i < t.count; ++i) n += ns_tiles_of<1>(t.mat[i].m, t.mat[i].n, what, true);
-    t.narrow[what] = CTAS == 1 && n <= (u64)sm_count();
-    n = 0;
     for (int i = 0; i < t.count; ++i) {
       NsMat &q = t.mat[i];
+      const unsigned k_blocks = panel_col_blocks(what == kGram ? q.n : q.m);
+      q.splits[what] = (unsigned char)ns_along(k_blocks, part_blocks);
       q.first_tile[what] = (unsigned)n;
-      q.tiles[what] = (unsigned)ns_tiles_of<CTAS>(q.m, q.n, what, t.narrow[what]);
+      q.tiles[what] = (unsigned)ns_tiles_of<CTAS>(q.m, q.n, what, t.narrow[what]) * q.splits[what];
       n += q.tiles[what];
     }
     t.tiles[what] = (unsigned)n;
@@ -887,17 +1030,25 @@ static void run_group(MuonTable &t, char *base, int steps) {
     q.partial = (double *)take(padded((u64)(q.chunks + 1) * 8));
   }
   t.stored = (unsigned *)take(256);
+  t.tickets = (unsigned *)take(ns_ticket_bytes());
+  t.parts = (float4 *)take(ns_parts_bytes());
+  t.ticket_count = (unsigned)(ns_ticket_bytes() / sizeof(unsigned));
   auto chunks = [](const MuonMat &q) { return (u64)q.chunks; };
   auto blocks = [](const MuonMat &q) { return (u64)panel_row_blocks(q.m) * panel_col_blocks(q.n); };
   if (!launch_over(t, chunks, muon_momentum_kernel)) return;
   if (!launch_over(t, [](const MuonMat &) { return (u64)1; }, muon_norm_kernel)) return;
   if (!launch_over(t, blocks, muon_load_kernel)) return;
   if (steps > 0) {
-    u64 tiles = 0;
-    for (int i = 0; i < t.count; ++i) tiles += ns_tiles_of<2>(t.mat[i].m, t.mat[i].n, kApply, false);
-    const bool pairs = tuned(kTuneMuonPairs) >= 0 ? tuned(kTuneMuonPairs) != 0 : tiles >= (u64)sm_count() / 2;
-    if (pairs) run_steps<2>(t, steps);
-    else run_steps<1>(t, steps);
+    NsTable table = steps_table(t);
+    double single = 0.0, paired = 0.0;
+    unsigned blocks;
+    for (int what = kGram; what <= kApply; ++what) {
+      single += ns_shape<1>(table, what, &blocks);
+      paired += ns_shape<2>(table, what, &blocks);
+    }
+    const bool pairs = tuned(kTuneMuonPairs) >= 0 ? tuned(kTuneMuonPairs) != 0 : paired < single;
+    if (pairs) run_steps<2>(table, steps);
+    else run_steps<1>(table, steps);
     return;
   }
   launch_over(t, chunks, muon_store_kernel);
@@ -908,7 +1059,7 @@ static void run_matrices(const std::vector<MuonMat> &mats, float mu, float epsil
   u64 largest = 0;
   std::vector<size_t> ends;
   for (size_t i = 0; i < mats.size();) {
-    u64 bytes = 256; // the counters of stored tiles
+    u64 bytes = 256 + ns_ticket_bytes() + ns_parts_bytes();
     size_t k = i;
     while (k < mats.size() && k - i < (size_t)kMuonMax && (k == i || bytes + scratch_bytes(mats[k]) <= kMuonScratch))
       bytes += scratch_bytes(mats[k++]);
