@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kMuonThreads) muon_load_kernel(const __grid_co
 enum MuonProduct { kGram = 0, kPolynomial = 1, kApply = 2 };
 constexpr int kNsStages = 3;
 constexpr unsigned kNsStageBytes = 4 * kPanelHalf; // left hi, left lo, right hi, right lo
-constexpr int kNsEpilogueWarps = 16, kNsThreads = (kNsEpilogueWarps + 3) * 32;
+constexpr int kNsEpilogueWarps = 16, kNsThreads = (kNsEpilogueWarps + 4) * 32;
 // Stages summed in tensor memory before they are added in registers (for pairs one costs 15 %).
 template <int CTAS> constexpr int kNsChunk = CTAS == 1 ? 1 : 2;
 // The truncation of such a sum shortens it by about one (single) to three units of 2^-23 on average,
@@ -280,12 +280,14 @@ __device__ __forceinline__ const NsMat &tile_at(const NsTable &t, int what, unsi
   return q;
 }
 
-// The linear term of a tile comes through the same ring of stages, after the first four K blocks (or
-// after the last): by then the draining warps are done with the tile before and take it at once. The
+// The linear term of a tile comes through the same ring of stages, after the first four K blocks (eight
+// for pairs; or after the last): by then the draining warps are done with the tile before and take it at once. The
 // gram matrix has none, nor have the other parts of a split K.
+template <int CTAS>
 __device__ __forceinline__ unsigned ns_linear_after(const NsTile &at, int what) {
+  constexpr unsigned kAfter = 4 * CTAS;
   if (what == kGram || at.part != 0) return ~0u;
-  return at.k_blocks < 4 ? at.k_blocks : 4;
+  return at.k_blocks < kAfter ? at.k_blocks : kAfter;
 }
 
 // One operand of a tile: 128 rows (64 where narrow) by 64 of K per stage. `plain`: the block in block
@@ -343,6 +345,7 @@ struct NsShared {
   NsTable table; // a copy: the roles index it at every tile, which is slow in constant memory
   uint32_t tmem;
   volatile unsigned gave_up;
+  volatile unsigned allowed; // tiles whose operands are stored, as the looking-out thread has seen
   unsigned written;     // draining warps that have written their part of a tile, over all tiles
   unsigned linear_read[2]; // draining warps that have read their part of a linear term's stage, over all tiles
 };
@@ -378,8 +381,7 @@ struct NsRing {
   }
 };
 
-// Waits until matrix q's products up to this one (step s, product what) are stored. Relaxed polling, then
-// one fence: an acquiring load would fence at every turn.
+// Waits until matrix q's products up to this one (step s, product what) are stored.
 template <int CTAS>
 __device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, int s, int what, volatile unsigned *gave_up) {
   unsigned target = 0;
@@ -389,8 +391,8 @@ __device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, in
   long long start = 0;
   for (unsigned spins = 0;; ++spins) {
     unsigned now;
-    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(counter) : "memory");
-    if (now >= target) break;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(counter) : "memory");
+    if (now >= target) return true;
     if (spins == 0) start = clock64();
     if ((spins & 63) == 63) {
       if (*gave_up) return false;
@@ -400,8 +402,6 @@ __device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, in
       }
     }
   }
-  asm volatile("fence.acq_rel.gpu;" ::: "memory");
-  return true;
 }
 
 // The same for a counter in shared memory.
@@ -440,9 +440,9 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
     // K blocks before these are above the diagonal
     const unsigned flip_left = what == kGram ? 0 : 2 * CTAS * at.i;
     const unsigned flip_right = what == kGram ? 0 : what == kApply ? ~0u : 2 * CTAS * (narrow ? at.j / 2 : at.j);
-    if (!ns_wait_stored<CTAS>(t, q, s, what, &sh.gave_up)) return false;
+    if (!ns_wait_counter(&sh.allowed, ++ring.tiles, &sh.gave_up)) return false;
     asm volatile("fence.proxy.async.global;" ::: "memory"); // panels are written with plain stores
-    const unsigned k_linear = ns_linear_after(at, what);
+    const unsigned k_linear = ns_linear_after<CTAS>(at, what);
     for (unsigned k = 0; k <= at.k_blocks; ++k) {
       if (k == k_linear) {
         // the linear term, b A or a X: two block columns of this CTA's rows to a stage
@@ -474,6 +474,20 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
   return true;
 }
 
+// ---- the thread that looks out for the tiles' operands, ahead of the one that loads (to which a look and
+// its fence at every tile cost 3,000 to 4,000 cycles without a load in flight)
+template <int CTAS>
+__device__ bool ns_look_out(NsShared &sh, NsRing &ring, int s, int what) {
+  const NsTable &t = sh.table;
+  for (unsigned tile = ring.first; tile < t.tiles[what]; tile += gridDim.x / CTAS) {
+    NsTile at;
+    const NsMat &q = tile_at<CTAS>(t, what, tile, at);
+    if (!ns_wait_stored<CTAS>(t, q, s, what, &sh.gave_up)) return false;
+    sh.allowed = ++ring.tiles;
+  }
+  return true;
+}
+
 // ---- the warp that issues the products (in the second CTA of a pair: passes on that its half is there).
 // All lanes walk the loops together, so that descriptors stay in uniform registers; one lane issues.
 template <int CTAS>
@@ -487,7 +501,7 @@ __device__ bool ns_multiply(NsShared &sh, NsRing &ring, int what) {
     tile_at<CTAS>(t, what, tile, at);
     const unsigned flip_left = what == kGram ? 0 : 2 * CTAS * at.i;
     const unsigned flip_right = what == kGram ? 0 : what == kApply ? ~0u : 2 * CTAS * (narrow ? at.j / 2 : at.j);
-    const unsigned k_linear = ns_linear_after(at, what);
+    const unsigned k_linear = ns_linear_after<CTAS>(at, what);
     for (unsigned k = 0; k <= at.k_blocks; ++k, ring.next_stage()) {
       if (k == k_linear) {
         // not for the tensor cores; but the second CTA's messages count every turn of the ring
@@ -569,7 +583,7 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
 #pragma unroll
     for (int i = 0; i < 16 * kGroups; ++i) acc[i] = 0.0f;
     const unsigned rounds = (at.k_blocks + kNsChunk<CTAS> - 1) / kNsChunk<CTAS>;
-    const unsigned k_linear = ns_linear_after(at, what);
+    const unsigned k_linear = ns_linear_after<CTAS>(at, what);
 #pragma unroll 1
     for (unsigned c = 0; c <= rounds; ++c) {
       if (k_linear != ~0u && c == (k_linear + kNsChunk<CTAS> - 1) / kNsChunk<CTAS>) {
@@ -799,7 +813,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
       barrier_init(smem_address(&sh.acc_empty[b]), kNsEpilogueWarps * CTAS);
     }
     barrier_init(smem_address(&sh.drained), 1);
-    sh.gave_up = sh.written = sh.linear_read[0] = sh.linear_read[1] = 0;
+    sh.gave_up = sh.allowed = sh.written = sh.linear_read[0] = sh.linear_read[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
@@ -822,7 +836,11 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
     ring.first = (me + workers - before) % workers;
     if (warp < kNsEpilogueWarps) ok = ns_drain<CTAS>(sh, ring, s, what, s + 1 == steps, piece);
     else if (warp == kNsEpilogueWarps + 1) ok = ns_multiply<CTAS>(sh, ring, what);
-    else if (lane == 0) ok = warp == kNsEpilogueWarps ? ns_load<CTAS>(sh, ring, s, what) : ns_publish<CTAS>(sh, ring, what);
+    else if (lane == 0) {
+      if (warp == kNsEpilogueWarps) ok = ns_load<CTAS>(sh, ring, s, what);
+      else if (warp == kNsEpilogueWarps + 2) ok = ns_publish<CTAS>(sh, ring, what);
+      else ok = ns_look_out<CTAS>(sh, ring, s, what);
+    }
     before = (before + t.tiles[what]) % workers;
   }
   if (!ok && lane == 0) { // after a wait that ran out: what is in flight ends before its memory goes away
