@@ -27,7 +27,7 @@ constexpr int kMuonMax = 32;                       // matrices per launch (256 b
 static_assert(kMuonMax * sizeof(unsigned) <= 256, "");
 constexpr u64 kMuonScratch = (u64)2 << 30;         // scratch of one group of matrices
 constexpr int kMuonThreads = 256;
-constexpr int kMuonChunk = kMuonThreads * 16;      // elements per CTA of the momentum pass
+constexpr int kMuonChunk = kMuonThreads * 32;      // elements per CTA of the momentum pass
 
 struct MuonMat {
   const float *g;  // gradient, or the input of orthogonalise
@@ -71,16 +71,42 @@ __global__ void __launch_bounds__(kMuonThreads) muon_momentum_kernel(const __gri
   const MuonMat &q = t.mat[matrix_of(t, blockIdx.x)];
   const u64 total = (u64)q.rows * q.cols, begin = (u64)(blockIdx.x - q.first) * kMuonChunk;
   double sum = 0.0;
-  for (int i = 0; i < kMuonChunk / kMuonThreads; ++i) {
-    const u64 j = begin + (u64)i * kMuonThreads + threadIdx.x;
-    if (j >= total) break;
-    float u = q.g[j];
+  auto one = [&](float g, float &v) {
+    float u = g;
     if (q.v) {
-      const float v = __fmaf_rn(t.mu, q.v[j], u);
-      q.v[j] = v;
-      u = update_of(t, u, v);
+      v = __fmaf_rn(t.mu, v, g);
+      u = update_of(t, g, v);
     }
     sum += (double)u * (double)u;
+  };
+  if (total - begin >= (u64)kMuonChunk && (((uintptr_t)q.g | (uintptr_t)q.v) & 15) == 0) {
+    const float4 *g4 = reinterpret_cast<const float4 *>(q.g + begin) + threadIdx.x;
+    float4 *v4 = q.v ? reinterpret_cast<float4 *>(q.v + begin) + threadIdx.x : nullptr;
+#pragma unroll 1
+    for (int batch = 0; batch < kMuonChunk / kMuonThreads / 16; ++batch, g4 += 4 * kMuonThreads) {
+      float4 g[4], v[4] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[i] = g4[i * kMuonThreads];
+      if (v4)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = v4[i * kMuonThreads];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        one(g[i].x, v[i].x);
+        one(g[i].y, v[i].y);
+        one(g[i].z, v[i].z);
+        one(g[i].w, v[i].w);
+        if (v4) v4[i * kMuonThreads] = v[i];
+      }
+      if (v4) v4 += 4 * kMuonThreads;
+    }
+  } else {
+#pragma unroll 4
+    for (u64 j = begin + threadIdx.x; j < begin + kMuonChunk && j < total; j += kMuonThreads) {
+      float v = q.v ? q.v[j] : 0.0f;
+      one(q.g[j], v);
+      if (q.v) q.v[j] = v;
+    }
   }
   __shared__ double part[kMuonThreads / 32];
 #pragma unroll
@@ -100,6 +126,7 @@ __global__ void __launch_bounds__(kMuonThreads) muon_norm_kernel(const __grid_co
   const MuonMat &q = t.mat[blockIdx.x];
   __shared__ double part[kMuonThreads];
   double sum = 0.0;
+#pragma unroll 8
   for (unsigned i = threadIdx.x; i < q.chunks; i += kMuonThreads) sum += q.partial[1 + i];
   if (blockIdx.x == 0)
     for (unsigned i = threadIdx.x; i < t.ticket_count; i += kMuonThreads) t.tickets[i] = 0;
@@ -121,37 +148,64 @@ __global__ void __launch_bounds__(kMuonThreads) muon_load_kernel(const __grid_co
   pdl_wait();
   pdl_launch_dependents();
   const MuonMat &q = t.mat[matrix_of(t, blockIdx.x)];
-  __shared__ float tile[kPanelCols][kPanelRows + 1]; // the block, turned
-  // in 64 bits: the norm may be outside fp32's range where the quotient is not
+  __shared__ float tile[kPanelRows][kPanelCols + 1];
+  // the factor in 64 bits: the norm may be outside fp32's range where the quotient is not; the products
+  // too, unless it is an ordinary number
   const double inv = (double)kSplitScale / (sqrt(q.partial[0]) + (double)t.epsilon);
+  const float inv32 = (float)inv;
+  const bool ordinary = inv32 > 1e-30f && inv32 < 1e30f;
+  auto value = [&](float u, float v) {
+    if (q.v) u = update_of(t, u, v);
+    return ordinary ? u * inv32 : (float)((double)u * inv);
+  };
   const unsigned col_blocks = panel_col_blocks(q.n), at = blockIdx.x - q.first;
   const unsigned rb = at / col_blocks, cb = at % col_blocks;
   const bool turned = q.rows > q.cols;
-  auto value = [&](u64 j) {
-    float u = q.g[j];
-    if (q.v) u = update_of(t, u, q.v[j]);
-    return (float)((double)u * inv);
-  };
-  if (turned) { // stored row = panel column
-    for (unsigned e = threadIdx.x; e < kPanelRows * kPanelCols; e += kMuonThreads) {
-      const unsigned i = e % kPanelRows, k = e / kPanelRows; // panel row, panel column
-      const unsigned r = cb * kPanelCols + k, c = rb * kPanelRows + i;
-      tile[k][i] = r < q.rows && c < q.cols ? value((u64)r * q.cols + c) : 0.0f;
-    }
-    __syncthreads();
+  // the block in the matrix as it is stored
+  const unsigned r0 = turned ? cb * kPanelCols : rb * kPanelRows, c0 = turned ? rb * kPanelRows : cb * kPanelCols;
+  constexpr int kEach = kPanelRows * kPanelCols / 4 / kMuonThreads; // float4 per thread
+  const unsigned wide = turned ? kPanelRows / 4 : kPanelCols / 4;     // float4 along a stored row of the block
+  float x[kEach][4];
+  const bool vec = (((uintptr_t)q.g | (uintptr_t)q.v) & 15) == 0 && q.cols % 4 == 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const unsigned item = e * kMuonThreads + threadIdx.x, r = r0 + item / wide, c = c0 + item % wide * 4;
+    const u64 j = (u64)r * q.cols + c;
+    float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = g;
+    if (r < q.rows && c < q.cols) {
+      if (vec) {
+        g = *reinterpret_cast<const float4 *>(q.g + j);
+        if (q.v) v = *reinterpret_cast<const float4 *>(q.v + j);
+      } else {
+        float *gs = &g.x, *vs = &v.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c + i < q.cols) {
+            gs[i] = q.g[j + i];
+            if (q.v) vs[i] = q.v[j + i];
+          }
+      }
+      x[e][0] = value(g.x, v.x);
+      x[e][1] = c + 1 < q.cols ? value(g.y, v.y) : 0.0f;
+      x[e][2] = c + 2 < q.cols ? value(g.z, v.z) : 0.0f;
+      x[e][3] = c + 3 < q.cols ? value(g.w, v.w) : 0.0f;
+    } else x[e][0] = x[e][1] = x[e][2] = x[e][3] = 0.0f;
   }
+  // through shared memory to eight neighbours along a panel row per thread
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const unsigned item = e * kMuonThreads + threadIdx.x, r = item / wide, c = item % wide * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tile[turned ? c + i : r][turned ? r : c + i] = x[e][i];
+  }
+  __syncthreads();
   char *block = q.x[0] + panel_block(rb, cb, col_blocks);
+#pragma unroll
   for (unsigned e = threadIdx.x; e < kPanelRows * 8; e += kMuonThreads) {
     const unsigned row = e / 8, chunk = e % 8;
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (turned) v[i] = tile[chunk * 8 + i][row];
-      else {
-        const unsigned r = rb * kPanelRows + row, c = cb * kPanelCols + chunk * 8 + i;
-        v[i] = r < q.rows && c < q.cols ? value((u64)r * q.cols + c) : 0.0f;
-      }
-    }
+    for (int i = 0; i < 8; ++i) v[i] = tile[row][chunk * 8 + i];
     uint4 hi, lo;
     split8(v, hi, lo);
     *reinterpret_cast<uint4 *>(block + panel_chunk(row, chunk)) = hi;
