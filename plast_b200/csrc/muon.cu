@@ -1127,7 +1127,9 @@ static void run_group(MuonTable &t, char *base, int steps) {
 }
 
 // All matrices, in groups that share one piece of scratch.
-static void run_matrices(const std::vector<MuonMat> &mats, float mu, float epsilon, int nesterov, int steps) {
+static void run_matrices(std::vector<MuonMat> &mats, float mu, float epsilon, int nesterov, int steps) {
+  // longest products first: what ends a product is short then, and the next ones have begun
+  std::stable_sort(mats.begin(), mats.end(), [](const MuonMat &a, const MuonMat &b) { return a.n != b.n ? a.n > b.n : a.m > b.m; });
   u64 largest = 0;
   std::vector<size_t> ends;
   for (size_t i = 0; i < mats.size();) {
