@@ -12,6 +12,7 @@ There is no CPU fallback: if the library is missing or cannot be loaded, importi
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from pathlib import Path
 
@@ -131,16 +132,16 @@ def _load() -> C.CDLL:
             f"{LIB_PATH} is missing: build it with `python -m plast_b200.build` "
             "(there is no CPU fallback for the CUDA path)")
     lib = C.CDLL(str(LIB_PATH))
-    # `inputs` as an address: any array of Tensor pointers, or of their addresses (see _addresses)
+    # addresses: any array of Tensor pointers or of their addresses (see _addresses), a Tensor's byref or address
     for op in FORWARD_OPS:
         fn = getattr(lib, f"{op}_cuda_forward")
-        fn.argtypes = [C.c_void_p, C.POINTER(CTensor), KernelParams]
+        fn.argtypes = [C.c_void_p, C.c_void_p, KernelParams]
         fn.restype = None
     for op in BACKWARD_OPS:
         fn = getattr(lib, f"{op}_cuda_backward")
-        fn.argtypes = [C.c_void_p, C.POINTER(CTensor), KernelParams]
+        fn.argtypes = [C.c_void_p, C.c_void_p, KernelParams]
         fn.restype = None
-    lib.sum_axis0_noalloc_cuda_forward.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(CTensor), KernelParams]
+    lib.sum_axis0_noalloc_cuda_forward.argtypes = [C.c_void_p, C.c_void_p, KernelParams]
     lib.sum_axis0_noalloc_cuda_forward.restype = None
     lib.plast_b200_chain_forward.argtypes = [C.POINTER(C.POINTER(CTensor)), C.c_int, C.POINTER(CTensor),
                                              C.POINTER(ChainStep), C.c_int]
@@ -153,10 +154,10 @@ def _load() -> C.CDLL:
     lib.plast_b200_chain_forward_host.restype = None
     lib.plast_b200_add_leaky_relu_row_sum.argtypes = [C.POINTER(CTensor)] * 4 + [C.c_float]
     lib.plast_b200_add_leaky_relu_row_sum.restype = None
-    lib.plast_b200_token_logprob.argtypes = [C.POINTER(CTensor)] * 8 + [C.c_float]
-    lib.plast_b200_token_logprob_backward.argtypes = [C.POINTER(CTensor)] * 6 + [C.c_float]
-    lib.plast_b200_qk_norm_rotary.argtypes = [C.POINTER(CTensor)] * 8 + [QkNormParams]
-    lib.plast_b200_qk_norm_rotary_backward.argtypes = [C.POINTER(CTensor)] * 8 + [QkNormParams]
+    lib.plast_b200_token_logprob.argtypes = [C.c_void_p] * 8 + [C.c_float]
+    lib.plast_b200_token_logprob_backward.argtypes = [C.c_void_p] * 6 + [C.c_float]
+    lib.plast_b200_qk_norm_rotary.argtypes = [C.c_void_p] * 8 + [QkNormParams]
+    lib.plast_b200_qk_norm_rotary_backward.argtypes = [C.c_void_p] * 8 + [QkNormParams]
     lib.plast_b200_rotary_frequencies.argtypes = [C.POINTER(RotaryScaling), C.c_uint64, C.c_float, C.POINTER(C.c_float),
                                                   C.POINTER(C.c_float)]
     lib.plast_b200_rotary_frequencies.restype = C.c_int
@@ -252,6 +253,7 @@ class Tensor:
             raise ValueError("ndim > MAX_NDIM")
         self.device = device
         self.c = CTensor()
+        self.address = C.addressof(self.c)      # of the struct: what a call passes
         self.c.ndim = len(shape)
         for i, s in enumerate(shape):
             self.c.shape[i] = s
@@ -400,7 +402,7 @@ def _addresses(tensors):
     """Tensor** as an array of addresses: a fifth of the time of an array of pointer objects, which is most of what a
     call on a small tensor costs. The caller's list keeps the structs alive."""
     n = len(tensors)
-    return (_ADDRESSES[n] if n < 9 else C.c_void_p * n)(*[C.addressof(t.c) for t in tensors])
+    return (_ADDRESSES[n] if n < 9 else C.c_void_p * n)(*[t.address for t in tensors])
 
 
 def check_error():
@@ -421,7 +423,7 @@ def forward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fva
             check: bool = True):
     """``<op>_cuda_forward(inputs, output, params)``; raises :class:`PlastError` on failure."""
     fn = _ENTRY.get(("forward", op)) or _entry("forward", op)
-    fn(_addresses(inputs), C.byref(output.c), KernelParams(dim, keepdim, fval))
+    fn(_addresses(inputs), output.address, _params(dim, keepdim, fval))
     if check:
         check_error()
     return output
@@ -431,13 +433,18 @@ def backward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fv
              check: bool = True):
     """``<op>_cuda_backward(inputs, output, params)``: accumulates into inputs[i].grad."""
     fn = _ENTRY.get(("backward", op)) or _entry("backward", op)
-    fn(_addresses(inputs), C.byref(output.c), KernelParams(dim, keepdim, fval))
+    fn(_addresses(inputs), output.address, _params(dim, keepdim, fval))
     if check:
         check_error()
 
 
-def _ref(t):
-    return None if t is None else C.byref(t.c)
+def _at(t):
+    return None if t is None else t.address
+
+
+@functools.lru_cache(maxsize=256)
+def _params(dim, keepdim, fval):
+    return KernelParams(dim, keepdim, fval)
 
 
 def token_logprob(logits, tokens, logprob, entropy=None, log_norm=None, stats=None, top_logprob=None, top_index=None,
@@ -445,8 +452,8 @@ def token_logprob(logits, tokens, logprob, entropy=None, log_norm=None, stats=No
     """Log probability of one given token per row of logits [..., C], with the distribution's entropy and log
     normaliser, the statistics that the backward needs ([..., 2]) and the k = top_index.shape[-1] best
     alternatives; optional outputs may be None."""
-    lib.plast_b200_token_logprob(_ref(logits), _ref(tokens), _ref(logprob), _ref(entropy), _ref(log_norm), _ref(stats),
-                                 _ref(top_logprob), _ref(top_index), temperature)
+    lib.plast_b200_token_logprob(_at(logits), _at(tokens), _at(logprob), _at(entropy), _at(log_norm), _at(stats),
+                                 _at(top_logprob), _at(top_index), temperature)
     if check:
         check_error()
     return logprob
@@ -455,8 +462,8 @@ def token_logprob(logits, tokens, logprob, entropy=None, log_norm=None, stats=No
 def token_logprob_backward(logits, tokens, stats, logprob=None, entropy=None, log_norm=None, temperature: float = 1.0,
                            check: bool = True):
     """logits.grad += the gradient of the upstream gradients in logprob.grad, entropy.grad and log_norm.grad."""
-    lib.plast_b200_token_logprob_backward(_ref(logits), _ref(tokens), _ref(stats), _ref(logprob), _ref(entropy),
-                                          _ref(log_norm), temperature)
+    lib.plast_b200_token_logprob_backward(_at(logits), _at(tokens), _at(stats), _at(logprob), _at(entropy),
+                                          _at(log_norm), temperature)
     if check:
         check_error()
 
@@ -478,8 +485,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, 
                    layout: int = ROTARY_HALVES, amplitude: float = 1.0, check: bool = True):
     """Root-mean-square norm of every query and key head, its weight and the rotation, in one launch. k, k_weight
     and k_out may be None together, a weight alone too."""
-    lib.plast_b200_qk_norm_rotary(_ref(q), _ref(k), _ref(q_weight), _ref(k_weight), _ref(positions), _ref(inv_freq),
-                                  _ref(q_out), _ref(k_out), QkNormParams(epsilon, amplitude, layout))
+    lib.plast_b200_qk_norm_rotary(_at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions), _at(inv_freq),
+                                  _at(q_out), _at(k_out), QkNormParams(epsilon, amplitude, layout))
     if check:
         check_error()
     return q_out, k_out
@@ -488,8 +495,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, 
 def qk_norm_rotary_backward(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, epsilon: float = 1e-6,
                             layout: int = ROTARY_HALVES, amplitude: float = 1.0, check: bool = True):
     """Adds to q.grad, k.grad and the weights' gradients, reading q_out.grad and k_out.grad."""
-    lib.plast_b200_qk_norm_rotary_backward(_ref(q), _ref(k), _ref(q_weight), _ref(k_weight), _ref(positions),
-                                           _ref(inv_freq), _ref(q_out), _ref(k_out),
+    lib.plast_b200_qk_norm_rotary_backward(_at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions),
+                                           _at(inv_freq), _at(q_out), _at(k_out),
                                            QkNormParams(epsilon, amplitude, layout))
     if check:
         check_error()

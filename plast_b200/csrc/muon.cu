@@ -537,6 +537,7 @@ __device__ bool ns_look_out(NsShared &sh, NsRing &ring, int s, int what) {
     NsTile at;
     const NsMat &q = tile_at<CTAS>(t, what, tile, at);
     if (!ns_wait_stored<CTAS>(t, q, s, what, &sh.gave_up)) return false;
+    __threadfence_block();
     sh.allowed = ++ring.tiles;
   }
   return true;
@@ -1141,7 +1142,7 @@ static void run_matrices(std::vector<MuonMat> &mats, float mu, float epsilon, in
     ends.push_back(i = k);
   }
   char *scratch = nullptr;
-  PB_CUDA(scratch_alloc_async((void **)&scratch, largest));
+  if (!check_cuda(scratch_alloc_async((void **)&scratch, largest))) return;
   size_t i = 0;
   for (size_t end : ends) {
     MuonTable t = {};

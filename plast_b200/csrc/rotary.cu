@@ -754,7 +754,11 @@ void plast_b200_qk_norm_rotary_backward(Tensor *q, Tensor *k, Tensor *q_weight, 
   const unsigned max_blocks = (unsigned)sm_count() * 2; // all resident: each keeps one partial sum
   float *scratch = nullptr;
   if (wants_weight[0] || wants_weight[1]) {
-    PB_CUDA(scratch_alloc_async((void **)&scratch, (size_t)2 * max_blocks * p.head * sizeof(float)));
+    const cudaError_t e = scratch_alloc_async((void **)&scratch, (size_t)2 * max_blocks * p.head * sizeof(float));
+    if (e != cudaSuccess) {
+      cudaGetLastError(); // reported here, not by the next call
+      return set_error(PLAST_B200_ERR_CUDA, "%s: no scratch for the weight gradients: %s", name, cudaGetErrorString(e));
+    }
     for (int i = 0; i < sides; ++i)
       if (wants_weight[i]) p.side[i].partial = scratch + (size_t)i * max_blocks * p.head;
   }

@@ -15,6 +15,7 @@
 #include "row_map.cuh"
 #include "ew_kernel_device.cuh" // pdl_wait / pdl_launch_dependents
 
+#include <algorithm>
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -114,7 +115,8 @@ __device__ __forceinline__ unsigned index_of(u64key k) { return 0xffffffffu - (u
 struct LpShared {
   u64key cand[kLpCandidates]; // a list per warp while the row streams
   u64key last[kLpCandidates]; // what is left of them at the end
-  u64key best[PLAST_TOKEN_TOP_MAX];
+  u64key best[PLAST_TOKEN_TOP_MAX];   // of the CTA
+  u64key chosen[PLAST_TOKEN_TOP_MAX]; // of the cluster
   u64key join[kLpMaxCluster * PLAST_TOKEN_TOP_MAX];
   float stat[kLpMaxCluster][3];
   float warp_stat[kLpMaxThreads / 32][3];
@@ -182,15 +184,37 @@ __device__ __forceinline__ float next_above(float v) {
   return __int_as_float(v == 0.0f ? 1 : b > 0 ? b + 1 : b - 1);
 }
 
-// Cuts a warp's list of candidates to its k best; the last of them is the new threshold.
-__device__ __noinline__ u64key cut_list(u64key *list, unsigned count, u64key *spare, int k) {
+// Cuts a warp's list of candidates to its k best, in order; returns the last of them, the new threshold.
+// k times the warp's largest: a lane looks after every 32nd place and looks again when it has lost one.
+__device__ __forceinline__ u64key cut_list(u64key *list, unsigned count, u64key *spare, int k) {
   const unsigned lane = threadIdx.x & 31;
   __syncwarp();
-  select_best(spare, list, count, k, lane, 32);
-  __syncwarp();
+  u64key mine = 0;
+  unsigned at = 0;
+  auto look = [&] {
+    mine = 0;
+    for (unsigned i = lane; i < count; i += 32)
+      if (list[i] > mine) {
+        mine = list[i];
+        at = i;
+      }
+  };
+  look();
+  u64key best = 0;
+  for (int r = 0; r < k; ++r) {
+    const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(mine >> 32));
+    const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(mine >> 32) == hi ? (unsigned)mine : 0u);
+    best = ((u64key)hi << 32) | lo;
+    if (mine == best) { // one lane: keys are distinct
+      spare[r] = best;
+      list[at] = 0;
+      look();
+    }
+    __syncwarp();
+  }
   if ((int)lane < k) list[lane] = spare[lane];
   __syncwarp();
-  return list[k - 1];
+  return best;
 }
 
 // ---- forward -----------------------------------------------------------------------------------------
@@ -204,7 +228,7 @@ __device__ __noinline__ u64key cut_list(u64key *list, unsigned count, u64key *sp
 // only better). About 3 k logits of a random row pass. A list that is full is cut to its k best, so any
 // order and any number of ties ends with the exact answer.
 template <bool UNIT, bool TOP>
-__global__ void __launch_bounds__(kLpMaxThreads) token_logprob_kernel(const __grid_constant__ LpParams p) {
+__global__ void __launch_bounds__(kLpMaxThreads, 2) token_logprob_kernel(const __grid_constant__ LpParams p) {
   __shared__ LpShared sh;
   namespace cg = cooperative_groups;
   pdl_wait();
@@ -216,14 +240,10 @@ __global__ void __launch_bounds__(kLpMaxThreads) token_logprob_kernel(const __gr
   const float *x = p.x + off[0];
   const float c = p.scale_log2;
   const int k = p.top;
-  // thread 0 of the row's first CTA reports; its two dependent loads start now
-  int token = -1;
+  // thread 0 of the row's first CTA reports; of its two dependent loads the second starts with the stream
+  const bool reports = rank == 0 && threadIdx.x == 0;
+  int token = reports ? p.token[off[1]] : -1;
   float x_token = 0.0f;
-  if (rank == 0 && threadIdx.x == 0) {
-    token = p.token[off[1]];
-    if (token >= 0 && (unsigned)token < p.cols) x_token = x[(u64)token * p.col_stride];
-    else token = -1;
-  }
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   // the warp's candidates: `room` places of the shared list; keys above `threshold` are wanted
   const unsigned room = kLpCandidates / warps;
@@ -235,6 +255,8 @@ __global__ void __launch_bounds__(kLpMaxThreads) token_logprob_kernel(const __gr
   if (TOP) {
     if (lane == 0) sh.warp_bound[warp] = -INFINITY;
     if (threadIdx.x == 0) sh.count = 0;
+    // places that a selection does not fill stay 0 (a key is never 0)
+    if (threadIdx.x < PLAST_TOKEN_TOP_MAX) sh.best[threadIdx.x] = sh.chosen[threadIdx.x] = 0;
     __syncthreads();
   }
   // vectors of four logits; the first one starts at the 16-byte boundary at or before the row
@@ -267,6 +289,10 @@ __global__ void __launch_bounds__(kLpMaxThreads) token_logprob_kernel(const __gr
         for (int i = 0; i < 4; ++i)
           v[4 * u + i] = (at < last && j + i >= 0 && j + i < (long long)p.cols) ? x[(u64)(j + i) * p.col_stride] : -INFINITY;
       }
+    }
+    if (reports && base == first) {
+      if (token >= 0 && (unsigned)token < p.cols) x_token = x[(u64)token * p.col_stride];
+      else token = -1;
     }
     float top = v[0];
 #pragma unroll
@@ -325,10 +351,7 @@ __global__ void __launch_bounds__(kLpMaxThreads) token_logprob_kernel(const __gr
     sh.warp_stat[warp][2] = st.u;
   }
   __syncthreads();
-  if (TOP) {
-    // what the final bound leaves of the lists, then the k best of that; places that the selection does
-    // not fill stay 0 (a key is never 0)
-    for (int i = threadIdx.x; i < k; i += blockDim.x) sh.best[i] = 0;
+  if (TOP) { // what the final bound leaves of the lists
     const float low = common_bound(sh, k, nth);
     const u64key floor_key = (key_of(low, 0) >> 32) << 32; // larger keys have at least this value
     for (unsigned i = lane; i < count; i += 32) {
@@ -336,46 +359,15 @@ __global__ void __launch_bounds__(kLpMaxThreads) token_logprob_kernel(const __gr
       if (key > floor_key) sh.last[atomicAdd(&sh.count, 1u)] = key;
     }
     __syncthreads();
-    select_best(sh.best, sh.last, sh.count, k, threadIdx.x, blockDim.x);
-    __syncthreads();
   }
-  if (warp == 0) {
-    st.init();
-    if (lane < warps) { st.m = sh.warp_stat[lane][0]; st.s = sh.warp_stat[lane][1]; st.u = sh.warp_stat[lane][2]; }
-    st.merge_warp(c);
-  }
-  __syncwarp();
-  if (p.cluster > 1) {
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // every CTA of the cluster runs
-    LpShared *lead_sh = cg::this_cluster().map_shared_rank(&sh, 0);
-    if (threadIdx.x == 0) {
-      lead_sh->stat[rank][0] = st.m;
-      lead_sh->stat[rank][1] = st.s;
-      lead_sh->stat[rank][2] = st.u;
-    }
-    if (TOP)
-      for (int i = threadIdx.x; i < k; i += blockDim.x) lead_sh->join[rank * k + i] = sh.best[i];
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank != 0) return;
-    if (warp == 0) {
-      st.init();
-      if (lane < p.cluster) { st.m = sh.stat[lane][0]; st.s = sh.stat[lane][1]; st.u = sh.stat[lane][2]; }
-      st.merge_warp(c);
-    }
-    if (TOP) {
-      for (int i = threadIdx.x; i < k; i += blockDim.x) sh.best[i] = 0;
-      __syncthreads();
-      select_best(sh.best, sh.join, p.cluster * k, k, threadIdx.x, blockDim.x);
-      __syncthreads();
-    }
-  }
-  if (threadIdx.x == 0) {
-    // the last few operations of a row in 64 bits, each result rounded once
+
+  // ---- the row's results: the upper half of the CTA selects while thread 0 does the scalars, the last few
+  // operations of a row in 64 bits, each result rounded once
+  auto report = [&] {
     const bool empty = st.s == 0.0f; // every logit is -inf
     const double log_s = log((double)st.s);
-    const double L = empty ? -INFINITY : (double)st.m / p.temperature + log_s;
     const double shift = (double)st.m; // log p = (x - m) / T - log S keeps its digits where L has none
+    const double L = empty ? -INFINITY : shift / p.temperature + log_s;
     double h = empty ? 0.0 : log_s - kLn2 * ((double)st.u / (double)st.s);
     if (h < 0.0) h = 0.0; // rounding of U; a NaN passes
     double lp = 0.0;
@@ -387,15 +379,47 @@ __global__ void __launch_bounds__(kLpMaxThreads) token_logprob_kernel(const __gr
     sh.log_s = log_s;
     sh.shift = shift;
     sh.empty = empty;
+  };
+  const unsigned upper = blockDim.x / 2;
+  if (TOP && threadIdx.x >= upper) select_best(sh.best, sh.last, sh.count, k, threadIdx.x - upper, upper);
+  if (warp == 0) {
+    st.init();
+    if (lane < warps) { st.m = sh.warp_stat[lane][0]; st.s = sh.warp_stat[lane][1]; st.u = sh.warp_stat[lane][2]; }
+    st.merge_warp(c);
+    if (p.cluster == 1 && threadIdx.x == 0) report();
   }
-  if (TOP) {
-    __syncthreads();
-    if ((int)threadIdx.x < k) {
-      const u64key key = sh.best[threadIdx.x];
-      const u64 at = (u64)row * k + threadIdx.x;
-      p.top_index[at] = key ? (int)index_of(key) : -1;
-      p.top_logprob[at] = !key ? NAN : sh.empty ? -INFINITY : (float)(((double)value_of(key) - sh.shift) / p.temperature - sh.log_s);
+  if (TOP) __syncthreads();
+  const u64key *chosen = sh.best;
+  __syncwarp();
+  if (p.cluster > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // every CTA of the cluster runs
+    LpShared *lead_sh = cg::this_cluster().map_shared_rank(&sh, 0);
+    if (threadIdx.x == 0) {
+      lead_sh->stat[rank][0] = st.m;
+      lead_sh->stat[rank][1] = st.s;
+      lead_sh->stat[rank][2] = st.u;
     }
+    if (TOP)
+      for (int i = threadIdx.x; i < k; i += blockDim.x) lead_sh->join[rank * k + i] = sh.best[i];
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank != 0) return;
+    if (TOP && threadIdx.x >= upper) select_best(sh.chosen, sh.join, p.cluster * k, k, threadIdx.x - upper, upper);
+    if (warp == 0) {
+      st.init();
+      if (lane < p.cluster) { st.m = sh.stat[lane][0]; st.s = sh.stat[lane][1]; st.u = sh.stat[lane][2]; }
+      st.merge_warp(c);
+      if (threadIdx.x == 0) report();
+    }
+    if (TOP) __syncthreads();
+    chosen = sh.chosen;
+  }
+  if (TOP && (int)threadIdx.x < k) {
+    const u64key key = chosen[threadIdx.x];
+    const u64 at = (u64)row * k + threadIdx.x;
+    p.top_index[at] = key ? (int)index_of(key) : -1;
+    p.top_logprob[at] = !key ? NAN : sh.empty ? -INFINITY : (float)(((double)value_of(key) - sh.shift) / p.temperature - sh.log_s);
   }
 }
 
@@ -409,11 +433,12 @@ struct LpGradParams {
   const float *g_logprob, *g_entropy, *g_log_norm; // any may be NULL
   RowMap map;                                      // 0: logits, 1: tokens, 2: gradient
   u64 col_stride, grad_stride;
-  unsigned cols;
+  unsigned cols, piece; // piece: vectors of four (or logits) per CTA
   float scale_log2, inv_t;
 };
 
-// A streaming pass over the row: 4 B read and 8 B for the += per logit.
+// A streaming pass: 4 B read and 8 B for the += per logit. A CTA takes a piece of one row (grid.y), so that a
+// thousand long rows end together: whole rows of 50001 run in 3.4 turns of the GPU.
 template <bool VEC>
 __global__ void __launch_bounds__(kLpMaxThreads) token_logprob_backward_kernel(const __grid_constant__ LpGradParams p) {
   pdl_wait();
@@ -444,14 +469,16 @@ __global__ void __launch_bounds__(kLpMaxThreads) token_logprob_backward_kernel(c
   if (VEC) {
     const unsigned lead = (unsigned)(((uintptr_t)x >> 2) & 3);
     const unsigned vectors = (unsigned)(((u64)p.cols + lead + 3) >> 2);
-    for (unsigned at0 = threadIdx.x; at0 < vectors; at0 += blockDim.x * 2) {
+    const unsigned begin = blockIdx.y * p.piece, end = vectors - begin < p.piece ? vectors : begin + p.piece;
+    if (begin >= vectors) return; // the row's lead made one piece fewer
+    for (unsigned at0 = begin + threadIdx.x; at0 < end; at0 += blockDim.x * 2) {
       float4 q[2], d[2];
       bool full[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const unsigned at = at0 + u * blockDim.x;
         const long long j = (long long)at * 4 - lead;
-        full[u] = at < vectors && j >= 0 && j + 4 <= (long long)p.cols;
+        full[u] = at < end && j >= 0 && j + 4 <= (long long)p.cols;
         if (full[u]) {
           q[u] = __ldcs(reinterpret_cast<const float4 *>(x + j));
           d[u] = __ldcs(reinterpret_cast<const float4 *>(dx + j));
@@ -467,14 +494,15 @@ __global__ void __launch_bounds__(kLpMaxThreads) token_logprob_backward_kernel(c
           d[u].z += grad(q[u].z, (unsigned)j + 2);
           d[u].w += grad(q[u].w, (unsigned)j + 3);
           __stcs(reinterpret_cast<float4 *>(dx + j), d[u]);
-        } else if (at < vectors) {
+        } else if (at < end) {
           for (int i = 0; i < 4; ++i)
             if (j + i >= 0 && j + i < (long long)p.cols) dx[j + i] += grad(x[j + i], (unsigned)(j + i));
         }
       }
     }
   } else {
-    for (unsigned j = threadIdx.x; j < p.cols; j += blockDim.x) {
+    const unsigned begin = blockIdx.y * p.piece, end = p.cols - begin < p.piece ? p.cols : begin + p.piece;
+    for (unsigned j = begin + threadIdx.x; j < end; j += blockDim.x) {
       float *d = dx + (u64)j * p.grad_stride;
       *d += grad(x[(u64)j * p.col_stride], j);
     }
@@ -672,7 +700,10 @@ void plast_b200_token_logprob_backward(Tensor *logits, const Tensor *tokens, con
              (((uintptr_t)p.x ^ (uintptr_t)p.dx) & 15) == 0;
   for (int d = 0; d < p.map.nd && vec; ++d)
     if (p.map.size[d] > 1) vec = ((p.map.stride[0][d] ^ p.map.stride[2][d]) & 3) == 0;
-  const dim3 grid((unsigned)s.rows), block(lp_threads(s.cols, kLpMaxThreads));
+  // pieces of at least 16384 logits, at most 65535 of them; a row may start up to three before its first vector
+  const unsigned items = vec ? (unsigned)((s.cols + 3 + 3) / 4) : (unsigned)s.cols;
+  p.piece = std::max(vec ? 4096u : 16384u, items / 65535 + 1);
+  const dim3 grid((unsigned)s.rows, (items + p.piece - 1) / p.piece), block(lp_threads(std::min<u64>(s.cols, 16384), kLpMaxThreads));
   PB_CUDA(vec ? launch_k(token_logprob_backward_kernel<true>, grid, block, 0, stream(), p)
               : launch_k(token_logprob_backward_kernel<false>, grid, block, 0, stream(), p));
   count_launch();

@@ -73,7 +73,7 @@ def param_array(params):
 
 def _address_array(params):
     """param_array() as plain addresses, for the length of one call."""
-    return (C.c_void_p * max(len(params), 1))(*[None if p is None else C.addressof(p.c) for p in params])
+    return (C.c_void_p * max(len(params), 1))(*[None if p is None else p.address for p in params])
 
 
 def step(optimizer, params) -> None:

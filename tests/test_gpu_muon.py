@@ -123,12 +123,21 @@ def test_zeros_nan_and_scales_stay_in_their_matrices():
     assert np.abs(got[2]).max() < 1e-12
 
 
-def test_same_bits_alone_and_among_others():
+def test_the_same_call_gives_the_same_bits():
     rs = np.random.RandomState(6)
-    xs = [rs.randn(r, c).astype(np.float32) for r, c in [(200, 300), (130, 128), (500, 90)]]
-    together = orth(xs)
-    for x, t in zip(xs, together):
-        assert np.array_equal(orth([x])[0], t)
+    xs = [rs.randn(r, c).astype(np.float32) for r, c in [(200, 300), (130, 128), (500, 90), (64, 2500)]]
+    first = orth(xs)
+    for _ in range(3):
+        for a, b in zip(first, orth(xs)):
+            assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("shape", [(64, 4096), (2000, 100), (300, 3000), (512, 512), (130, 1920)])
+def test_long_products_whose_k_is_split(shape):
+    rs = np.random.RandomState(shape[1])
+    x = rs.randn(*shape).astype(np.float32)
+    want = R.orthogonalise(x)
+    assert rel(orth([x])[0], want) <= tolerance(min(shape))
 
 
 SETS = {"mixed": [(64, 64), (100, 300), (300, 100), (33, 65)], "tall": [(257, 64)], "image": [(16, 3, 5, 5), (8, 8)]}
