@@ -21,9 +21,6 @@
 
 namespace pb {
 
-#ifndef LP_THREADS
-#define LP_THREADS 256
-#endif
 constexpr int kLpMaxThreads = 512;
 constexpr int kLpUnroll = 4;      // float4 per thread and trip
 constexpr int kLpCandidates = 1024;
@@ -162,6 +159,18 @@ __device__ __forceinline__ float warp_nth(float v, int j) {
   return unordered(best);
 }
 
+// The k-th largest of the lanes' values: a bitonic sort, largest first.
+__device__ __forceinline__ float warp_kth(float v, int k) {
+  const unsigned lane = threadIdx.x & 31;
+#pragma unroll
+  for (unsigned size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (unsigned o = size / 2; o; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, v, o);
+      v = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(v, other) : fminf(v, other);
+    }
+  return __shfl_sync(0xffffffffu, v, k - 1);
+}
 // A value that at least k distinct logits reach, from the warps' `nth`-th largest lane maxima: where one
 // per warp does (nth == 1), the k-th largest of them, else the smallest.
 __device__ __forceinline__ float common_bound(const LpShared &sh, int k, int nth) {
@@ -217,7 +226,60 @@ __device__ __forceinline__ u64key cut_list(u64key *list, unsigned count, u64key 
   return best;
 }
 
-// ---- forward -----------------------------------------------------------------------------------------
+// What is reported of a row besides its alternatives: the last few operations in 64 bits, each result
+// rounded once. `log_s` and `shift`: log p of a logit x is (x - shift) / T - log_s, which keeps its
+// digits where the log normaliser has none.
+__device__ __forceinline__ void report_row(const LpParams &p, unsigned row, const LpStat &st, int token, float x_token, double &log_s,
+                                           double &shift, int &empty) {
+  empty = st.s == 0.0f; // every logit is -inf
+  log_s = log((double)st.s);
+  shift = (double)st.m;
+  const double L = empty ? -INFINITY : shift / p.temperature + log_s;
+  double h = empty ? 0.0 : log_s - kLn2 * ((double)st.u / (double)st.s);
+  if (h < 0.0) h = 0.0; // rounding of U; a NaN passes
+  double lp = 0.0;
+  if (token >= 0) lp = empty ? -INFINITY : ((double)x_token - shift) / p.temperature - log_s;
+  p.logprob[row] = (float)lp;
+  if (p.entropy) p.entropy[row] = (float)h;
+  if (p.log_norm) p.log_norm[row] = (float)L;
+  if (p.stats) p.stats[row] = make_float2(st.m, st.s);
+}
+__device__ __forceinline__ void report_alternative(const LpParams &p, unsigned row, int i, u64key key, double log_s, double shift, int empty) {
+  const u64 at = (u64)row * p.top + i;
+  p.top_index[at] = key ? (int)index_of(key) : -1;
+  p.top_logprob[at] = !key ? NAN : empty ? -INFINITY : (float)(((double)value_of(key) - shift) / p.temperature - log_s);
+}
+
+// A row (or slice) as vectors of four logits; the first one starts at the 16-byte boundary at or before it.
+template <bool UNIT> struct LpRow {
+  const float *x;
+  u64 stride;
+  unsigned cols, lead, vectors;
+  __device__ __forceinline__ LpRow(const float *x, const LpParams &p) : x(x), stride(p.col_stride), cols(p.cols) {
+    lead = UNIT ? (unsigned)(((uintptr_t)x >> 2) & 3) : 0u;
+    vectors = (unsigned)(((u64)cols + lead + 3) >> 2);
+  }
+  __device__ __forceinline__ long long index(unsigned at) const { return (long long)at * 4 - lead; } // of its first lane
+  // four logits of vector `at`, -inf where there are none
+  __device__ __forceinline__ void fetch(unsigned at, unsigned last, float *v) const {
+    const long long j = index(at);
+    if (at < last && j >= 0 && j + 4 <= (long long)cols) {
+      if (UNIT) {
+        const float4 q = __ldcs(reinterpret_cast<const float4 *>(x + j));
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = x[(u64)(j + i) * stride];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = (at < last && j + i >= 0 && j + i < (long long)cols) ? x[(u64)(j + i) * stride] : -INFINITY;
+    }
+  }
+};
+
+// ---- forward, few rows --------------------------------------------------------------------------------
 // One cluster of CTAs per row (1 where the rows fill the GPU; up to 8 where there are few rows, whose
 // slices are joined through distributed shared memory). A trip moves 16 logits per thread.
 //
@@ -259,9 +321,8 @@ __global__ void __launch_bounds__(kLpMaxThreads, 2) token_logprob_kernel(const _
     if (threadIdx.x < PLAST_TOKEN_TOP_MAX) sh.best[threadIdx.x] = sh.chosen[threadIdx.x] = 0;
     __syncthreads();
   }
-  // vectors of four logits; the first one starts at the 16-byte boundary at or before the row
-  const unsigned lead = UNIT ? (unsigned)(((uintptr_t)x >> 2) & 3) : 0u;
-  const unsigned vectors = (unsigned)(((u64)p.cols + lead + 3) >> 2);
+  const LpRow<UNIT> r(x, p);
+  const unsigned lead = r.lead, vectors = r.vectors;
   const unsigned slice = (vectors + p.cluster - 1) / p.cluster;
   const unsigned first = rank * slice < vectors ? rank * slice : vectors;
   const unsigned last = vectors - first < slice ? vectors : first + slice;
@@ -273,23 +334,7 @@ __global__ void __launch_bounds__(kLpMaxThreads, 2) token_logprob_kernel(const _
   for (unsigned base = first; base < last; base += trip) {
     float v[kLpUnroll * 4];
 #pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u) {
-      const unsigned at = base + u * blockDim.x + threadIdx.x;
-      const long long j = (long long)at * 4 - lead; // logit index of the vector's first lane
-      if (at < last && j >= 0 && j + 4 <= (long long)p.cols) {
-        if (UNIT) {
-          const float4 q = __ldcs(reinterpret_cast<const float4 *>(x + j));
-          v[4 * u] = q.x; v[4 * u + 1] = q.y; v[4 * u + 2] = q.z; v[4 * u + 3] = q.w;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * u + i] = x[(u64)(j + i) * p.col_stride];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[4 * u + i] = (at < last && j + i >= 0 && j + i < (long long)p.cols) ? x[(u64)(j + i) * p.col_stride] : -INFINITY;
-      }
-    }
+    for (int u = 0; u < kLpUnroll; ++u) r.fetch(base + u * blockDim.x + threadIdx.x, last, v + 4 * u);
     if (reports && base == first) {
       if (token >= 0 && (unsigned)token < p.cols) x_token = x[(u64)token * p.col_stride];
       else token = -1;
@@ -361,32 +406,14 @@ __global__ void __launch_bounds__(kLpMaxThreads, 2) token_logprob_kernel(const _
     __syncthreads();
   }
 
-  // ---- the row's results: the upper half of the CTA selects while thread 0 does the scalars, the last few
-  // operations of a row in 64 bits, each result rounded once
-  auto report = [&] {
-    const bool empty = st.s == 0.0f; // every logit is -inf
-    const double log_s = log((double)st.s);
-    const double shift = (double)st.m; // log p = (x - m) / T - log S keeps its digits where L has none
-    const double L = empty ? -INFINITY : shift / p.temperature + log_s;
-    double h = empty ? 0.0 : log_s - kLn2 * ((double)st.u / (double)st.s);
-    if (h < 0.0) h = 0.0; // rounding of U; a NaN passes
-    double lp = 0.0;
-    if (token >= 0) lp = empty ? -INFINITY : ((double)x_token - shift) / p.temperature - log_s;
-    p.logprob[row] = (float)lp;
-    if (p.entropy) p.entropy[row] = (float)h;
-    if (p.log_norm) p.log_norm[row] = (float)L;
-    if (p.stats) p.stats[row] = make_float2(st.m, st.s);
-    sh.log_s = log_s;
-    sh.shift = shift;
-    sh.empty = empty;
-  };
+  // ---- the row's results: the upper half of the CTA selects while thread 0 does the scalars
   const unsigned upper = blockDim.x / 2;
   if (TOP && threadIdx.x >= upper) select_best(sh.best, sh.last, sh.count, k, threadIdx.x - upper, upper);
   if (warp == 0) {
     st.init();
     if (lane < warps) { st.m = sh.warp_stat[lane][0]; st.s = sh.warp_stat[lane][1]; st.u = sh.warp_stat[lane][2]; }
     st.merge_warp(c);
-    if (p.cluster == 1 && threadIdx.x == 0) report();
+    if (p.cluster == 1 && threadIdx.x == 0) report_row(p, row, st, token, x_token, sh.log_s, sh.shift, sh.empty);
   }
   if (TOP) __syncthreads();
   const u64key *chosen = sh.best;
@@ -410,16 +437,245 @@ __global__ void __launch_bounds__(kLpMaxThreads, 2) token_logprob_kernel(const _
       st.init();
       if (lane < p.cluster) { st.m = sh.stat[lane][0]; st.s = sh.stat[lane][1]; st.u = sh.stat[lane][2]; }
       st.merge_warp(c);
-      if (threadIdx.x == 0) report();
+      if (threadIdx.x == 0) report_row(p, row, st, token, x_token, sh.log_s, sh.shift, sh.empty);
     }
     if (TOP) __syncthreads();
     chosen = sh.chosen;
   }
-  if (TOP && (int)threadIdx.x < k) {
-    const u64key key = chosen[threadIdx.x];
-    const u64 at = (u64)row * k + threadIdx.x;
-    p.top_index[at] = key ? (int)index_of(key) : -1;
-    p.top_logprob[at] = !key ? NAN : sh.empty ? -INFINITY : (float)(((double)value_of(key) - sh.shift) / p.temperature - sh.log_s);
+  if (TOP && (int)threadIdx.x < k) report_alternative(p, row, threadIdx.x, chosen[threadIdx.x], sh.log_s, sh.shift, sh.empty);
+}
+
+// ---- forward, many rows -------------------------------------------------------------------------------
+// A persistent CTA whose eight warps stream one row after the other while a ninth finishes the row before.
+// The end of a row is a chain of short steps (joining statistics, alternatives, logarithms) of 4 us, with
+// alternatives 6 to 9; in the streaming warps it leaves HBM idle for as long. Measured: 8192 rows of 65536 in
+// 314 us without alternatives (6.8 TB/s) and 348 with sixteen. With short rows the finishing warp is the
+// bound, hence the rule at the launch.
+//
+// The stream notes the largest logit of every thread and piece (one or more trips). A lane of the finishing
+// warp looks after eight threads; the k-th largest of the lanes' largest notes (above 16: of the largest
+// notes of the lanes' halves) is a bound, since k distinct logits reach it. The pieces whose note reaches it
+// are fetched again and the k best of what reaches it are kept: some 1.5 k logits of a random row. A list
+// that gets long is cut to its k best, whose last is a threshold from then on, so any order and any number
+// of ties ends with the exact answer.
+constexpr int kLpRowCtas = 4, kLpStream = 256, kLpRowThreads = kLpStream + 32, kLpPieces = 16, kLpHits = 256;
+struct LpRowShared {
+  float note[2][kLpPieces * kLpStream];
+  float stat[2][kLpStream / 32][3];
+  unsigned trips[2];
+  u64key list[kLpCandidates], spare[PLAST_TOKEN_TOP_MAX];
+  unsigned short hits[kLpHits];
+  unsigned char reach[kLpStream];
+};
+// named barriers: a row's notes are there / may be overwritten (two buffers)
+__device__ __forceinline__ void rows_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kLpRowThreads) : "memory"); }
+__device__ __forceinline__ void rows_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kLpRowThreads) : "memory"); }
+
+template <bool UNIT, bool TOP>
+__global__ void __launch_bounds__(kLpRowThreads, kLpRowCtas) token_logprob_rows_kernel(const __grid_constant__ LpParams p, unsigned rows) {
+  __shared__ LpRowShared sh;
+  pdl_wait();
+  pdl_launch_dependents();
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float c = p.scale_log2;
+  constexpr unsigned kTrip = kLpStream * kLpUnroll;
+  // the same for every row but for its lead, which adds at most one vector
+  const unsigned most_trips = (unsigned)((((u64)p.cols + 6) / 4 + kTrip - 1) / kTrip);
+  unsigned piece_log = 0;
+  while (((most_trips + (1u << piece_log) - 1) >> piece_log) > kLpPieces) ++piece_log;
+  unsigned turn = 0;
+
+  if (warp < kLpStream / 32) { // ---- stream
+    for (unsigned row = blockIdx.x; row < rows; row += gridDim.x, ++turn) {
+      const unsigned buf = turn & 1;
+      u64 off[3];
+      row_offsets(p.map, row, off);
+      const LpRow<UNIT> r(p.x + off[0], p);
+      LpStat st;
+      st.init();
+      if (turn >= 2) rows_sync(3 + buf);
+      float note = -INFINITY;
+      unsigned trips = 0;
+      for (unsigned base = 0; base < r.vectors; base += kTrip) {
+        float v[kLpUnroll * 4];
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u) r.fetch(base + u * kLpStream + threadIdx.x, r.vectors, v + 4 * u);
+        float top = v[0];
+#pragma unroll
+        for (int i = 1; i < kLpUnroll * 4; ++i) top = fmaxf(top, v[i]);
+        if (top > st.m) st.raise(top, c);
+#pragma unroll
+        for (int i = 0; i < kLpUnroll * 4; ++i) st.add(v[i], c);
+        if (TOP) {
+          note = fmaxf(note, top); // drops a NaN
+          ++trips;
+          if ((trips & ((1u << piece_log) - 1)) == 0 || base + kTrip >= r.vectors) {
+            sh.note[buf][((trips - 1) >> piece_log) * kLpStream + threadIdx.x] = note;
+            note = -INFINITY;
+          }
+        }
+      }
+      st.merge_warp(c);
+      if (lane == 0) {
+        sh.stat[buf][warp][0] = st.m;
+        sh.stat[buf][warp][1] = st.s;
+        sh.stat[buf][warp][2] = st.u;
+      }
+      if (TOP && threadIdx.x == 0) sh.trips[buf] = trips;
+      rows_arrive(1 + buf);
+    }
+    return;
+  }
+
+  // ---- finish
+  const int k = p.top;
+  for (unsigned row = blockIdx.x; row < rows; row += gridDim.x, ++turn) {
+    const unsigned buf = turn & 1;
+    u64 off[3];
+    row_offsets(p.map, row, off);
+    const LpRow<UNIT> r(p.x + off[0], p);
+    int token = p.token[off[1]];
+    float x_token = 0.0f;
+    if (token >= 0 && (unsigned)token < p.cols) x_token = r.x[(u64)token * p.col_stride];
+    else token = -1;
+    rows_sync(1 + buf);
+    LpStat st;
+    st.init();
+    if (lane < kLpStream / 32) { st.m = sh.stat[buf][lane][0]; st.s = sh.stat[buf][lane][1]; st.u = sh.stat[buf][lane][2]; }
+    st.merge_warp(c);
+    unsigned count = 0;
+    if (TOP) {
+      const unsigned trips = sh.trips[buf], here = (trips + (1u << piece_log) - 1) >> piece_log;
+      const float *note = sh.note[buf];
+      // A lane looks after eight threads; the k-th largest of the lanes' largest logits is the bound.
+      // (of more than 16: of the lanes' two halves)
+      float top[kLpStream / 32];
+#pragma unroll
+      for (int i = 0; i < kLpStream / 32; ++i) {
+        top[i] = -INFINITY;
+#pragma unroll 4
+        for (unsigned piece = 0; piece < here; ++piece) top[i] = fmaxf(top[i], note[piece * kLpStream + i * 32 + lane]);
+      }
+      float low = top[0], high = top[kLpStream / 64];
+#pragma unroll
+      for (int i = 1; i < kLpStream / 64; ++i) {
+        low = fmaxf(low, top[i]);
+        high = fmaxf(high, top[kLpStream / 64 + i]);
+      }
+      float bound;
+      if (k <= 16) bound = warp_kth(fmaxf(low, high), k);
+      else { // the largest of 64, k times, each time without the one that had it
+        unsigned a = ordered(fmaxf(low, high)), b = ordered(fminf(low, high)), best = 0;
+        for (int n = 0; n < k; ++n) {
+          best = __reduce_max_sync(0xffffffffu, a);
+          if (lane == __ffs(__ballot_sync(0xffffffffu, a == best)) - 1u) {
+            a = b;
+            b = 0;
+          }
+        }
+        bound = unordered(best);
+      }
+      u64key threshold = 0; // larger keys are wanted
+      unsigned hits = 0;
+      // the pieces behind the first `hits` notes of the list, one per lane
+      auto look_again = [&] {
+        __syncwarp();
+        for (unsigned h0 = 0; h0 < hits; h0 += 32) {
+          const bool mine = h0 + lane < hits;
+          const unsigned hit = mine ? sh.hits[h0 + lane] : 0, thread = hit % kLpStream, piece = hit / kLpStream;
+          for (unsigned t = piece << piece_log, n = 0; n < (1u << piece_log); ++n, ++t) {
+            const unsigned at0 = t * kTrip + thread;
+            float v[kLpUnroll * 4];
+            unsigned todo = 0;
+#pragma unroll
+            for (int u = 0; u < kLpUnroll; ++u) {
+              v[4 * u] = v[4 * u + 1] = v[4 * u + 2] = v[4 * u + 3] = -INFINITY;
+              if (mine) r.fetch(at0 + u * kLpStream, r.vectors, v + 4 * u);
+            }
+            if (mine) {
+#pragma unroll
+              for (int i = 0; i < kLpUnroll * 4; ++i) todo |= (v[i] >= bound ? 1u : 0u) << i;
+              if (threshold) { // of many equal logits only those before the last of the list are wanted
+                const float least = value_of(threshold);
+                const long long before = index_of(threshold), j0 = r.index(at0);
+#pragma unroll
+                for (int i = 0; i < kLpUnroll * 4; ++i)
+                  if (v[i] < least || (v[i] == least && j0 + (i / 4) * (4 * kLpStream) + (i & 3) >= before)) todo &= ~(1u << i);
+              }
+            }
+            while (__any_sync(0xffffffffu, todo != 0)) {
+              u64key key = 0;
+              if (todo) {
+                const unsigned i = __ffs(todo) - 1;
+                todo &= todo - 1;
+                float value = v[0];
+#pragma unroll
+                for (int m = 1; m < kLpUnroll * 4; ++m) value = i == m ? v[m] : value;
+                const unsigned at = at0 + (i / 4) * kLpStream;
+                const long long j = r.index(at) + (i & 3);
+                if (at < r.vectors && j >= 0 && j < (long long)p.cols) key = key_of(value, (unsigned)j);
+                if (key <= threshold) key = 0;
+              }
+              const unsigned with = __ballot_sync(0xffffffffu, key != 0), n_with = __popc(with);
+              if (count + n_with > kLpCandidates) {
+                threshold = cut_list(sh.list, count, sh.spare, k);
+                count = k;
+              }
+              if (key) sh.list[count + __popc(with & ((1u << lane) - 1))] = key;
+              count += n_with;
+            }
+          }
+          if (count > 128) { // many equal logits: most of the rest need not be looked at
+            threshold = cut_list(sh.list, count, sh.spare, k);
+            count = k;
+          }
+        }
+        hits = 0;
+        __syncwarp();
+      };
+      // the threads that reach it, then their pieces that do
+      unsigned threads = 0;
+#pragma unroll
+      for (int i = 0; i < kLpStream / 32; ++i) {
+        const unsigned with = __ballot_sync(0xffffffffu, top[i] >= bound);
+        if (top[i] >= bound) sh.reach[threads + __popc(with & ((1u << lane) - 1))] = (unsigned char)(i * 32 + lane);
+        threads += __popc(with);
+      }
+      __syncwarp();
+      for (unsigned piece = 0; piece < here; ++piece) {
+        // a logit that equals the last of a cut list comes after it: pieces follow the row
+        const float least = threshold ? max_nan(bound, next_above(value_of(threshold))) : bound;
+        for (unsigned i = 0; i < threads; i += 32) {
+          const unsigned thread = i + lane < threads ? sh.reach[i + lane] : 0;
+          const bool hit = i + lane < threads && note[piece * kLpStream + thread] >= least;
+          const unsigned with = __ballot_sync(0xffffffffu, hit);
+          if (!with) continue;
+          if (hit) sh.hits[hits + __popc(with & ((1u << lane) - 1))] = (unsigned short)(piece * kLpStream + thread);
+          hits += __popc(with);
+          if (hits > kLpHits - 32) look_again();
+        }
+        if (hits > 96) look_again();
+      }
+      look_again();
+      if (count > 64) cut_list(sh.list, count, sh.spare, k);
+      else {
+        sh.spare[lane] = 0;
+        __syncwarp();
+        select_best(sh.spare, sh.list, count, k, lane, 32);
+        __syncwarp();
+      }
+    }
+    rows_arrive(3 + buf); // the notes are used up
+    double log_s, shift;
+    int empty;
+    if (lane == 0) report_row(p, row, st, token, x_token, log_s, shift, empty);
+    if (TOP) {
+      log_s = __shfl_sync(0xffffffffu, log_s, 0);
+      shift = __shfl_sync(0xffffffffu, shift, 0);
+      empty = __shfl_sync(0xffffffffu, empty, 0);
+      if ((int)lane < k) report_alternative(p, row, lane, sh.spare[lane], log_s, shift, empty);
+      __syncwarp();
+    }
   }
 }
 
@@ -637,15 +893,34 @@ void plast_b200_token_logprob(const Tensor *logits, const Tensor *tokens, Tensor
   p.top = (int)top;
   p.scale_log2 = (float)(1.4426950408889634 / (double)temperature);
   p.temperature = temperature;
-  // many rows: smaller CTAs, so that the ends of some rows (a chain of short steps) overlap the streams of
-  // others (2048 rows of 32768, 16 alternatives: 99 us with 512 threads)
-  const unsigned threads = lp_threads(s.cols, s.rows >= 2 * (u64)sm_count() ? LP_THREADS : kLpMaxThreads);
+  // Rows for every resident CTA (four to an SM), and long enough that a stream covers the end of the row
+  // before: the persistent kernel. Against the other one, us, with 0 / 1 / 16 / 32 alternatives:
+  //   2048 rows of 32768: 48 / 60 / 67 / 89  (49 / 62 / 81 / 94)
+  //   4096 rows of 16384: 46 / 71 / 79 / 116 (53 / 76 / 98 / 114)
+  //   4096 rows of 8192:  28 / 56 / 64 / 99  (34 / 55 / 67 / 78)
+  //   16384 rows of 2048: 83 / 182 / .. / 327 (46 / 89 / .. / 126)
+  const u64 resident = (u64)sm_count() * kLpRowCtas;
+  const bool by_rows = s.rows >= resident && s.cols >= (top == 0 ? 4096 : top <= 16 ? 8192 : 16384);
+  // The other one: with rows for all resident CTAs smaller ones, so that the ends of some rows overlap the
+  // streams of others (4096 rows of 16384, 16 alternatives: 132 us with 512 threads, 98 with 256)
+  const unsigned threads = lp_threads(s.cols, s.rows >= resident ? 256 : kLpMaxThreads);
   // few rows: split each over a cluster while every CTA keeps at least one full trip
   p.cluster = 1;
   while (p.cluster < kLpMaxCluster && s.rows * p.cluster < (u64)sm_count() &&
          s.cols / (p.cluster * 2) >= (u64)threads * 4 * kLpUnroll)
     p.cluster *= 2;
   const bool unit = s.col_stride == 1 || s.cols == 1;
+  if (by_rows) {
+    const dim3 row_grid((unsigned)resident);
+    const unsigned rows = (unsigned)s.rows;
+    PB_CUDA(top ? (unit ? launch_k(token_logprob_rows_kernel<true, true>, row_grid, dim3(kLpRowThreads), 0, stream(), p, rows)
+                        : launch_k(token_logprob_rows_kernel<false, true>, row_grid, dim3(kLpRowThreads), 0, stream(), p, rows))
+                : (unit ? launch_k(token_logprob_rows_kernel<true, false>, row_grid, dim3(kLpRowThreads), 0, stream(), p, rows)
+                        : launch_k(token_logprob_rows_kernel<false, false>, row_grid, dim3(kLpRowThreads), 0, stream(), p, rows)));
+    count_launch();
+    note_kernel(top ? "token_logprob_rows_top" : "token_logprob_rows");
+    return end_call();
+  }
   const dim3 grid((unsigned)(s.rows * p.cluster)), block(threads);
   cudaError_t e;
   if (top) e = unit ? launch_kc(p.cluster, token_logprob_kernel<true, true>, grid, block, 0, stream(), p)

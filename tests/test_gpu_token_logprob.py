@@ -337,3 +337,48 @@ def test_offsets_beyond_32_bits():
     # about 2^12 additions in a thread
     np.testing.assert_allclose(lp.numpy()[1:], [3 - np.log(np.exp(3) + rest), 4 - np.log(np.exp(4) + np.exp(2) + rest)],
                                atol=2.0 ** -12 + 1e-5)
+
+
+@pytest.mark.parametrize("cols", [8192, 16387, 50001, 70000])
+@pytest.mark.parametrize("kind", ["random", "equal", "two_values", "ascending", "descending", "masked"])
+def test_many_long_rows(kind, cols):
+    """More rows than resident CTAs: the persistent kernel, several rows per CTA, lists that overflow, empty rows."""
+    rs = np.random.RandomState(cols)
+    rows, i = 1300 if cols < 20000 else 620, np.arange(cols)
+    x = {"random": lambda: rs.randn(rows, cols) * 3, "equal": lambda: np.broadcast_to(rs.randn(rows, 1), (rows, cols)),
+         "two_values": lambda: np.broadcast_to((i * 7919 % 3 == 0) * 1.0, (rows, cols)),
+         "ascending": lambda: np.broadcast_to(i * 1e-3, (rows, cols)),
+         "descending": lambda: np.broadcast_to(-i * 1e-3, (rows, cols)),
+         "masked": lambda: np.where(rs.rand(rows, cols) < 0.999, -np.inf, rs.randn(rows, cols))}[kind]().astype(np.float32)
+    x = np.array(x)
+    x[5] = -np.inf
+    x[7, 3] = np.nan
+    token = rs.randint(-1, cols + 1, rows)
+    for top in (0, 1, 5, 16) if cols < 16384 else (0, 1, 20, 32):
+        t = run(x, token, 0.8, top)
+        assert pb.last_kernel() == ("token_logprob_rows_top" if top else "token_logprob_rows")
+        pick = np.r_[0:12, rs.randint(0, rows, 20), rows - 3:rows]
+        ref = R.token_logprob(x[pick], token[pick], 0.8, top)
+        # the merges and a thread's additions as in log_sum_bound, with up to cols / 256 additions
+        bound = R.log_sum_bound(ref, cols) + cols / 256 * U
+        for k in ("logprob", "log_norm", "entropy"):
+            got = t[k].numpy()[pick]
+            np.testing.assert_allclose(got, ref[k], rtol=2 * U, atol=bound * (1 if k != "entropy" else 1 + 2 * np.log(cols)), err_msg=k)
+        if top:
+            assert np.array_equal(t["top_index"].numpy()[pick], ref["top_index"])
+            np.testing.assert_allclose(t["top_logprob"].numpy()[pick], ref["top_logprob"], rtol=2 * U, atol=bound)
+
+
+def test_many_long_rows_of_a_view():
+    rs = np.random.RandomState(3)
+    x, token = rs.randn(620, 8201).astype(np.float32), rs.randint(0, 8201, 620)
+    for view in (strided, transposed):
+        check(run(x, token, 1.3, 6, view=view), x, token, 1.3, 6)
+        assert pb.last_kernel() == "token_logprob_rows_top"
+
+
+@pytest.mark.parametrize("rows, cols, top", [(591, 16384, 8), (600, 4096, 0), (600, 4095, 0), (600, 8191, 1), (1300, 16383, 32), (1300, 300, 3)])
+def test_on_both_sides_of_the_rule(rows, cols, top):
+    rs = np.random.RandomState(rows + cols)
+    x, token = rs.randn(rows, cols).astype(np.float32), rs.randint(0, cols, rows)
+    check(run(x, token, 1.0, top), x, token, 1.0, top)
