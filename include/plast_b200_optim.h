@@ -110,14 +110,15 @@ typedef struct {
  *   data = data (1 - lr weight_decay) - lr s orthogonalised(u)
  * optimizer->m holds one momentum per parameter, contiguous and of its size; where it is NULL the
  * first step creates zeros for the list (freed by plast_b200_muon_state_release, like Adam's), so a
- * first step is not captured into a graph. A call that is refused changes nothing. */
+ * first step is not captured into a graph. No parameter or momentum may overlap another buffer of the
+ * call. A call that is refused changes nothing. */
 void muon_step_cuda(Muon *optimizer, Tensor **parameters, int num_parameters);
 void plast_b200_muon_state_release(Tensor **m);
 
 /* The orthogonalisation alone, for `count` matrices at once: X = x / (|x|_F + epsilon), then `steps`
  * times (0 to PLAST_MUON_MAX_STEPS) X <- a X + (b A + c A A) X with A = X X^T (of the smaller side)
  * and (a, b, c) = (3.4445, -4.7750, 2.0315). Contiguous FLOAT32 tensors as above; an output may be
- * its own input. The norm is summed in 64 bits, every product has fp32 accuracy. A matrix of zeros
+ * its own input and overlaps no other tensor of the call. The norm is summed in 64 bits, every product has fp32 accuracy. A matrix of zeros
  * gives zeros; a NaN or an infinity makes its matrix NaN. */
 void plast_b200_orthogonalise(const Tensor **inputs, Tensor **outputs, int count, int steps, float epsilon);
 

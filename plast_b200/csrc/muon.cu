@@ -1192,12 +1192,27 @@ static bool check_matrix(const char *name, int i, const Tensor *t, const char *w
   return true;
 }
 
-// A buffer that is written must appear once.
-static bool all_distinct(const char *name, std::vector<const void *> written) {
-  std::sort(written.begin(), written.end());
-  if (std::adjacent_find(written.begin(), written.end()) == written.end()) return true;
-  set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: one buffer would be written twice", name);
-  return false;
+// The buffers of a call. One that is written overlaps no other, but that it may be its own matrix's input.
+struct MuonSpan {
+  const char *begin, *end;
+  bool written;
+  int matrix;
+};
+static MuonSpan span_of(const Tensor *t, bool written, int matrix) {
+  const char *p = (const char *)t->data;
+  return MuonSpan{p, p + numel(t) * 4, written, matrix};
+}
+static bool apart(const char *name, std::vector<MuonSpan> spans, bool in_place) {
+  std::sort(spans.begin(), spans.end(), [](const MuonSpan &a, const MuonSpan &b) { return a.begin < b.begin; });
+  for (size_t i = 0; i < spans.size(); ++i)
+    for (size_t k = i + 1; k < spans.size() && spans[k].begin < spans[i].end; ++k) {
+      const MuonSpan &a = spans[i], &b = spans[k];
+      if (!a.written && !b.written) continue;
+      if (in_place && a.written != b.written && a.matrix == b.matrix && a.begin == b.begin && a.end == b.end) continue;
+      set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: a buffer that is written overlaps another one", name);
+      return false;
+    }
+  return true;
 }
 
 static bool check_steps(const char *name, int steps, float epsilon) {
@@ -1274,7 +1289,7 @@ static void muon_step(Muon *opt, Tensor **parameters, int num_parameters) {
     return set_error(PLAST_B200_ERR_UNSUPPORTED, "muon: unknown scale rule");
   std::vector<MuonMat> mats;
   std::vector<int> index;
-  std::vector<const void *> written;
+  std::vector<MuonSpan> spans;
   for (int i = 0; i < num_parameters; ++i) {
     const Tensor *p = parameters[i];
     if (!p || !p->grad) continue;
@@ -1293,9 +1308,10 @@ static void muon_step(Muon *opt, Tensor **parameters, int num_parameters) {
     q.keep = 1.0f - opt->lr * opt->weight_decay;
     mats.push_back(q);
     index.push_back(i);
-    written.push_back(q.w);
+    spans.push_back(span_of(p, true, i));
+    spans.push_back(span_of(p->grad, false, i));
   }
-  if (!all_distinct(name, written)) return;
+  if (!apart(name, spans, false)) return;
   // momenta: the caller's, or made here on the first step
   bool made = false;
   if (opt->m) {
@@ -1315,9 +1331,9 @@ static void muon_step(Muon *opt, Tensor **parameters, int num_parameters) {
     if (numel(m) != (u64)mats[k].rows * mats[k].cols)
       return set_error(PLAST_B200_ERR_SHAPE, "muon: momentum %d differs in size", index[k]);
     mats[k].v = (float *)m->data;
-    written.push_back(m->data);
+    if (!made) spans.push_back(span_of(m, true, index[k]));
   }
-  if (!all_distinct(name, written)) return;
+  if (!made && !apart(name, spans, false)) return;
   if (mats.empty()) return;
   run_matrices(mats, opt->momentum, opt->epsilon, opt->nesterov != 0, opt->ns_steps);
   note_kernel("muon");
@@ -1329,7 +1345,7 @@ static void orthogonalise(const Tensor **inputs, Tensor **outputs, int count, in
   if ((!inputs || !outputs) && count > 0) return set_error(PLAST_B200_ERR_NULL, "%s: inputs or outputs is NULL", name);
   if (!check_steps(name, steps, epsilon)) return;
   std::vector<MuonMat> mats;
-  std::vector<const void *> written;
+  std::vector<MuonSpan> spans;
   for (int i = 0; i < count; ++i) {
     MuonMat q = {};
     if (!inputs[i] || !outputs[i]) return set_error(PLAST_B200_ERR_NULL, "%s: tensor %d is NULL", name, i);
@@ -1343,14 +1359,10 @@ static void orthogonalise(const Tensor **inputs, Tensor **outputs, int count, in
     q.keep = 0.0f;
     q.rate = -1.0f;
     mats.push_back(q);
-    written.push_back(q.w);
+    spans.push_back(span_of(inputs[i], false, i));
+    spans.push_back(span_of(outputs[i], true, i));
   }
-  if (!all_distinct(name, written)) return;
-  // an output may be its own input, but not another one's
-  std::sort(written.begin(), written.end());
-  for (const MuonMat &q : mats)
-    if (q.g != q.w && std::binary_search(written.begin(), written.end(), (const void *)q.g))
-      return set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: an output is another matrix's input", name);
+  if (!apart(name, spans, true)) return;
   if (mats.empty()) return;
   run_matrices(mats, 0.0f, epsilon, 0, steps);
   note_kernel("orthogonalise");

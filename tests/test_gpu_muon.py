@@ -231,6 +231,49 @@ def test_graph_replays_match_eager_steps():
         assert np.array_equal(g, w)
 
 
+def test_two_streams_and_two_graphs_at_once():
+    """Calls on two streams, then two captured calls replayed on two streams, neither waiting for the other."""
+    torch = pytest.importorskip("torch")
+    rs = np.random.RandomState(19)
+    xs = [[pb.Tensor.from_numpy(rs.randn(*s).astype(np.float32)) for s in shapes]
+          for shapes in ([(520, 900), (130, 70)], [(1000, 600)])]
+    want = []
+    for group in xs:
+        outs = [pb.Tensor(x.shape) for x in group]
+        O.orthogonalise(group, outs)
+        want.append([o.numpy() for o in outs])
+    outs = [[pb.Tensor(x.shape) for x in group] for group in xs]
+    streams, graphs = [torch.cuda.Stream() for _ in xs], []
+
+    def check():
+        torch.cuda.synchronize()
+        for group, w in zip(outs, want):
+            for o, v in zip(group, w):
+                assert np.array_equal(o.numpy(), v)
+                o.zero_()
+        torch.cuda.synchronize()
+
+    pb.synchronize()
+    try:
+        for _ in range(5):
+            for stream, group, out in zip(streams, xs, outs):
+                pb.lib.plast_b200_set_stream(C.c_void_p(stream.cuda_stream))
+                O.orthogonalise(group, out)
+        check()
+        for stream, group, out in zip(streams, xs, outs):
+            pb.lib.plast_b200_set_stream(C.c_void_p(stream.cuda_stream))
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                O.orthogonalise(group, out)
+        for _ in range(5):
+            for stream, graph in zip(streams, graphs):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        check()
+    finally:
+        pb.lib.plast_b200_set_stream(None)
+
+
 def test_nothing_outside_the_matrices_is_written():
     rs = np.random.RandomState(10)
     host = rs.randn(3000).astype(np.float32)

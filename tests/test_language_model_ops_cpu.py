@@ -201,6 +201,17 @@ def test_muon_refusals_change_nothing():
     refused("UNSUPPORTED", f, [p, p])
     refused("UNSUPPORTED", f, params((4, 4), (4, 4)), moments=[T(4, 4)] * 2)
     refused("NULL", f, params((4, 4), (4, 4)), moments=[T(4, 4), None])
+    base = T(12, 4)
+    halves = [base.view((8, 4), (4, 1)), base.view((8, 4), (4, 1), offset=16)]     # rows 0 to 7 and 4 to 11
+    for t in halves:
+        t.set_grad(T(8, 4))
+    refused("UNSUPPORTED", f, halves)
+    refused("UNSUPPORTED", f, params((8, 4), (8, 4)), moments=halves)
+    t = base.view((8, 4), (4, 1))
+    t.set_grad(base.view((8, 4), (4, 1), offset=4))
+    refused("UNSUPPORTED", f, [t])                            # its own gradient, a row on
+    t.set_grad(T(8, 4))
+    refused("UNSUPPORTED", f, [t], moments=[base.view((8, 4), (4, 1))])
     refused("SHAPE", f, params((4, 4)), moments=[T(4, 3)])
     refused("DTYPE", f, params((4, 4)), moments=[T(4, 4, dtype=I)])
     t = T(8, 8).transpose(0, 1)
@@ -232,5 +243,8 @@ def test_orthogonalise_refusals():
     refused("UNSUPPORTED", O.orthogonalise, [x.transpose(0, 1)], [T(6, 4)])
     refused("UNSUPPORTED", O.orthogonalise, [x, y], [o, o])
     refused("UNSUPPORTED", O.orthogonalise, [x, y], [y, o])
+    base = T(8, 6)
+    refused("UNSUPPORTED", O.orthogonalise, [base.view((4, 6), (6, 1))], [base.view((4, 6), (6, 1), offset=6)])
+    refused("UNSUPPORTED", O.orthogonalise, [x, y], [base.view((4, 6), (6, 1)), base.view((4, 6), (6, 1), offset=18)])
     refused("UNSUPPORTED", O.orthogonalise, [x], [o], 40)
     refused("UNSUPPORTED", O.orthogonalise, [x], [o], 5, -1.0)
