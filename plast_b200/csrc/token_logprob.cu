@@ -42,7 +42,7 @@ struct LpParams {
   int top;
   unsigned cluster;
   float scale_log2; // log2(e) / T
-  double temperature;
+  double inv_temperature;
 };
 
 __device__ __forceinline__ float ex2(float t) {
@@ -85,9 +85,9 @@ struct LpStat {
     u += o.u;
   }
   // all lanes of a warp, in a tree (every lane ends with the same bits: the merge is symmetric)
-  __device__ __forceinline__ void merge_warp(float c) {
+  __device__ __forceinline__ void merge_warp(float c, int lanes = 32) {
 #pragma unroll 1
-    for (int o = 16; o; o >>= 1) {
+    for (int o = lanes / 2; o; o >>= 1) {
       const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o),
                   ou = __shfl_xor_sync(0xffffffffu, u, o);
       merge(om, os, ou, c);
@@ -234,11 +234,11 @@ __device__ __forceinline__ void report_row(const LpParams &p, unsigned row, cons
   empty = st.s == 0.0f; // every logit is -inf
   log_s = log((double)st.s);
   shift = (double)st.m;
-  const double L = empty ? -INFINITY : shift / p.temperature + log_s;
+  const double L = empty ? -INFINITY : shift * p.inv_temperature + log_s;
   double h = empty ? 0.0 : log_s - kLn2 * ((double)st.u / (double)st.s);
   if (h < 0.0) h = 0.0; // rounding of U; a NaN passes
   double lp = 0.0;
-  if (token >= 0) lp = empty ? -INFINITY : ((double)x_token - shift) / p.temperature - log_s;
+  if (token >= 0) lp = empty ? -INFINITY : ((double)x_token - shift) * p.inv_temperature - log_s;
   p.logprob[row] = (float)lp;
   if (p.entropy) p.entropy[row] = (float)h;
   if (p.log_norm) p.log_norm[row] = (float)L;
@@ -247,7 +247,7 @@ __device__ __forceinline__ void report_row(const LpParams &p, unsigned row, cons
 __device__ __forceinline__ void report_alternative(const LpParams &p, unsigned row, int i, u64key key, double log_s, double shift, int empty) {
   const u64 at = (u64)row * p.top + i;
   p.top_index[at] = key ? (int)index_of(key) : -1;
-  p.top_logprob[at] = !key ? NAN : empty ? -INFINITY : (float)(((double)value_of(key) - shift) / p.temperature - log_s);
+  p.top_logprob[at] = !key ? NAN : empty ? -INFINITY : (float)(((double)value_of(key) - shift) * p.inv_temperature - log_s);
 }
 
 // A row (or slice) as vectors of four logits; the first one starts at the 16-byte boundary at or before it.
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kLpMaxThreads, 2) token_logprob_kernel(const _
 // of ties ends with the exact answer.
 constexpr int kLpRowCtas = 4, kLpStream = 256, kLpRowThreads = kLpStream + 32, kLpPieces = 16, kLpHits = 256;
 struct LpRowShared {
-  float note[2][kLpPieces * kLpStream];
+  float note[2][kLpPieces * kLpStream], whole[2][kLpStream];
   float stat[2][kLpStream / 32][3];
   unsigned trips[2];
   u64key list[kLpCandidates], spare[PLAST_TOKEN_TOP_MAX];
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kLpRowThreads, kLpRowCtas) token_logprob_rows_
       LpStat st;
       st.init();
       if (turn >= 2) rows_sync(3 + buf);
-      float note = -INFINITY;
+      float note = -INFINITY, whole = -INFINITY;
       unsigned trips = 0;
       for (unsigned base = 0; base < r.vectors; base += kTrip) {
         float v[kLpUnroll * 4];
@@ -511,10 +511,12 @@ __global__ void __launch_bounds__(kLpRowThreads, kLpRowCtas) token_logprob_rows_
           ++trips;
           if ((trips & ((1u << piece_log) - 1)) == 0 || base + kTrip >= r.vectors) {
             sh.note[buf][((trips - 1) >> piece_log) * kLpStream + threadIdx.x] = note;
+            whole = fmaxf(whole, note);
             note = -INFINITY;
           }
         }
       }
+      if (TOP) sh.whole[buf][threadIdx.x] = whole;
       st.merge_warp(c);
       if (lane == 0) {
         sh.stat[buf][warp][0] = st.m;
@@ -542,8 +544,9 @@ __global__ void __launch_bounds__(kLpRowThreads, kLpRowCtas) token_logprob_rows_
     LpStat st;
     st.init();
     if (lane < kLpStream / 32) { st.m = sh.stat[buf][lane][0]; st.s = sh.stat[buf][lane][1]; st.u = sh.stat[buf][lane][2]; }
-    st.merge_warp(c);
+    st.merge_warp(c, kLpStream / 32);
     unsigned count = 0;
+    bool used_up = false; // the notes
     if (TOP) {
       const unsigned trips = sh.trips[buf], here = (trips + (1u << piece_log) - 1) >> piece_log;
       const float *note = sh.note[buf];
@@ -551,11 +554,7 @@ __global__ void __launch_bounds__(kLpRowThreads, kLpRowCtas) token_logprob_rows_
       // (of more than 16: of the lanes' two halves)
       float top[kLpStream / 32];
 #pragma unroll
-      for (int i = 0; i < kLpStream / 32; ++i) {
-        top[i] = -INFINITY;
-#pragma unroll 4
-        for (unsigned piece = 0; piece < here; ++piece) top[i] = fmaxf(top[i], note[piece * kLpStream + i * 32 + lane]);
-      }
+      for (int i = 0; i < kLpStream / 32; ++i) top[i] = sh.whole[buf][i * 32 + lane];
       float low = top[0], high = top[kLpStream / 64];
 #pragma unroll
       for (int i = 1; i < kLpStream / 64; ++i) {
@@ -563,7 +562,8 @@ __global__ void __launch_bounds__(kLpRowThreads, kLpRowCtas) token_logprob_rows_
         high = fmaxf(high, top[kLpStream / 64 + i]);
       }
       float bound;
-      if (k <= 16) bound = warp_kth(fmaxf(low, high), k);
+      if (k <= 4) bound = warp_nth(fmaxf(low, high), k);
+      else if (k <= 16) bound = warp_kth(fmaxf(low, high), k);
       else { // the largest of 64, k times, each time without the one that had it
         unsigned a = ordered(fmaxf(low, high)), b = ordered(fminf(low, high)), best = 0;
         for (int n = 0; n < k; ++n) {
@@ -642,30 +642,78 @@ __global__ void __launch_bounds__(kLpRowThreads, kLpRowCtas) token_logprob_rows_
         threads += __popc(with);
       }
       __syncwarp();
-      for (unsigned piece = 0; piece < here; ++piece) {
-        // a logit that equals the last of a cut list comes after it: pieces follow the row
-        const float least = threshold ? max_nan(bound, next_above(value_of(threshold))) : bound;
-        for (unsigned i = 0; i < threads; i += 32) {
-          const unsigned thread = i + lane < threads ? sh.reach[i + lane] : 0;
-          const bool hit = i + lane < threads && note[piece * kLpStream + thread] >= least;
-          const unsigned with = __ballot_sync(0xffffffffu, hit);
-          if (!with) continue;
-          if (hit) sh.hits[hits + __popc(with & ((1u << lane) - 1))] = (unsigned short)(piece * kLpStream + thread);
-          hits += __popc(with);
-          if (hits > kLpHits - 32) look_again();
+      // Ties: where the k-th best is as large as the best, the first k logits of that value are the answer, in an
+      // empty row the first k of all. They are looked for at the start of the row.
+      bool found = false;
+      if (threads > 32 && __all_sync(0xffffffffu, fmaxf(low, high) <= bound)) {
+        float v[16];
+#pragma unroll
+        for (unsigned i = 0; i < 16; ++i) v[i] = i * 32 + lane < p.cols ? r.x[(u64)(i * 32 + lane) * r.stride] : NAN;
+#pragma unroll
+        for (unsigned i = 0; i < 16; ++i) {
+          const unsigned with = __ballot_sync(0xffffffffu, v[i] == bound), at = count + __popc(with & ((1u << lane) - 1));
+          if (v[i] == bound && at < (unsigned)k) sh.spare[at] = key_of(v[i], i * 32 + lane);
+          count += __popc(with);
         }
-        if (hits > 96) look_again();
+        found = count >= (unsigned)k;
+        count = found ? k : 0;
       }
-      look_again();
-      if (count > 64) cut_list(sh.list, count, sh.spare, k);
-      else {
-        sh.spare[lane] = 0;
-        __syncwarp();
-        select_best(sh.spare, sh.list, count, k, lane, 32);
-        __syncwarp();
+      if (!found) {
+        // a thread per lane (two where k is large), its pieces as bits
+        bool listed = threads <= 64;
+        for (unsigned i = 0; listed && i < threads; i += 32) {
+          const unsigned thread = i + lane < threads ? sh.reach[i + lane] : 0;
+          unsigned pieces = 0;
+          if (i + lane < threads) {
+#pragma unroll
+            for (unsigned piece = 0; piece < (unsigned)kLpPieces; ++piece)
+              if (piece < here && note[piece * kLpStream + thread] >= bound) pieces |= 1u << piece;
+          }
+          unsigned at = __popc(pieces);
+#pragma unroll
+          for (int o = 1; o < 32; o *= 2) {
+            const unsigned before = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= (unsigned)o) at += before;
+          }
+          const unsigned more = __shfl_sync(0xffffffffu, at, 31);
+          listed = hits + more <= (unsigned)kLpHits;
+          if (!listed) break;
+          at += hits - __popc(pieces);
+          for (; pieces; pieces &= pieces - 1)
+            sh.hits[at++] = (unsigned short)((__ffs(pieces) - 1) * kLpStream + thread);
+          hits += more;
+        }
+        if (listed) {
+          used_up = true;
+          __syncwarp();
+          rows_arrive(3 + buf);
+        } else hits = 0;
+        if (!listed)
+          for (unsigned piece = 0; piece < here; ++piece) {
+            // a logit that equals the last of a cut list comes after it: pieces follow the row
+            const float least = threshold ? max_nan(bound, next_above(value_of(threshold))) : bound;
+            for (unsigned i = 0; i < threads; i += 32) {
+              const unsigned thread = i + lane < threads ? sh.reach[i + lane] : 0;
+              const bool hit = i + lane < threads && note[piece * kLpStream + thread] >= least;
+              const unsigned with = __ballot_sync(0xffffffffu, hit);
+              if (!with) continue;
+              if (hit) sh.hits[hits + __popc(with & ((1u << lane) - 1))] = (unsigned short)(piece * kLpStream + thread);
+              hits += __popc(with);
+              if (hits > kLpHits - 32) look_again();
+            }
+            if (hits > 96) look_again();
+          }
+        look_again();
+        if (count > 96) cut_list(sh.list, count, sh.spare, k);
+        else {
+          sh.spare[lane] = 0;
+          __syncwarp();
+          select_best(sh.spare, sh.list, count, k, lane, 32);
+        }
       }
+      __syncwarp();
     }
-    rows_arrive(3 + buf); // the notes are used up
+    if (!used_up) rows_arrive(3 + buf);
     double log_s, shift;
     int empty;
     if (lane == 0) report_row(p, row, st, token, x_token, log_s, shift, empty);
@@ -892,7 +940,7 @@ void plast_b200_token_logprob(const Tensor *logits, const Tensor *tokens, Tensor
   p.cols = (unsigned)s.cols;
   p.top = (int)top;
   p.scale_log2 = (float)(1.4426950408889634 / (double)temperature);
-  p.temperature = temperature;
+  p.inv_temperature = 1.0 / (double)temperature;
   // Rows for every resident CTA (four to an SM), and long enough that a stream covers the end of the row
   // before: the persistent kernel. Against the other one, us, with 0 / 1 / 16 / 32 alternatives:
   //   2048 rows of 32768: 48 / 60 / 67 / 89  (49 / 62 / 81 / 94)
