@@ -447,10 +447,10 @@ __global__ void __launch_bounds__(kLpMaxThreads, 2) token_logprob_kernel(const _
 
 // ---- forward, many rows -------------------------------------------------------------------------------
 // A persistent CTA whose eight warps stream one row after the other while a ninth finishes the row before.
-// The end of a row is a chain of short steps (joining statistics, alternatives, logarithms) of 4 us, with
-// alternatives 6 to 9; in the streaming warps it leaves HBM idle for as long. Measured: 8192 rows of 65536 in
-// 314 us without alternatives (6.8 TB/s) and 348 with sixteen. With short rows the finishing warp is the
-// bound, hence the rule at the launch.
+// The end of a row is a chain of short steps (joining statistics, alternatives, logarithms) of 3 us, with
+// alternatives 6 to 7 beside the stream; in the streaming warps it leaves HBM idle for as long. Measured: 8192
+// rows of 65536 in 313 us without alternatives (6.9 TB/s) and 343 with sixteen, 2048 rows of 32768 in 49 and 56
+// (the last row's end among them). With short rows the finishing warp is the bound, hence the rule at the launch.
 //
 // The stream notes the largest logit of every thread and piece (one or more trips). A lane of the finishing
 // warp looks after eight threads; the k-th largest of the lanes' largest notes (above 16: of the largest
@@ -943,10 +943,11 @@ void plast_b200_token_logprob(const Tensor *logits, const Tensor *tokens, Tensor
   p.inv_temperature = 1.0 / (double)temperature;
   // Rows for every resident CTA (four to an SM), and long enough that a stream covers the end of the row
   // before: the persistent kernel. Against the other one, us, with 0 / 1 / 16 / 32 alternatives:
-  //   2048 rows of 32768: 48 / 60 / 67 / 89  (49 / 62 / 81 / 94)
-  //   4096 rows of 16384: 46 / 71 / 79 / 116 (53 / 76 / 98 / 114)
-  //   4096 rows of 8192:  28 / 56 / 64 / 99  (34 / 55 / 67 / 78)
-  //   16384 rows of 2048: 83 / 182 / .. / 327 (46 / 89 / .. / 126)
+  //   2048 rows of 32768: 48 / 54 / 56 / 77  (49 / 61 / 80 / 93)
+  //   4096 rows of 16384: 46 / 58 / 67 / 106 (52 / 74 / 97 / 112)
+  //   4096 rows of 8192:  27 / 47 / 56 / 93  (32 / 53 / 65 / 77)
+  //   4096 rows of 4096:  19 / 41 / 49 / 85  (23 / 42 / 47 / 57)
+  //   4096 rows of 2048:  21 / 42 / 49 / 83  (12 / 21 / 26 / 36)
   const u64 resident = (u64)sm_count() * kLpRowCtas;
   const bool by_rows = s.rows >= resident && s.cols >= (top == 0 ? 4096 : top <= 16 ? 8192 : 16384);
   // The other one: with rows for all resident CTAs smaller ones, so that the ends of some rows overlap the
