@@ -877,6 +877,31 @@ static bool check_stats(const Tensor *t, u64 rows) {
   return true;
 }
 
+// Whether the kernel for many rows serves. Against the other one, measured in us with 0 / 1 / 16 / 32
+// alternatives (or, with fewer rows than resident CTAs, 0 / 5 / 20):
+//   rows for every resident CTA, four to an SM: where a row's stream covers the end of the row before
+//     2048 rows of 32768: 48 / 54 / 56 / 77  (49 / 61 / 80 / 93)
+//     4096 rows of 16384: 46 / 58 / 67 / 106 (52 / 74 / 97 / 112)
+//     4096 rows of 8192:  27 / 47 / 56 / 93  (32 / 53 / 65 / 77)
+//     4096 rows of 4096:  19 / 41 / 49 / 85  (23 / 42 / 47 / 57)
+//     4096 rows of 2048:  21 / 42 / 49 / 83  (12 / 21 / 26 / 36)
+//   more rows than the other one has resident CTAs, two to an SM:
+//     450 rows of 60000:  21 / 27 / 28 (25 / 37 / 50)
+//     300 rows of 200000: 57 / 65 / 67 (54 / 66 / 80)
+//     590 rows of 4096:   5.6 / 7.9 / 9.6 (4.7 / 8.3 / 10.6)
+//   fewer rows: for the alternatives' sake, up to the length where a row is better shared by a cluster
+//     200 rows of 16384:  5.5 / 9.1 / 10.5 (5.4 / 10.4 / 15.1)
+//     75 rows of 60000:   9.9 / 14.8 / 16.1 (9.0 / 15.4 / 20.7)
+//     140 rows of 200000: 43 / 52 / 55 (22 / 30 / 41)
+//   few rows, with 20 alternatives: 24 rows of 24000: 10.4 (13.0), of 60000: 15.2 (15.0)
+static bool rows_kernel_serves(u64 rows, u64 cols, u64 top) {
+  const u64 sms = (u64)sm_count();
+  if (rows >= sms * kLpRowCtas) return cols >= (top == 0 ? 4096 : top <= 16 ? 8192 : 16384);
+  if (rows > sms * 2) return cols >= 8192;
+  if (top > 16 && cols >= 8192 && cols <= 40960) return true;
+  return top > 0 && rows >= sms / 2 && cols >= 16384 && cols <= 65536;
+}
+
 static unsigned lp_threads(u64 cols, unsigned most) { // one trip of the CTA covers threads * 16 logits
   unsigned t = most;
   while (t > 64 && (u64)t * 8 >= cols) t /= 2;
@@ -941,15 +966,8 @@ void plast_b200_token_logprob(const Tensor *logits, const Tensor *tokens, Tensor
   p.top = (int)top;
   p.scale_log2 = (float)(1.4426950408889634 / (double)temperature);
   p.inv_temperature = 1.0 / (double)temperature;
-  // Rows for every resident CTA (four to an SM), and long enough that a stream covers the end of the row
-  // before: the persistent kernel. Against the other one, us, with 0 / 1 / 16 / 32 alternatives:
-  //   2048 rows of 32768: 48 / 54 / 56 / 77  (49 / 61 / 80 / 93)
-  //   4096 rows of 16384: 46 / 58 / 67 / 106 (52 / 74 / 97 / 112)
-  //   4096 rows of 8192:  27 / 47 / 56 / 93  (32 / 53 / 65 / 77)
-  //   4096 rows of 4096:  19 / 41 / 49 / 85  (23 / 42 / 47 / 57)
-  //   4096 rows of 2048:  21 / 42 / 49 / 83  (12 / 21 / 26 / 36)
   const u64 resident = (u64)sm_count() * kLpRowCtas;
-  const bool by_rows = s.rows >= resident && s.cols >= (top == 0 ? 4096 : top <= 16 ? 8192 : 16384);
+  const bool by_rows = rows_kernel_serves(s.rows, s.cols, top);
   // The other one: with rows for all resident CTAs smaller ones, so that the ends of some rows overlap the
   // streams of others (4096 rows of 16384, 16 alternatives: 132 us with 512 threads, 98 with 256)
   const unsigned threads = lp_threads(s.cols, s.rows >= resident ? 256 : kLpMaxThreads);
@@ -960,7 +978,7 @@ void plast_b200_token_logprob(const Tensor *logits, const Tensor *tokens, Tensor
     p.cluster *= 2;
   const bool unit = s.col_stride == 1 || s.cols == 1;
   if (by_rows) {
-    const dim3 row_grid((unsigned)resident);
+    const dim3 row_grid((unsigned)std::min(s.rows, resident));
     const unsigned rows = (unsigned)s.rows;
     PB_CUDA(top ? (unit ? launch_k(token_logprob_rows_kernel<true, true>, row_grid, dim3(kLpRowThreads), 0, stream(), p, rows)
                         : launch_k(token_logprob_rows_kernel<false, true>, row_grid, dim3(kLpRowThreads), 0, stream(), p, rows))

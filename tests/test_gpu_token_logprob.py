@@ -377,7 +377,9 @@ def test_many_long_rows_of_a_view():
         assert pb.last_kernel() == "token_logprob_rows_top"
 
 
-@pytest.mark.parametrize("rows, cols, top", [(591, 16384, 8), (600, 4096, 0), (600, 4095, 0), (600, 8191, 1), (1300, 16383, 32), (1300, 300, 3)])
+@pytest.mark.parametrize("rows, cols, top", [(591, 16384, 8), (600, 4096, 0), (600, 4095, 0), (600, 8191, 1), (1300, 16383, 32), (1300, 300, 3),
+                                             (297, 8192, 0), (296, 8192, 0), (300, 8191, 5), (74, 16384, 1), (73, 16384, 1), (80, 65537, 4),
+                                             (1, 8192, 17), (3, 40960, 32), (3, 40961, 32), (2, 8191, 20)])
 def test_on_both_sides_of_the_rule(rows, cols, top):
     rs = np.random.RandomState(rows + cols)
     x, token = rs.randn(rows, cols).astype(np.float32), rs.randint(0, cols, rows)
