@@ -71,7 +71,8 @@ int plast_b200_rotary_frequencies(const PlastRotaryScaling *scaling, u64 rotated
  * its last dim ([head], [1, head], ...), or NULL for none. An output may be its own input.
  * Backward recomputes the norm from q and k, reads q_out->grad and k_out->grad and adds to the
  * gradients of q, k and the weights, each where requires_grad is set; weight gradients are summed in
- * a fixed order. (A forward that ran in place has overwritten what backward needs.) Inside a
+ * a fixed order. The sum of squares is held in 32 bits: a head whose elements pass about 10^18 overflows
+ * it and gives zeros. (A forward that ran in place has overwritten what backward needs.) Inside a
  * plast_b200_peer_reduce_begin / _end bracket the weight gradients are refused: this call does not
  * combine them across ranks. */
 typedef struct PlastQkNormParams {

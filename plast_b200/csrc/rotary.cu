@@ -465,11 +465,29 @@ static void launch_heads(HeadParams &p, int sides, unsigned max_blocks) {
   while (p.log_group < 5 && (1u << p.log_group) < p.slots) ++p.log_group;
   const unsigned per_lane = (p.slots + (1u << p.log_group) - 1) >> p.log_group;
   const unsigned groups = kHeadThreads >> p.log_group;
-  u64 rows = 0;
-  for (int i = 0; i < sides; ++i) rows += (u64)p.side[i].items * p.side[i].heads;
-  // heads per item: share the angles among up to 8 heads while the GPU stays full (1024 threads an SM)
+  // Heads per item, which share its angles: 1 to 8, whichever makes the turns of the GPU cheapest. A turn costs its
+  // heads and the angles, the latter in heads: 1.5 where little else is done, less beside more traffic. Measured
+  // with 1 .. 8 heads: rotary of 3000 positions, 32 heads, half rotated, with gradient 49 / 48 / 55 us for 2 / 4 / 8 (of
+  // 8196 positions 119 / 112 / 116); norm and rotation of 8192 positions, 32 + 8 heads, with gradient 209 / 190 / 182.
+  const unsigned per_sm = NORM && BACK ? 2 : per_lane * vec <= 4 && vec4 ? 4 : per_lane <= 2 ? 2 : 1;
+  const double angles = 2.0 * p.half / p.head * (BACK ? (NORM ? 0.4 : 0.8) : 1.5);
   unsigned share = 1;
-  while (share < 8 && (rows / (share * 2)) * (kHeadThreads / groups) >= (u64)sm_count() * 1024) share *= 2;
+  double least = 0.0;
+  for (unsigned n = 1; n <= 8; n *= 2) {
+    u64 blocks = 0;
+    for (int i = 0; i < sides; ++i) {
+      const HeadSide &sd = p.side[i];
+      const unsigned each = n < sd.heads ? n : sd.heads;
+      blocks += ((u64)sd.items * ((sd.heads + each - 1) / each) + groups - 1) / groups;
+    }
+    const u64 turns = (blocks + (u64)sm_count() * per_sm - 1) / ((u64)sm_count() * per_sm);
+    const double cost = (double)turns * ((n == 1 ? 1.6 : n) + angles); // one head alone leaves memory waiting
+    if (n == 1 || cost < least) {
+      least = cost;
+      share = n;
+    }
+    if (turns <= 1) break; // more heads per item take longer
+  }
   u64 want = 0;
   for (int i = 0; i < sides; ++i) {
     HeadSide &sd = p.side[i];
