@@ -744,7 +744,7 @@ struct LpGradParams {
 // A streaming pass: 4 B read and 8 B for the += per logit. A CTA takes a piece of one row (grid.y), so that a
 // thousand long rows end together: whole rows of 50001 run in 3.4 turns of the GPU.
 template <bool VEC>
-__global__ void __launch_bounds__(kLpMaxThreads) token_logprob_backward_kernel(const __grid_constant__ LpGradParams p) {
+__global__ void __launch_bounds__(256) token_logprob_backward_kernel(const __grid_constant__ LpGradParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const unsigned row = blockIdx.x;
@@ -1042,10 +1042,13 @@ void plast_b200_token_logprob_backward(Tensor *logits, const Tensor *tokens, con
              (((uintptr_t)p.x ^ (uintptr_t)p.dx) & 15) == 0;
   for (int d = 0; d < p.map.nd && vec; ++d)
     if (p.map.size[d] > 1) vec = ((p.map.stride[0][d] ^ p.map.stride[2][d]) & 3) == 0;
-  // pieces of at least 16384 logits, at most 65535 of them; a row may start up to three before its first vector
+  // Pieces of at least 8192 logits (16384 where that leaves 16 turns of the GPU and more), at most 65535 of them; a
+  // row may start up to three before its first vector. 1021 rows of 50001: 98 us (100 with 16384, 102 with 16384
+  // and 512 threads), 8192 of 65536: 953 us (965 with 8192, 975), 4000 of 8000: 60 us (63 with 512 threads).
   const unsigned items = vec ? (unsigned)((s.cols + 3 + 3) / 4) : (unsigned)s.cols;
-  p.piece = std::max(vec ? 4096u : 16384u, items / 65535 + 1);
-  const dim3 grid((unsigned)s.rows, (items + p.piece - 1) / p.piece), block(lp_threads(std::min<u64>(s.cols, 16384), kLpMaxThreads));
+  const bool many = s.rows * (items / 4096) >= (u64)sm_count() * 4 * 16;
+  p.piece = std::max(!vec ? 16384u : many ? 4096u : 2048u, items / 65535 + 1);
+  const dim3 grid((unsigned)s.rows, (items + p.piece - 1) / p.piece), block(lp_threads(s.cols, 256));
   PB_CUDA(vec ? launch_k(token_logprob_backward_kernel<true>, grid, block, 0, stream(), p)
               : launch_k(token_logprob_backward_kernel<false>, grid, block, 0, stream(), p));
   count_launch();
