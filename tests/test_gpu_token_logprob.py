@@ -231,14 +231,42 @@ def test_gradient(cols, temperature):
 
 
 @pytest.mark.parametrize("view,grad_view", [(strided, strided), (strided, None), (transposed, transposed), (None, strided)])
-def test_gradient_of_views(view, grad_view):
+@pytest.mark.parametrize("cols", [301, 40001])
+def test_gradient_of_views(view, grad_view, cols):
     rs = np.random.RandomState(8)
-    x, token = rs.randn(5, 301).astype(np.float32), rs.randint(0, 301, 5)
-    g, start = upstream(rs, 5), rs.randn(5, 301).astype(np.float32)
+    x, token = rs.randn(5, cols).astype(np.float32), rs.randint(0, cols, 5)
+    g, start = upstream(rs, 5), rs.randn(5, cols).astype(np.float32)
     ref = R.token_logprob(x, token, 1.0)
     want = want_grad(ref, token, 1.0, g, start)
     _, got = backward(x, token, 1.0, g, start, view, grad_view)
     assert (np.abs(got - want) <= grad_bound(ref, want, start, x, token, 1.0, g)).all()
+
+
+def test_gradient_of_many_long_rows():
+    """Enough rows for the longer pieces; a few of them against the formula."""
+    torch = pytest.importorskip("torch")
+    rows, cols = 2500, 65533
+    torch.manual_seed(4)
+    x, dx = torch.randn(rows, cols, device="cuda"), torch.zeros(rows, cols, device="cuda")
+    rs = np.random.RandomState(4)
+    token, g = rs.randint(0, cols, rows).astype(np.int32), upstream(rs, rows)
+    torch.cuda.synchronize()
+    X = pb.Tensor.wrap_pointer(x.data_ptr(), [rows, cols], owner=x)
+    X.c.requires_grad = True
+    X.set_grad(pb.Tensor.wrap_pointer(dx.data_ptr(), [rows, cols], owner=dx))
+    lp, H, L, st = (pb.Tensor(s) for s in ((rows,), (rows,), (rows,), (rows, 2)))
+    T = pb.Tensor.from_numpy(token)
+    pb.token_logprob(X, T, lp, entropy=H, log_norm=L, stats=st)
+    for t, k in ((lp, "logprob"), (H, "entropy"), (L, "log_norm")):
+        t.set_grad(pb.Tensor.from_numpy(g[k]))
+    pb.token_logprob_backward(X, T, st, lp, entropy=H, log_norm=L)
+    pb.synchronize()
+    pick = np.r_[0, 1, 2, 1250, rows - 1]
+    xs, ts, gs = x[pick].cpu().numpy(), token[pick], {k: v[pick] for k, v in g.items()}
+    ref, start = R.token_logprob(xs, ts, 1.0), np.zeros((len(pick), cols), np.float32)
+    want = want_grad(ref, ts, 1.0, gs, start)
+    got = dx[pick].cpu().numpy()
+    assert (np.abs(got - want) <= grad_bound(ref, want, start, xs, ts, 1.0, gs)).all()
 
 
 def test_gradient_matches_differences():
@@ -340,13 +368,15 @@ def test_offsets_beyond_32_bits():
 
 
 @pytest.mark.parametrize("cols", [8192, 16387, 50001, 70000])
-@pytest.mark.parametrize("kind", ["random", "equal", "two_values", "ascending", "descending", "masked"])
+@pytest.mark.parametrize("kind", ["random", "equal", "two_values", "late_ties", "zeros", "ascending", "descending", "masked"])
 def test_many_long_rows(kind, cols):
     """More rows than resident CTAs: the persistent kernel, several rows per CTA, lists that overflow, empty rows."""
     rs = np.random.RandomState(cols)
     rows, i = 1300 if cols < 20000 else 620, np.arange(cols)
     x = {"random": lambda: rs.randn(rows, cols) * 3, "equal": lambda: np.broadcast_to(rs.randn(rows, 1), (rows, cols)),
          "two_values": lambda: np.broadcast_to((i * 7919 % 3 == 0) * 1.0, (rows, cols)),
+         "late_ties": lambda: np.broadcast_to((i >= cols - 700) * 1.0, (rows, cols)),
+         "zeros": lambda: np.broadcast_to(np.where(i % 3 == 1, -0.0, 0.0), (rows, cols)),
          "ascending": lambda: np.broadcast_to(i * 1e-3, (rows, cols)),
          "descending": lambda: np.broadcast_to(-i * 1e-3, (rows, cols)),
          "masked": lambda: np.where(rs.rand(rows, cols) < 0.999, -np.inf, rs.randn(rows, cols))}[kind]().astype(np.float32)
