@@ -12,7 +12,6 @@ There is no CPU fallback: if the library is missing or cannot be loaded, importi
 from __future__ import annotations
 
 import ctypes as C
-import functools
 import os
 from pathlib import Path
 
@@ -423,7 +422,7 @@ def forward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fva
             check: bool = True):
     """``<op>_cuda_forward(inputs, output, params)``; raises :class:`PlastError` on failure."""
     fn = _ENTRY.get(("forward", op)) or _entry("forward", op)
-    fn(_addresses(inputs), output.address, _params(dim, keepdim, fval))
+    fn(_addresses(inputs), output.address, KernelParams(dim, keepdim, fval))
     if check:
         check_error()
     return output
@@ -433,18 +432,13 @@ def backward(op: str, inputs, output: Tensor, dim: int = 0, keepdim: int = 0, fv
              check: bool = True):
     """``<op>_cuda_backward(inputs, output, params)``: accumulates into inputs[i].grad."""
     fn = _ENTRY.get(("backward", op)) or _entry("backward", op)
-    fn(_addresses(inputs), output.address, _params(dim, keepdim, fval))
+    fn(_addresses(inputs), output.address, KernelParams(dim, keepdim, fval))
     if check:
         check_error()
 
 
 def _at(t):
     return None if t is None else t.address
-
-
-@functools.lru_cache(maxsize=256)
-def _params(dim, keepdim, fval):
-    return KernelParams(dim, keepdim, fval)
 
 
 def token_logprob(logits, tokens, logprob, entropy=None, log_norm=None, stats=None, top_logprob=None, top_index=None,
