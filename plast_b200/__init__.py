@@ -131,16 +131,15 @@ def _load() -> C.CDLL:
             f"{LIB_PATH} is missing: build it with `python -m plast_b200.build` "
             "(there is no CPU fallback for the CUDA path)")
     lib = C.CDLL(str(LIB_PATH))
-    # addresses: any array of Tensor pointers or of their addresses (see _addresses), a Tensor's byref or address
     for op in FORWARD_OPS:
         fn = getattr(lib, f"{op}_cuda_forward")
-        fn.argtypes = [C.c_void_p, C.c_void_p, KernelParams]
+        fn.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(CTensor), KernelParams]
         fn.restype = None
     for op in BACKWARD_OPS:
         fn = getattr(lib, f"{op}_cuda_backward")
-        fn.argtypes = [C.c_void_p, C.c_void_p, KernelParams]
+        fn.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(CTensor), KernelParams]
         fn.restype = None
-    lib.sum_axis0_noalloc_cuda_forward.argtypes = [C.c_void_p, C.c_void_p, KernelParams]
+    lib.sum_axis0_noalloc_cuda_forward.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(CTensor), KernelParams]
     lib.sum_axis0_noalloc_cuda_forward.restype = None
     lib.plast_b200_chain_forward.argtypes = [C.POINTER(C.POINTER(CTensor)), C.c_int, C.POINTER(CTensor),
                                              C.POINTER(ChainStep), C.c_int]
@@ -153,10 +152,10 @@ def _load() -> C.CDLL:
     lib.plast_b200_chain_forward_host.restype = None
     lib.plast_b200_add_leaky_relu_row_sum.argtypes = [C.POINTER(CTensor)] * 4 + [C.c_float]
     lib.plast_b200_add_leaky_relu_row_sum.restype = None
-    lib.plast_b200_token_logprob.argtypes = [C.c_void_p] * 8 + [C.c_float]
-    lib.plast_b200_token_logprob_backward.argtypes = [C.c_void_p] * 6 + [C.c_float]
-    lib.plast_b200_qk_norm_rotary.argtypes = [C.c_void_p] * 8 + [QkNormParams]
-    lib.plast_b200_qk_norm_rotary_backward.argtypes = [C.c_void_p] * 8 + [QkNormParams]
+    lib.plast_b200_token_logprob.argtypes = [C.POINTER(CTensor)] * 8 + [C.c_float]
+    lib.plast_b200_token_logprob_backward.argtypes = [C.POINTER(CTensor)] * 6 + [C.c_float]
+    lib.plast_b200_qk_norm_rotary.argtypes = [C.POINTER(CTensor)] * 8 + [QkNormParams]
+    lib.plast_b200_qk_norm_rotary_backward.argtypes = [C.POINTER(CTensor)] * 8 + [QkNormParams]
     lib.plast_b200_rotary_frequencies.argtypes = [C.POINTER(RotaryScaling), C.c_uint64, C.c_float, C.POINTER(C.c_float),
                                                   C.POINTER(C.c_float)]
     lib.plast_b200_rotary_frequencies.restype = C.c_int
@@ -410,11 +409,25 @@ def check_error():
         raise PlastError(code, lib.plast_b200_last_error_message().decode())
 
 
-_ENTRY = {}                                          # (direction, op) -> the entry point, looked up once
+def _by_address(name: str, *argtypes):
+    """A handle on an entry point for the calls of this package, whose addresses are those of Tensor objects. The
+    handle of that name in `lib` is for everybody else and checks the types of its pointers."""
+    typed = getattr(lib, name)
+    fn = _LazyLib._lib[name]
+    fn.argtypes, fn.restype = argtypes, typed.restype
+    return fn
+
+
+_ENTRY = {}                                          # (direction, op) or name -> the handle, looked up once
 
 
 def _entry(direction: str, op: str):
-    fn = _ENTRY[direction, op] = getattr(lib, f"{op}_cuda_{direction}")
+    fn = _ENTRY[direction, op] = _by_address(f"{op}_cuda_{direction}", C.c_void_p, C.c_void_p, KernelParams)
+    return fn
+
+
+def _tensors_entry(name: str, tensors: int, params):
+    fn = _ENTRY[name] = _by_address(name, *[C.c_void_p] * tensors, params)
     return fn
 
 
@@ -446,8 +459,9 @@ def token_logprob(logits, tokens, logprob, entropy=None, log_norm=None, stats=No
     """Log probability of one given token per row of logits [..., C], with the distribution's entropy and log
     normaliser, the statistics that the backward needs ([..., 2]) and the k = top_index.shape[-1] best
     alternatives; optional outputs may be None."""
-    lib.plast_b200_token_logprob(_at(logits), _at(tokens), _at(logprob), _at(entropy), _at(log_norm), _at(stats),
-                                 _at(top_logprob), _at(top_index), temperature)
+    fn = _ENTRY.get("plast_b200_token_logprob") or _tensors_entry("plast_b200_token_logprob", 8, C.c_float)
+    fn(_at(logits), _at(tokens), _at(logprob), _at(entropy), _at(log_norm), _at(stats), _at(top_logprob), _at(top_index),
+       temperature)
     if check:
         check_error()
     return logprob
@@ -456,8 +470,8 @@ def token_logprob(logits, tokens, logprob, entropy=None, log_norm=None, stats=No
 def token_logprob_backward(logits, tokens, stats, logprob=None, entropy=None, log_norm=None, temperature: float = 1.0,
                            check: bool = True):
     """logits.grad += the gradient of the upstream gradients in logprob.grad, entropy.grad and log_norm.grad."""
-    lib.plast_b200_token_logprob_backward(_at(logits), _at(tokens), _at(stats), _at(logprob), _at(entropy),
-                                          _at(log_norm), temperature)
+    fn = _ENTRY.get("plast_b200_token_logprob_backward") or _tensors_entry("plast_b200_token_logprob_backward", 6, C.c_float)
+    fn(_at(logits), _at(tokens), _at(stats), _at(logprob), _at(entropy), _at(log_norm), temperature)
     if check:
         check_error()
 
@@ -479,8 +493,9 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, 
                    layout: int = ROTARY_HALVES, amplitude: float = 1.0, check: bool = True):
     """Root-mean-square norm of every query and key head, its weight and the rotation, in one launch. k, k_weight
     and k_out may be None together, a weight alone too."""
-    lib.plast_b200_qk_norm_rotary(_at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions), _at(inv_freq),
-                                  _at(q_out), _at(k_out), QkNormParams(epsilon, amplitude, layout))
+    fn = _ENTRY.get("plast_b200_qk_norm_rotary") or _tensors_entry("plast_b200_qk_norm_rotary", 8, QkNormParams)
+    fn(_at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions), _at(inv_freq), _at(q_out), _at(k_out),
+       QkNormParams(epsilon, amplitude, layout))
     if check:
         check_error()
     return q_out, k_out
@@ -489,9 +504,9 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, 
 def qk_norm_rotary_backward(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, epsilon: float = 1e-6,
                             layout: int = ROTARY_HALVES, amplitude: float = 1.0, check: bool = True):
     """Adds to q.grad, k.grad and the weights' gradients, reading q_out.grad and k_out.grad."""
-    lib.plast_b200_qk_norm_rotary_backward(_at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions),
-                                           _at(inv_freq), _at(q_out), _at(k_out),
-                                           QkNormParams(epsilon, amplitude, layout))
+    fn = _ENTRY.get("plast_b200_qk_norm_rotary_backward") or _tensors_entry("plast_b200_qk_norm_rotary_backward", 8, QkNormParams)
+    fn(_at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions), _at(inv_freq), _at(q_out), _at(k_out),
+       QkNormParams(epsilon, amplitude, layout))
     if check:
         check_error()
 

@@ -54,7 +54,7 @@ lib.plast_b200_fusion_release.restype = None
 lib.plast_b200_fusion_program.argtypes = [C.c_uint64, C.POINTER(ChainStep), C.c_int, C.POINTER(C.c_int)]
 lib.plast_b200_fusion_program.restype = C.c_int
 for _name in ("chain_cuda_forward", "chain_cuda_backward"):
-    getattr(lib, _name).argtypes = [C.c_void_p, C.c_void_p, KernelParams]
+    getattr(lib, _name).argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(CTensor), KernelParams]
     getattr(lib, _name).restype = None
 
 

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 
-from . import CTensor, check_error, lib
+from . import CTensor, _by_address, check_error, lib
 
 
 class SGD(C.Structure):
@@ -52,14 +52,19 @@ assert C.sizeof(SGD) == 4 and C.sizeof(Adam) == 56 and C.sizeof(AdamW) == 56
 assert Adam.t.offset == 16 and Adam.m.offset == 24 and AdamW.t.offset == 20 and AdamW.m.offset == 24
 
 for _name, _struct in (("sgd_step_cuda", SGD), ("adam_step_cuda", Adam), ("adamw_step_cuda", AdamW), ("muon_step_cuda", Muon)):
-    getattr(lib, _name).argtypes = [C.POINTER(_struct), C.c_void_p, C.c_int]   # any array of Tensor pointers or addresses
+    getattr(lib, _name).argtypes = [C.POINTER(_struct), C.POINTER(C.POINTER(CTensor)), C.c_int]
     getattr(lib, _name).restype = None
 lib.plast_b200_adam_state_release.argtypes = [C.POINTER(C.POINTER(CTensor)), C.POINTER(C.POINTER(CTensor))]
 lib.plast_b200_adam_state_release.restype = None
 lib.plast_b200_muon_state_release.argtypes = [C.POINTER(C.POINTER(CTensor))]
 lib.plast_b200_muon_state_release.restype = None
-lib.plast_b200_orthogonalise.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_float]
+lib.plast_b200_orthogonalise.argtypes = [C.POINTER(C.POINTER(CTensor))] * 2 + [C.c_int, C.c_int, C.c_float]
 lib.plast_b200_orthogonalise.restype = None
+
+# by the addresses of _address_array
+_STEP = {_struct: _by_address(_name, C.POINTER(_struct), C.c_void_p, C.c_int)
+         for _name, _struct in (("sgd_step_cuda", SGD), ("adam_step_cuda", Adam), ("adamw_step_cuda", AdamW), ("muon_step_cuda", Muon))}
+_orthogonalise = _by_address("plast_b200_orthogonalise", C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_float)
 
 
 def param_array(params):
@@ -78,9 +83,7 @@ def _address_array(params):
 
 def step(optimizer, params) -> None:
     """One optimiser step on the GPU over a list of parameters (Tensor objects with .grad)."""
-    fn = {SGD: lib.sgd_step_cuda, Adam: lib.adam_step_cuda, AdamW: lib.adamw_step_cuda,
-          Muon: lib.muon_step_cuda}[type(optimizer)]
-    fn(C.byref(optimizer), _address_array(params), len(params))
+    _STEP[type(optimizer)](C.byref(optimizer), _address_array(params), len(params))
     check_error()
 
 
@@ -88,7 +91,7 @@ def orthogonalise(inputs, outputs, steps: int = 5, epsilon: float = 1e-7) -> Non
     """outputs[i] = the Newton-Schulz orthogonalisation of inputs[i], all matrices at once."""
     if len(inputs) != len(outputs):
         raise ValueError("as many outputs as inputs")
-    lib.plast_b200_orthogonalise(_address_array(inputs), _address_array(outputs), len(inputs), steps, epsilon)
+    _orthogonalise(_address_array(inputs), _address_array(outputs), len(inputs), steps, epsilon)
     check_error()
 
 

@@ -40,3 +40,43 @@ def test_a_scalar_that_changes_is_read_at_every_call(given, call):
     del given[:]
     call("leaky_relu", [x], y, dim=pb.FULL_REDUCE, keepdim=True, fval=1, check=False)
     assert given == [(pb.FULL_REDUCE, 1, 1.0)]
+
+
+TENSORS, TENSOR = pb.C.POINTER(pb.C.POINTER(pb.CTensor)), pb.C.POINTER(pb.CTensor)
+
+
+def takes(name):
+    from plast_b200 import graph, optim  # noqa: F401  (they declare entry points of their own)
+    return getattr(pb.lib, name).argtypes
+
+
+@pytest.mark.parametrize("name,wanted", [
+    *[(f"{op}_cuda_forward", [TENSORS, TENSOR]) for op in pb.FORWARD_OPS + ["chain", "sum_axis0_noalloc"]],
+    *[(f"{op}_cuda_backward", [TENSORS, TENSOR]) for op in pb.BACKWARD_OPS + ["chain"]],
+    *[(f"{kind}_step_cuda", [None, TENSORS]) for kind in ("sgd", "adam", "adamw", "muon")],
+    ("plast_b200_orthogonalise", [TENSORS, TENSORS]), ("plast_b200_token_logprob", [TENSOR] * 8),
+    ("plast_b200_token_logprob_backward", [TENSOR] * 6), ("plast_b200_qk_norm_rotary", [TENSOR] * 8),
+    ("plast_b200_qk_norm_rotary_backward", [TENSOR] * 8)])
+def test_entry_points_refuse_what_is_no_tensor_pointer(name, wanted):
+    """By their declared types (a call with a wrong one must not be made): a number, bytes, an untyped address, one
+    level of pointers too few or too many."""
+    t = pb.Tensor((2,), device="cpu")
+    one, many = pb.C.byref(t.c), pb._ptr_array([t, t])
+    for declared, kind in zip(takes(name), wanted):
+        if kind is None:
+            continue
+        declared.from_param(many if kind is TENSORS else one)
+        for wrong in (5, b"bytes", pb.C.c_void_p(8), one if kind is TENSORS else many, t):
+            with pytest.raises(TypeError):
+                declared.from_param(wrong)
+
+
+def test_the_layer_takes_tensors_only():
+    from plast_b200 import optim
+    x, row = pb.Tensor((2, 3), device="cpu"), pb.Tensor((2,), device="cpu")
+    for wrong in (5, b"bytes", np.zeros(3, np.float32), pb.C.byref(x.c)):
+        for call in (lambda: pb.forward("neg", [wrong], x), lambda: pb.forward("neg", [x], wrong),
+                     lambda: pb.backward("neg", [wrong], x), lambda: pb.token_logprob(wrong, row, row),
+                     lambda: optim.step(optim.SGD(0.1), [wrong]), lambda: optim.orthogonalise([wrong], [x])):
+            with pytest.raises((AttributeError, TypeError)):
+                call()
