@@ -401,7 +401,10 @@ __device__ __forceinline__ void load_operand(const NsOperand &o, uint32_t dst, u
 }
 
 struct NsShared {
-  uint64_t full[kNsStages], peer_full[kNsStages], empty[kNsStages], acc_full[2], acc_empty[2], drained;
+  // A wait knows a turn of a barrier by its parity alone: it must not begin before the turn before is over, nor be left
+  // behind by two. So every barrier has waiters that wait for each of its turns: `full` is of operands (the issuing
+  // warp), `linear_full` of linear terms (by their part, which the same draining warps read each time, and stage).
+  uint64_t full[kNsStages], peer_full[kNsStages], empty[kNsStages], linear_full[2][kNsStages], acc_full[2], acc_empty[2], drained;
   NsTable table; // a copy: the roles index it at every tile, which is slow in constant memory
   uint32_t tmem;
   volatile unsigned gave_up;
@@ -421,7 +424,8 @@ struct NsRing {
   uint32_t stages;      // shared memory
   unsigned rank;        // in the pair
   unsigned first;       // this CTA's (pair's) first tile of the product at hand
-  unsigned stage, phase; // of the next stage
+  unsigned stage, phase; // of the next stage; the phase is that of its `empty`
+  unsigned turns;       // by stage, a bit: the parity of the next turn of its `full` or `linear_full` for this role
   unsigned buf, turn;   // of the next accumulator
   unsigned tiles;       // so far
   __device__ __forceinline__ void skip_stages(unsigned n) {
@@ -434,6 +438,12 @@ struct NsRing {
       stage = 0;
       phase ^= 1;
     }
+  }
+  // parity of the turn that is waited for (once)
+  __device__ __forceinline__ unsigned take_turn(unsigned at) {
+    const unsigned parity = (turns >> at) & 1;
+    turns ^= 1u << at;
+    return parity;
   }
   __device__ __forceinline__ void next_accumulator() {
     buf ^= 1;
@@ -511,12 +521,13 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
         const unsigned cb0 = narrow ? at.j : at.j * 2 * CTAS, cb_end = cb0 + (narrow ? 1 : 2 * CTAS);
         for (unsigned c = 0; c < CTAS; ++c, ring.next_stage()) {
           if (!barrier_wait(smem_address(&sh.empty[ring.stage]), ring.phase ^ 1, &sh.gave_up)) return false;
-          const uint32_t bar = smem_address(&sh.full[ring.stage]), dst = ring.stages + ring.stage * kNsStageBytes;
+          const uint32_t bar = smem_address(&sh.linear_full[c][ring.stage]), dst = ring.stages + ring.stage * kNsStageBytes;
           const unsigned first = cb0 + 2 * c;
           unsigned n = 0; // block columns that exist
           if (rb < rows)
             while (n < 2 && first + n < cb_end && first + n < cbs) ++n;
           barrier_expect(bar, n * 2 * kPanelHalf);
+          ring.turns ^= 1u << (kNsStages * (1 + c) + ring.stage);
           if (n) bulk_load(dst, old + panel_block(rb, first, cbs), n * 2 * kPanelHalf, bar); // neighbours in memory
         }
       }
@@ -526,6 +537,7 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
       const unsigned kb = at.k0 + k;
       const bool fl = kb < flip_left, fr = kb < flip_right;
       barrier_expect(bar, (fl ? left.flip_bytes : left.plain_bytes) + (fr ? right.flip_bytes : right.plain_bytes));
+      ring.turns ^= 1u << ring.stage;
       load_operand(left, dst, kb, fl, bar);
       load_operand(right, dst + 2 * kPanelHalf, kb, fr, bar);
       ring.next_stage();
@@ -564,19 +576,11 @@ __device__ bool ns_multiply(NsShared &sh, NsRing &ring, int what) {
     const unsigned flip_right = what == kGram ? 0 : what == kApply ? ~0u : 2 * CTAS * (narrow ? at.j / 2 : at.j);
     const unsigned k_linear = ns_linear_after<CTAS>(at, what);
     for (unsigned k = 0; k <= at.k_blocks; ++k, ring.next_stage()) {
-      if (k == k_linear) {
-        // not for the tensor cores; but the second CTA's messages count every turn of the ring
-        if (CTAS > 1 && ring.rank != 0) {
-          for (int c = 0; c < CTAS; ++c, ring.next_stage()) {
-            if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.full[ring.stage]), ring.phase, &sh.gave_up))) return false;
-            if (elect_one()) barrier_arrive_at(smem_address(&sh.peer_full[ring.stage]), 0);
-            __syncwarp();
-          }
-        } else ring.skip_stages(CTAS);
-      }
+      if (k == k_linear) ring.skip_stages(CTAS); // not for the tensor cores
       if (k == at.k_blocks) break;
       const uint32_t full = smem_address(&sh.full[ring.stage]);
-      if (!__all_sync(0xffffffffu, barrier_wait(full, ring.phase, &sh.gave_up))) return false;
+      const unsigned parity = ring.take_turn(ring.stage);
+      if (!__all_sync(0xffffffffu, barrier_wait(full, parity, &sh.gave_up))) return false;
       if (CTAS > 1 && ring.rank != 0) {
         if (elect_one()) barrier_arrive_at(smem_address(&sh.peer_full[ring.stage]), 0);
         __syncwarp();
@@ -585,7 +589,7 @@ __device__ bool ns_multiply(NsShared &sh, NsRing &ring, int what) {
       const bool first = k % kNsChunk<CTAS> == 0, last = k % kNsChunk<CTAS> == kNsChunk<CTAS> - 1 || k + 1 == at.k_blocks;
       if (first && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_empty[ring.buf]), ring.turn ^ 1, &sh.gave_up)))
         return false;
-      if (CTAS > 1 && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.peer_full[ring.stage]), ring.phase, &sh.gave_up)))
+      if (CTAS > 1 && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.peer_full[ring.stage]), parity, &sh.gave_up)))
         return false;
       tmem_fence_after();
       const bool fl = at.k0 + k < flip_left, fr = at.k0 + k < flip_right;
@@ -628,6 +632,7 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
   const unsigned row_in_tile = (warp & 3) * 32 + lane;
   const bool narrow = CTAS == 1 && t.narrow[what];
   const unsigned columns = narrow ? 16 : 32 * CTAS;
+  const unsigned part_of_linear = CTAS > 1 ? quarter / 2 : 0; // whose stage holds the warp's columns
   const float init = (float)(what == kPolynomial ? kNsLinear / kNsC : (double)kNsA - kNsS) * kSplitScale;
   const float diagonal = (float)(what == kGram ? -kNsT : what == kPolynomial ? kNsLinear * kNsT - kNsC * kNsT * kNsT + kNsS : 0.0) * kSplitScale;
   const float finish = what == kPolynomial ? kNsC * kSplitUnscale : kSplitUnscale;
@@ -650,8 +655,10 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
       if (k_linear != ~0u && c == (k_linear + kNsChunk<CTAS> - 1) / kNsChunk<CTAS>) {
         // the lane's row of the linear term, from the stage that holds the warp's block column
         NsRing here = ring;
-        here.skip_stages(k_linear + (CTAS > 1 ? quarter / 2 : 0));
-        if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.full[here.stage]), here.phase, &sh.gave_up))) return false;
+        here.skip_stages(k_linear + part_of_linear);
+        if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.linear_full[part_of_linear][here.stage]), ring.take_turn(here.stage),
+                                                  &sh.gave_up)))
+          return false;
         const unsigned block = CTAS > 1 ? (quarter & 1) : narrow ? 0 : quarter / 2;
         const unsigned chunk0 = CTAS > 1 ? 0 : narrow ? quarter * 2 : (quarter & 1) * 4;
         const char *old = dynamic_stage(ring.stages, here.stage) + block * (2 * kPanelHalf);
@@ -676,8 +683,8 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
         __syncwarp();
         if (lane == 0) {
           __threadfence_block();
-          const unsigned mine = CTAS > 1 ? quarter / 2 : 0, share = kNsEpilogueWarps / CTAS;
-          if (atomicAdd(&sh.linear_read[mine], 1u) % share == share - 1) barrier_arrive(smem_address(&sh.empty[here.stage]));
+          const unsigned share = kNsEpilogueWarps / CTAS;
+          if (atomicAdd(&sh.linear_read[part_of_linear], 1u) % share == share - 1) barrier_arrive(smem_address(&sh.empty[here.stage]));
         }
       }
       if (c == rounds) break;
@@ -862,12 +869,13 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
   const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (unsigned i = threadIdx.x; i < sizeof(NsTable) / 4; i += kNsThreads)
     reinterpret_cast<unsigned *>(&sh.table)[i] = reinterpret_cast<const unsigned *>(&param)[i];
-  NsRing ring = {smem_address(dynamic_smem), CTAS == 1 ? 0 : blockIdx.x % CTAS, 0, 0, 0, 0, 0, 0};
+  NsRing ring = {smem_address(dynamic_smem), CTAS == 1 ? 0 : blockIdx.x % CTAS, 0, 0, 0, 0, 0, 0, 0};
   if (threadIdx.x == 0) {
     for (int s = 0; s < kNsStages; ++s) {
       barrier_init(smem_address(&sh.full[s]), 1);
       barrier_init(smem_address(&sh.peer_full[s]), 1);
       barrier_init(smem_address(&sh.empty[s]), 1);
+      for (int c = 0; c < 2; ++c) barrier_init(smem_address(&sh.linear_full[c][s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
       barrier_init(smem_address(&sh.acc_full[b]), 1);
@@ -907,10 +915,9 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
   if (!ok && lane == 0) { // after a wait that ran out: what is in flight ends before its memory goes away
     const long long start = clock64();
     if (warp == kNsEpilogueWarps)
-      for (int st = 0; st < kNsStages; ++st) {
-        // the phase of this stage's last copy: the current one where the ring has passed it
-        const unsigned phase = (unsigned)st < ring.stage ? ring.phase : ring.phase ^ 1;
-        while (!barrier_try(smem_address(&sh.full[st]), phase) && clock64() - start < 10000000) {}
+      for (int i = 0; i < 3 * kNsStages; ++i) { // the last copy of each barrier
+        const uint32_t bar = i < kNsStages ? smem_address(&sh.full[i]) : smem_address(&sh.linear_full[i / kNsStages - 1][i % kNsStages]);
+        while (!barrier_try(bar, ((ring.turns >> i) & 1) ^ 1) && clock64() - start < 10000000) {}
       }
     if (warp == kNsEpilogueWarps + 1 && ring.rank == 0) {
       mma_commit<CTAS>(smem_address(&sh.drained));

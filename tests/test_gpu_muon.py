@@ -364,3 +364,25 @@ def test_one_training_step_of_a_small_language_model():
         want = w - 0.02 * np.sqrt(max(1.0, r / c)) * o
         # the gradient has at most 12 directions of T tokens: fewer than min(r, c), so compare where the values are lifted
         assert np.linalg.norm(p.numpy() - want) <= 0.03 * np.linalg.norm(o) * tolerance(1) + 4 * U * np.linalg.norm(w)
+
+
+def same_bits_and_right(xs, times):
+    """Against 64 bits, and the same bits from `times` calls."""
+    ins, outs = [pb.Tensor.from_numpy(x) for x in xs], [pb.Tensor(x.shape) for x in xs]
+    O.orthogonalise(ins, outs)
+    first = [o.numpy() for o in outs]
+    for x, got in zip(xs, first):
+        assert rel(got, R.orthogonalise(x)) <= tolerance(min(x.shape)), x.shape
+    for _ in range(times):
+        for o in outs:
+            o.zero_()
+        O.orthogonalise(ins, outs)
+        for o, want in zip(outs, first):
+            assert np.array_equal(o.numpy(), want), want.shape
+
+
+@pytest.mark.parametrize("shape", [(64, 32768), (32768, 40), (128, 20001), (250, 12000)])
+def test_many_tiles_of_few_k_blocks_in_a_cta(shape):
+    """A tile of one or two K blocks and its linear term fill the ring of stages once or not at all: terms and operands
+    take turns on the same stage from one tile to the next."""
+    same_bits_and_right([np.random.RandomState(shape[1]).randn(*shape).astype(np.float32)], 10)
