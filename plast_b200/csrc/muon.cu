@@ -410,7 +410,7 @@ struct NsShared {
   volatile unsigned gave_up;
   volatile unsigned allowed; // tiles whose operands are stored, as the looking-out thread has seen
   unsigned written;     // draining warps that have written their part of a tile, over all tiles
-  unsigned linear_read[2]; // draining warps that have read their part of a linear term's stage, over all tiles
+  unsigned linear_read[kNsStages]; // draining warps that have read a linear term in this stage, over all tiles
 };
 constexpr unsigned kNsSmem = kNsStages * kNsStageBytes + kNsEpilogueWarps * kNsPieceBytes + sizeof(NsShared);
 static_assert(kNsSmem <= 232448, "227 KB of shared memory per CTA");
@@ -679,12 +679,16 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
               }
             }
         }
-        // the last of the warps that share the stage gives it back
+        // the last of the warps that share the stage gives it back (counted by stage: warps that are ahead read the
+        // next tile's term in another one, and none in this one before it is given back)
         __syncwarp();
         if (lane == 0) {
           __threadfence_block();
           const unsigned share = kNsEpilogueWarps / CTAS;
-          if (atomicAdd(&sh.linear_read[part_of_linear], 1u) % share == share - 1) barrier_arrive(smem_address(&sh.empty[here.stage]));
+          if (atomicAdd(&sh.linear_read[here.stage], 1u) % share == share - 1) {
+            __threadfence_block();
+            barrier_arrive(smem_address(&sh.empty[here.stage]));
+          }
         }
       }
       if (c == rounds) break;
@@ -882,7 +886,8 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
       barrier_init(smem_address(&sh.acc_empty[b]), kNsEpilogueWarps * CTAS);
     }
     barrier_init(smem_address(&sh.drained), 1);
-    sh.gave_up = sh.allowed = sh.written = sh.linear_read[0] = sh.linear_read[1] = 0;
+    sh.gave_up = sh.allowed = sh.written = 0;
+    for (int s = 0; s < kNsStages; ++s) sh.linear_read[s] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();

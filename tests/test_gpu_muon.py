@@ -386,3 +386,11 @@ def test_many_tiles_of_few_k_blocks_in_a_cta(shape):
     """A tile of one or two K blocks and its linear term fill the ring of stages once or not at all: terms and operands
     take turns on the same stage from one tile to the next."""
     same_bits_and_right([np.random.RandomState(shape[1]).randn(*shape).astype(np.float32)], 10)
+
+
+@pytest.mark.parametrize("shapes", [[(64, 4672)] * 32, [(64, 4672), (33, 4650), (128, 4700)] * 10])
+def test_warps_of_a_cta_on_different_tiles(shapes):
+    """Tiles of one K block from many matrices: some of the warps that read a tile's linear term are a tile ahead of
+    the others, those that have nothing to store among them."""
+    rs = np.random.RandomState(len(shapes[0]))
+    same_bits_and_right([rs.randn(*s).astype(np.float32) for s in shapes], 10)
