@@ -39,7 +39,7 @@ struct MuonMat {
   const float *g;  // gradient, or the input of orthogonalise
   float *v;        // momentum; NULL: u = g
   float *w;        // weight (w = w * keep - rate * X) or, with keep == 0 and rate == -1, the output
-  char *x[2], *a, *b; // panels: X (two, in turn), A, B
+  char *x[2], *a; // panels: X (two, in turn), A, B behind A
   double *partial; // sums of squares of the momentum pass, then partial[0] holds their total
   float keep, rate;
   unsigned rows, cols; // as stored
@@ -261,13 +261,14 @@ constexpr unsigned kNsMostParts = 8;   // of a split K
 constexpr unsigned kNsPieceBytes = 2048; // per draining warp: 32 rows of 32 columns of hi or lo, or 32 x 16 floats
 
 struct NsMat {
-  char *x[2], *a, *b;
+  char *x[2], *a; // B lies behind A
   float *w;
   float keep, rate;
   unsigned m, n;
   unsigned first_tile[3], tiles[3]; // a tile whose K is split counts once for each part
   unsigned char splits[3];
   bool turned; // stored as n x m
+  __device__ __forceinline__ char *b() const { return a + panel_block(panel_row_blocks(m), 0, panel_col_blocks(m)); }
 };
 struct NsTable {
   NsMat mat[kMuonMax];
@@ -409,7 +410,7 @@ struct NsShared {
   uint32_t tmem;
   volatile unsigned gave_up;
   volatile unsigned allowed; // tiles whose operands are stored, as the looking-out thread has seen
-  unsigned written;     // draining warps that have written their part of a tile, over all tiles
+  alignas(16) unsigned written[kNsEpilogueWarps]; // per draining warp: tiles that it has written its part of
   unsigned linear_read[kNsStages]; // draining warps that have read a linear term in this stage, over all tiles
 };
 constexpr unsigned kNsSmem = kNsStages * kNsStageBytes + kNsEpilogueWarps * kNsPieceBytes + sizeof(NsShared);
@@ -427,7 +428,7 @@ struct NsRing {
   unsigned stage, phase; // of the next stage; the phase is that of its `empty`
   unsigned turns;       // by stage, a bit: the parity of the next turn of its `full` or `linear_full` for this role
   unsigned buf, turn;   // of the next accumulator
-  unsigned tiles;       // so far
+  unsigned tiles;       // so far, for the roles that count them
   __device__ __forceinline__ void skip_stages(unsigned n) {
     stage += n;
     phase ^= (stage / kNsStages) & 1;
@@ -489,6 +490,32 @@ __device__ __noinline__ bool ns_wait_counter(const volatile unsigned *counter, u
   return true;
 }
 
+// Until every draining warp has written its part of `target` tiles. (One count for all of them would not tell: a warp
+// may be two tiles ahead of another, as far as the two accumulators go.)
+__device__ __noinline__ bool ns_wait_written(const unsigned *written, unsigned target, volatile unsigned *gave_up) {
+  const uint32_t at = smem_address(written);
+  const long long start = clock64();
+  for (unsigned spins = 0;; ++spins) {
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < kNsEpilogueWarps / 4; ++i) {
+      uint4 v;
+      asm volatile("ld.volatile.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at + 16 * i) : "memory");
+      all = all && v.x >= target && v.y >= target && v.z >= target && v.w >= target;
+    }
+    if (all) break;
+    if ((spins & 63) == 63) {
+      if (*gave_up) return false;
+      if (clock64() - start > kWaitCycles) {
+        *gave_up = 1;
+        return false;
+      }
+    }
+  }
+  __threadfence_block();
+  return true;
+}
+
 // The roles below take the product as an argument, not as a template: three copies of each do not fit
 // the instruction cache, and a tile of a small matrix runs its code once (measured with three copies,
 // 180 KB: 2,400 cycles to store a tile of 128 x 64, all of it fetching instructions).
@@ -503,7 +530,7 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
     NsTile at;
     const NsMat &q = tile_at<CTAS>(t, what, tile, at);
     const unsigned rows = panel_row_blocks(q.m), xcb = panel_col_blocks(q.n), mcb = panel_col_blocks(q.m);
-    const NsOperand left = operand_of(what == kGram ? q.x[from] : what == kPolynomial ? q.a : q.b, at.i * CTAS + ring.rank, rows,
+    const NsOperand left = operand_of(what == kGram ? q.x[from] : what == kPolynomial ? q.a : q.b(), at.i * CTAS + ring.rank, rows,
                                       what == kGram ? xcb : mcb, false);
     const NsOperand right = operand_of(what == kPolynomial ? q.a : q.x[from], at.j * CTAS + ring.rank, rows,
                                        what == kPolynomial ? mcb : xcb, narrow);
@@ -754,7 +781,7 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
     }
     if (rows_exist && mine) {
       if (what != kApply || !last) {
-        char *out = what == kGram ? q.a : what == kPolynomial ? q.b : q.x[(s & 1) ^ 1];
+        char *out = what == kGram ? q.a : what == kPolynomial ? q.b() : q.x[(s & 1) ^ 1];
         if (rb * 128 + 128 > q.m && row >= q.m) {
           // padding stays zero (an operand read from beyond the panel may leave anything in the sums)
 #pragma unroll
@@ -845,7 +872,7 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
         if (mine) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(t.stored + (&q - t.mat)) : "memory");
       }
       __threadfence_block();
-      atomicAdd(&sh.written, 1u);
+      *(volatile unsigned *)&sh.written[warp] = ++ring.tiles;
     }
   }
   return true;
@@ -859,7 +886,7 @@ __device__ bool ns_publish(NsShared &sh, NsRing &ring, int what) {
   for (unsigned tile = ring.first; tile < t.tiles[what]; tile += gridDim.x / CTAS) {
     NsTile at;
     const NsMat &q = tile_at<CTAS>(t, what, tile, at);
-    if (!ns_wait_counter(&sh.written, ++ring.tiles * kNsEpilogueWarps, &sh.gave_up)) return false;
+    if (!ns_wait_written(sh.written, ++ring.tiles, &sh.gave_up)) return false;
     if (at.parts == 1)
       asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(t.stored + (&q - t.mat)), "n"(kNsEpilogueWarps) : "memory");
   }
@@ -886,7 +913,8 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
       barrier_init(smem_address(&sh.acc_empty[b]), kNsEpilogueWarps * CTAS);
     }
     barrier_init(smem_address(&sh.drained), 1);
-    sh.gave_up = sh.allowed = sh.written = 0;
+    sh.gave_up = sh.allowed = 0;
+    for (int w = 0; w < kNsEpilogueWarps; ++w) sh.written[w] = 0;
     for (int s = 0; s < kNsStages; ++s) sh.linear_read[s] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -1047,7 +1075,6 @@ static NsTable steps_table(const MuonTable &mt) {
     d.x[0] = q.x[0];
     d.x[1] = q.x[1];
     d.a = q.a;
-    d.b = q.b;
     d.w = q.w;
     d.keep = q.keep;
     d.rate = q.rate;
@@ -1117,7 +1144,7 @@ static void run_group(MuonTable &t, char *base, int steps) {
     q.x[0] = take(panel_bytes(q.m, q.n));
     q.x[1] = take(panel_bytes(q.m, q.n));
     q.a = take(panel_bytes(q.m, q.m));
-    q.b = take(panel_bytes(q.m, q.m));
+    take(panel_bytes(q.m, q.m)); // B
     q.partial = (double *)take(padded((u64)(q.chunks + 1) * 8));
   }
   t.stored = (unsigned *)take(256);

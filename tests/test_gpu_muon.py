@@ -394,3 +394,12 @@ def test_warps_of_a_cta_on_different_tiles(shapes):
     the others, those that have nothing to store among them."""
     rs = np.random.RandomState(len(shapes[0]))
     same_bits_and_right([rs.randn(*s).astype(np.float32) for s in shapes], 10)
+
+
+@pytest.mark.parametrize("shapes", [[(100, 1000 + 70 * i) for i in range(28)], [(128, 128), (40, 2100), (60, 61), (64, 700)] * 8,
+                                    [(200 + i, 290) for i in range(30)]])
+def test_warps_that_have_nothing_to_store_run_ahead(shapes):
+    """More tiles than CTAs, at ragged right edges, of matrices whose products follow each other closely: a tile may be
+    told of when every warp has stored its part of this very tile."""
+    rs = np.random.RandomState(len(shapes))
+    same_bits_and_right([rs.randn(*s).astype(np.float32) for s in shapes], 10)
