@@ -758,6 +758,7 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
         asm volatile("fence.acq_rel.gpu;" ::: "memory");
       }
       mine = __shfl_sync(0xffffffffu, before, 0) == at.parts - 1;
+      __syncwarp(); // what lane 0 has acquired is there for all lanes (a shuffle orders no memory)
       if (mine) {
 #pragma unroll
         for (int i = 0; i < 16 * kGroups; ++i) acc[i] = 0.0f;

@@ -403,3 +403,8 @@ def test_warps_that_have_nothing_to_store_run_ahead(shapes):
     told of when every warp has stored its part of this very tile."""
     rs = np.random.RandomState(len(shapes))
     same_bits_and_right([rs.randn(*s).astype(np.float32) for s in shapes], 10)
+
+
+def test_parts_of_a_split_k_are_added_in_one_order():
+    rs = np.random.RandomState(23)
+    same_bits_and_right([rs.randn(*s).astype(np.float32) for s in [(64, 9000), (120, 4000), (300, 3000)]], 20)
