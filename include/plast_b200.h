@@ -403,8 +403,9 @@ int plast_b200_chain_backward_try_compile(const PlastChainStep *steps, int n_ste
  * reduce combine through distributed shared memory instead of a ticket in global memory, 0 or 1 =
  * never, 11: 1 = the 3-D tile kernel for inputs turned along two different dims uses 32 x 16 x 16
  * tiles instead of 8 x 32 x 32, 12: the Newton-Schulz products by 0 = single CTAs, 1 = pairs of
- * CTAs); a negative value restores the built-in choice. Results do not
- * depend on the geometry beyond the order of additions. */
+ * CTAs, 13: the limit of a wait inside those products, in thousands of SM cycles); a negative value
+ * restores the built-in choice. Results do not depend on the geometry beyond the order of additions
+ * (a limit too short for a call leaves NaN in its results, see plast_b200_muon_status). */
 void plast_b200_tune(int key, long value);
 /* Test hook: runs the host-side iteration planner (drop size-1 dims, order by the strides of
  * argument `sort_arg`, merge dims every argument walks as one run) on caller-supplied metadata.

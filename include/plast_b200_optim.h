@@ -123,9 +123,10 @@ void plast_b200_muon_state_release(Tensor **m);
 void plast_b200_orthogonalise(const Tensor **inputs, Tensor **outputs, int count, int steps, float epsilon);
 
 /* Every wait inside the product kernels is limited to about two seconds. Where one runs out (which
- * takes a broken GPU or library) the results of that call and the following ones are NaN instead of
- * wrong, and this returns 1 once, after which they work again; 0 = all is well, -1 = a CUDA error.
- * Waits for the library stream. */
+ * takes a broken GPU or library) what the call could not compute of its results is NaN instead of
+ * wrong (the momenta of a step have moved), and this returns 1 once; later calls are not affected.
+ * 0 = all is well since the last look, -1 = a CUDA error. Waits for the library stream; a call on
+ * another stream of the device is told of when it has ended. */
 int plast_b200_muon_status(void);
 
 #ifdef __cplusplus

@@ -279,9 +279,10 @@ struct NsTable {
   unsigned tiles[3]; // of each product
   int narrow[3];     // tiles of 128 x 64 instead of 128 x 128
   int count;
+  long long wait_cycles; // limit of every wait
 };
 
-__device__ unsigned g_ns_gave_up; // a wait ran out: results are NaN from then on, see plast_b200_muon_status
+__device__ unsigned g_ns_gave_up; // CTAs in which a wait has run out, over all calls: see plast_b200_muon_status
 
 // tiles along a side, and of a product; `wide`: columns of a tile (256, 128 or 64)
 __host__ __device__ inline unsigned ns_along(unsigned size, unsigned tile) { return (size + tile - 1) / tile; }
@@ -408,7 +409,7 @@ struct NsShared {
   uint64_t full[kNsStages], peer_full[kNsStages], empty[kNsStages], linear_full[2][kNsStages], acc_full[2], acc_empty[2], drained;
   NsTable table; // a copy: the roles index it at every tile, which is slow in constant memory
   uint32_t tmem;
-  volatile unsigned gave_up;
+  WaitLimit wait;
   volatile unsigned allowed; // tiles whose operands are stored, as the looking-out thread has seen
   alignas(16) unsigned written[kNsEpilogueWarps]; // per draining warp: tiles that it has written its part of
   unsigned linear_read[kNsStages]; // draining warps that have read a linear term in this stage, over all tiles
@@ -454,7 +455,7 @@ struct NsRing {
 
 // Waits until matrix q's products up to this one (step s, product what) are stored.
 template <int CTAS>
-__device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, int s, int what, volatile unsigned *gave_up) {
+__device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, int s, int what, WaitLimit *wait) {
   unsigned target = 0;
   for (int w = 0; w < 3; ++w) target += q.tiles[w] / q.splits[w] * (s + (w < what));
   target *= CTAS * kNsEpilogueWarps;
@@ -465,34 +466,22 @@ __device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, in
     asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(counter) : "memory");
     if (now >= target) return true;
     if (spins == 0) start = clock64();
-    if ((spins & 63) == 63) {
-      if (*gave_up) return false;
-      if (clock64() - start > kWaitCycles) {
-        *gave_up = 1;
-        return false;
-      }
-    }
+    if ((spins & 63) == 63 && wait->over(start)) return false;
   }
 }
 
 // The same for a counter in shared memory.
-__device__ __noinline__ bool ns_wait_counter(const volatile unsigned *counter, unsigned target, volatile unsigned *gave_up) {
+__device__ __noinline__ bool ns_wait_counter(const volatile unsigned *counter, unsigned target, WaitLimit *wait) {
   const long long start = clock64();
   for (unsigned spins = 0; *counter < target; ++spins)
-    if ((spins & 63) == 63) {
-      if (*gave_up) return false;
-      if (clock64() - start > kWaitCycles) {
-        *gave_up = 1;
-        return false;
-      }
-    }
+    if ((spins & 63) == 63 && wait->over(start)) return false;
   __threadfence_block();
   return true;
 }
 
 // Until every draining warp has written its part of `target` tiles. (One count for all of them would not tell: a warp
 // may be two tiles ahead of another, as far as the two accumulators go.)
-__device__ __noinline__ bool ns_wait_written(const unsigned *written, unsigned target, volatile unsigned *gave_up) {
+__device__ __noinline__ bool ns_wait_written(const unsigned *written, unsigned target, WaitLimit *wait) {
   const uint32_t at = smem_address(written);
   const long long start = clock64();
   for (unsigned spins = 0;; ++spins) {
@@ -504,13 +493,7 @@ __device__ __noinline__ bool ns_wait_written(const unsigned *written, unsigned t
       all = all && v.x >= target && v.y >= target && v.z >= target && v.w >= target;
     }
     if (all) break;
-    if ((spins & 63) == 63) {
-      if (*gave_up) return false;
-      if (clock64() - start > kWaitCycles) {
-        *gave_up = 1;
-        return false;
-      }
-    }
+    if ((spins & 63) == 63 && wait->over(start)) return false;
   }
   __threadfence_block();
   return true;
@@ -537,7 +520,7 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
     // K blocks before these are above the diagonal
     const unsigned flip_left = what == kGram ? 0 : 2 * CTAS * at.i;
     const unsigned flip_right = what == kGram ? 0 : what == kApply ? ~0u : 2 * CTAS * (narrow ? at.j / 2 : at.j);
-    if (!ns_wait_counter(&sh.allowed, ++ring.tiles, &sh.gave_up)) return false;
+    if (!ns_wait_counter(&sh.allowed, ++ring.tiles, &sh.wait)) return false;
     asm volatile("fence.proxy.async.global;" ::: "memory"); // panels are written with plain stores
     const unsigned k_linear = ns_linear_after<CTAS>(at, what);
     for (unsigned k = 0; k <= at.k_blocks; ++k) {
@@ -547,7 +530,7 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
         const unsigned rb = at.i * CTAS + ring.rank, cbs = what == kPolynomial ? mcb : xcb;
         const unsigned cb0 = narrow ? at.j : at.j * 2 * CTAS, cb_end = cb0 + (narrow ? 1 : 2 * CTAS);
         for (unsigned c = 0; c < CTAS; ++c, ring.next_stage()) {
-          if (!barrier_wait(smem_address(&sh.empty[ring.stage]), ring.phase ^ 1, &sh.gave_up)) return false;
+          if (!barrier_wait(smem_address(&sh.empty[ring.stage]), ring.phase ^ 1, &sh.wait)) return false;
           const uint32_t bar = smem_address(&sh.linear_full[c][ring.stage]), dst = ring.stages + ring.stage * kNsStageBytes;
           const unsigned first = cb0 + 2 * c;
           unsigned n = 0; // block columns that exist
@@ -559,7 +542,7 @@ __device__ bool ns_load(NsShared &sh, NsRing &ring, int s, int what) {
         }
       }
       if (k == at.k_blocks) break;
-      if (!barrier_wait(smem_address(&sh.empty[ring.stage]), ring.phase ^ 1, &sh.gave_up)) return false;
+      if (!barrier_wait(smem_address(&sh.empty[ring.stage]), ring.phase ^ 1, &sh.wait)) return false;
       const uint32_t bar = smem_address(&sh.full[ring.stage]), dst = ring.stages + ring.stage * kNsStageBytes;
       const unsigned kb = at.k0 + k;
       const bool fl = kb < flip_left, fr = kb < flip_right;
@@ -581,7 +564,7 @@ __device__ bool ns_look_out(NsShared &sh, NsRing &ring, int s, int what) {
   for (unsigned tile = ring.first; tile < t.tiles[what]; tile += gridDim.x / CTAS) {
     NsTile at;
     const NsMat &q = tile_at<CTAS>(t, what, tile, at);
-    if (!ns_wait_stored<CTAS>(t, q, s, what, &sh.gave_up)) return false;
+    if (!ns_wait_stored<CTAS>(t, q, s, what, &sh.wait)) return false;
     __threadfence_block();
     sh.allowed = ++ring.tiles;
   }
@@ -607,16 +590,16 @@ __device__ bool ns_multiply(NsShared &sh, NsRing &ring, int what) {
       if (k == at.k_blocks) break;
       const uint32_t full = smem_address(&sh.full[ring.stage]);
       const unsigned parity = ring.take_turn(ring.stage);
-      if (!__all_sync(0xffffffffu, barrier_wait(full, parity, &sh.gave_up))) return false;
+      if (!__all_sync(0xffffffffu, barrier_wait(full, parity, &sh.wait))) return false;
       if (CTAS > 1 && ring.rank != 0) {
         if (elect_one()) barrier_arrive_at(smem_address(&sh.peer_full[ring.stage]), 0);
         __syncwarp();
         continue;
       }
       const bool first = k % kNsChunk<CTAS> == 0, last = k % kNsChunk<CTAS> == kNsChunk<CTAS> - 1 || k + 1 == at.k_blocks;
-      if (first && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_empty[ring.buf]), ring.turn ^ 1, &sh.gave_up)))
+      if (first && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_empty[ring.buf]), ring.turn ^ 1, &sh.wait)))
         return false;
-      if (CTAS > 1 && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.peer_full[ring.stage]), parity, &sh.gave_up)))
+      if (CTAS > 1 && !__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.peer_full[ring.stage]), parity, &sh.wait)))
         return false;
       tmem_fence_after();
       const bool fl = at.k0 + k < flip_left, fr = at.k0 + k < flip_right;
@@ -684,7 +667,7 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
         NsRing here = ring;
         here.skip_stages(k_linear + part_of_linear);
         if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.linear_full[part_of_linear][here.stage]), ring.take_turn(here.stage),
-                                                  &sh.gave_up)))
+                                                  &sh.wait)))
           return false;
         const unsigned block = CTAS > 1 ? (quarter & 1) : narrow ? 0 : quarter / 2;
         const unsigned chunk0 = CTAS > 1 ? 0 : narrow ? quarter * 2 : (quarter & 1) * 4;
@@ -719,7 +702,7 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
         }
       }
       if (c == rounds) break;
-      if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_full[ring.buf]), ring.turn, &sh.gave_up))) return false;
+      if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&sh.acc_full[ring.buf]), ring.turn, &sh.wait))) return false;
       tmem_fence_after();
       const uint32_t from = sh.tmem + (((warp & 3) * 32) << 16) + ring.buf * kColumns + quarter * columns;
 #pragma unroll
@@ -834,7 +817,7 @@ __device__ bool ns_drain(NsShared &sh, NsRing &ring, int s, int what, bool last,
       } else {
         // the weights (or the output), along the matrix's rows as they are stored: the lanes' rows where it
         // was turned, else 16 columns of two rows through shared memory
-        const float scale = g_ns_gave_up ? NAN : finish * kSplitUnscale * q.rate;
+        const float scale = finish * kSplitUnscale * q.rate;
         float *mine = reinterpret_cast<float *>(piece);
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
@@ -887,11 +870,26 @@ __device__ bool ns_publish(NsShared &sh, NsRing &ring, int what) {
   for (unsigned tile = ring.first; tile < t.tiles[what]; tile += gridDim.x / CTAS) {
     NsTile at;
     const NsMat &q = tile_at<CTAS>(t, what, tile, at);
-    if (!ns_wait_written(sh.written, ++ring.tiles, &sh.gave_up)) return false;
+    if (!ns_wait_written(sh.written, ++ring.tiles, &sh.wait)) return false;
     if (at.parts == 1)
       asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(t.stored + (&q - t.mat)), "n"(kNsEpilogueWarps) : "memory");
   }
   return true;
+}
+
+// After a wait that ran out: NaN over this CTA's tiles of the results. What other CTAs have stored was made of
+// complete operands; what they could not store they overwrite themselves (of a split K every CTA with a part).
+template <int CTAS>
+__device__ __noinline__ void ns_spoil(const NsTable &t, unsigned first, unsigned rank) {
+  for (unsigned tile = first; tile < t.tiles[kApply]; tile += gridDim.x / CTAS) {
+    NsTile at;
+    const NsMat &q = tile_at<CTAS>(t, kApply, tile, at);
+    const unsigned wide = ns_wide<CTAS>(CTAS == 1 && t.narrow[kApply]), row0 = (at.i * CTAS + rank) * 128, col0 = at.j * wide;
+    for (unsigned e = threadIdx.x; e < 128 * wide; e += kNsThreads) {
+      const unsigned row = row0 + e / wide, col = col0 + e % wide;
+      if (row < q.m && col < q.n) q.w[q.turned ? (u64)col * q.m + row : (u64)row * q.n + col] = NAN;
+    }
+  }
 }
 
 template <int CTAS>
@@ -914,7 +912,8 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
       barrier_init(smem_address(&sh.acc_empty[b]), kNsEpilogueWarps * CTAS);
     }
     barrier_init(smem_address(&sh.drained), 1);
-    sh.gave_up = sh.allowed = 0;
+    sh.wait.limit = param.wait_cycles;
+    sh.wait.gave_up = sh.allowed = 0;
     for (int w = 0; w < kNsEpilogueWarps; ++w) sh.written[w] = 0;
     for (int s = 0; s < kNsStages; ++s) sh.linear_read[s] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -946,24 +945,30 @@ __global__ void __launch_bounds__(kNsThreads, 1) muon_steps_kernel(const __grid_
     }
     before = (before + t.tiles[what]) % workers;
   }
-  if (!ok && lane == 0) { // after a wait that ran out: what is in flight ends before its memory goes away
+  __syncwarp();
+  __syncthreads();
+  if (sh.wait.gave_up) { // what is in flight ends before its memory goes away
     const long long start = clock64();
-    if (warp == kNsEpilogueWarps)
+    if (warp == kNsEpilogueWarps && lane == 0)
       for (int i = 0; i < 3 * kNsStages; ++i) { // the last copy of each barrier
         const uint32_t bar = i < kNsStages ? smem_address(&sh.full[i]) : smem_address(&sh.linear_full[i / kNsStages - 1][i % kNsStages]);
         while (!barrier_try(bar, ((ring.turns >> i) & 1) ^ 1) && clock64() - start < 10000000) {}
       }
-    if (warp == kNsEpilogueWarps + 1 && ring.rank == 0) {
+    if (warp == kNsEpilogueWarps + 1 && ring.rank == 0 && elect_one()) {
       mma_commit<CTAS>(smem_address(&sh.drained));
       while (!barrier_try(smem_address(&sh.drained), 0) && clock64() - start < 10000000) {}
     }
+    __syncwarp();
+    const unsigned skipped = (unsigned)((u64)(steps - 1) * (t.tiles[kGram] + t.tiles[kPolynomial] + t.tiles[kApply]) % workers);
+    before = (skipped + t.tiles[kGram] + t.tiles[kPolynomial]) % workers; // the last product's, as in the loop
+    ns_spoil<CTAS>(t, (me + workers - before) % workers, ring.rank);
+    if (threadIdx.x == 0) atomicAdd(&g_ns_gave_up, 1u);
   }
   __syncwarp();
   tmem_fence_before();
   __syncthreads();
   if (CTAS > 1) cluster_sync_all(); // nothing of this CTA is used by the other one any more
   tmem_fence_after();
-  if (threadIdx.x == 0 && sh.gave_up) atomicOr(&g_ns_gave_up, 1u);
   if (warp == kNsEpilogueWarps + 1) tmem_free<CTAS>(sh.tmem, 2 * 128 * CTAS);
 }
 
@@ -1070,6 +1075,7 @@ static NsTable steps_table(const MuonTable &mt) {
   t.tickets = mt.tickets;
   t.parts = mt.parts;
   t.room = (unsigned)sm_count();
+  t.wait_cycles = tuned(kTuneMuonWait) >= 0 ? tuned(kTuneMuonWait) * 1000ll : kWaitCycles;
   for (int i = 0; i < mt.count; ++i) {
     const MuonMat &q = mt.mat[i];
     NsMat &d = t.mat[i];
@@ -1441,14 +1447,23 @@ void plast_b200_orthogonalise(const Tensor **inputs, Tensor **outputs, int count
 
 int plast_b200_muon_status(void) {
   begin_call();
-  unsigned status = 0;
+  static std::mutex mutex;
+  static std::unordered_map<int, unsigned> told; // per device: what an earlier look has seen
+  int device = 0;
+  unsigned now = 0;
+  PB_CUDA_RET(cudaGetDevice(&device), -1);
+  PB_CUDA_RET(cudaMemcpyFromSymbolAsync(&now, g_ns_gave_up, sizeof now, 0, cudaMemcpyDeviceToHost, stream()), -1);
   PB_CUDA_RET(cudaStreamSynchronize(stream()), -1);
-  PB_CUDA_RET(cudaMemcpyFromSymbol(&status, g_ns_gave_up, sizeof status), -1);
-  if (status) {
-    const unsigned none = 0;
-    PB_CUDA_RET(cudaMemcpyToSymbol(g_ns_gave_up, &none, sizeof none), -1);
+  try {
+    std::lock_guard<std::mutex> lock(mutex);
+    unsigned &seen = told[device];
+    const bool more = now != seen;
+    seen = now;
+    return more;
+  } catch (...) { // std::bad_alloc
+    set_error(PLAST_B200_ERR_CUDA, "muon: out of host memory");
+    return -1;
   }
-  return (int)status;
 }
 
 void plast_b200_muon_state_release(Tensor **m) {

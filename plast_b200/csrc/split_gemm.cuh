@@ -84,24 +84,30 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, unsigned parity) {
                : "memory");
   return ok != 0;
 }
-// A wait that always ends: after about two seconds, or when another role of the CTA has given up, it
-// raises `*gave_up` (shared memory) and returns false; the caller then leaves its loop.
-constexpr long long kWaitCycles = 4000000000ll;
-__device__ __noinline__ bool barrier_wait_long(uint32_t bar, unsigned parity, volatile unsigned *gave_up) {
+// A wait that always ends: after `limit` cycles, or when another role of the CTA has given up, it raises
+// `gave_up` and returns false; the caller then leaves its loop.
+constexpr long long kWaitCycles = 4000000000ll; // about two seconds
+struct WaitLimit { // shared memory
+  long long limit;
+  volatile unsigned gave_up;
+  __device__ __forceinline__ bool over(long long start) { // looked at now and then
+    if (gave_up) return true;
+    if (clock64() - start <= limit) return false;
+    gave_up = 1;
+    return true;
+  }
+};
+__device__ __noinline__ bool barrier_wait_long(uint32_t bar, unsigned parity, WaitLimit *wait) {
   const long long start = clock64();
   for (;;) {
     for (int i = 0; i < 64; ++i)
       if (barrier_try(bar, parity)) return true;
-    if (*gave_up) return false;
-    if (clock64() - start > kWaitCycles) {
-      *gave_up = 1;
-      return false;
-    }
+    if (wait->over(start)) return false;
   }
 }
 
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, unsigned parity, volatile unsigned *gave_up) {
-  return barrier_try(bar, parity) || barrier_wait_long(bar, parity, gave_up);
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, unsigned parity, WaitLimit *wait) {
+  return barrier_try(bar, parity) || barrier_wait_long(bar, parity, wait);
 }
 
 // ---- copies and tensor core ----------------------------------------------------------------------------

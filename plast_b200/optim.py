@@ -95,6 +95,14 @@ def orthogonalise(inputs, outputs, steps: int = 5, epsilon: float = 1e-7) -> Non
     check_error()
 
 
+def muon_status() -> bool:
+    """Whether a wait inside a Muon step or an orthogonalisation has run out since the last look: results of such a
+    call hold NaN (plast_b200_muon_status). Waits for the library stream."""
+    status = lib.plast_b200_muon_status()
+    check_error()
+    return status != 0
+
+
 def release_state(optimizer) -> None:
     if isinstance(optimizer, Muon):
         if optimizer.m:

@@ -408,3 +408,44 @@ def test_warps_that_have_nothing_to_store_run_ahead(shapes):
 def test_parts_of_a_split_k_are_added_in_one_order():
     rs = np.random.RandomState(23)
     same_bits_and_right([rs.randn(*s).astype(np.float32) for s in [(64, 9000), (120, 4000), (300, 3000)]], 20)
+
+
+def test_a_wait_that_runs_out_leaves_nan_and_a_status():
+    """A limit of no cycles: the waits for a product of many microseconds give up at their first look. What was not
+    computed is NaN, the rest is right, the next call works."""
+    rs = np.random.RandomState(29)
+    xs = [rs.randn(2048, 2500).astype(np.float32), rs.randn(1900, 1500).astype(np.float32)]
+    ins, outs = [pb.Tensor.from_numpy(x) for x in xs], [pb.Tensor(x.shape) for x in xs]
+    ws = [rs.randn(*x.shape).astype(np.float32) for x in xs]
+
+    def orthogonalised():
+        O.orthogonalise(ins, outs)
+        return [o.numpy() for o in outs]
+
+    def stepped():
+        ps, ms = [pb.Tensor.from_numpy(w) for w in ws], [pb.Tensor.from_numpy(x) for x in xs]
+        for p, x in zip(ps, ins):
+            p.set_grad(x)
+        O.step(O.Muon.create(lr=0.1, momentum=0.5, moments=ms), ps)
+        return [p.numpy() for p in ps], [m.numpy() for m in ms]
+
+    want, (want_w, want_m) = orthogonalised(), stepped()
+    assert not O.muon_status()
+    for call in (orthogonalised, lambda: stepped()):
+        for o in outs:
+            o.copy_from(np.full(o.shape, 7.0, np.float32))
+        pb.lib.plast_b200_tune(13, 0)
+        try:
+            got = call()
+        finally:
+            pb.lib.plast_b200_tune(13, -1)
+        assert O.muon_status() and not O.muon_status()          # told once
+        if call is not orthogonalised:
+            got, moments = got
+            for g, w in zip(moments, want_m):
+                assert np.array_equal(g, w)
+        assert any(np.isnan(g).any() for g in got)
+        for g, w in zip(got, want if call is orthogonalised else want_w):
+            assert np.array_equal(g[~np.isnan(g)], w[~np.isnan(g)])
+    for g, w in zip(orthogonalised(), want):
+        assert np.array_equal(g, w)
