@@ -453,7 +453,8 @@ struct NsRing {
   }
 };
 
-// Waits until matrix q's products up to this one (step s, product what) are stored.
+// Waits until matrix q's products up to this one (step s, product what) are stored. The look-out thread begins to wait
+// when the product before begins, which may take longer than the limit: it counts from the last tile that was stored.
 template <int CTAS>
 __device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, int s, int what, WaitLimit *wait) {
   unsigned target = 0;
@@ -461,11 +462,13 @@ __device__ __noinline__ bool ns_wait_stored(const NsTable &t, const NsMat &q, in
   target *= CTAS * kNsEpilogueWarps;
   const unsigned *counter = t.stored + (&q - t.mat);
   long long start = 0;
+  unsigned last = 0;
   for (unsigned spins = 0;; ++spins) {
     unsigned now;
     asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(counter) : "memory");
     if (now >= target) return true;
-    if (spins == 0) start = clock64();
+    if (spins == 0 || now != last) start = clock64();
+    last = now;
     if ((spins & 63) == 63 && wait->over(start)) return false;
   }
 }

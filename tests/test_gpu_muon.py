@@ -449,3 +449,18 @@ def test_a_wait_that_runs_out_leaves_nan_and_a_status():
             assert np.array_equal(g[~np.isnan(g)], w[~np.isnan(g)])
     for g, w in zip(orthogonalised(), want):
         assert np.array_equal(g, w)
+
+
+def test_a_product_may_take_longer_than_the_limit_of_a_wait():
+    """8192 x 8192: a tile takes up to 0.25 million cycles and a product 2 million and more. What is waited for is a
+    tile at a time, so a limit of 1.2 million is not reached."""
+    torch = pytest.importorskip("torch")
+    x, out = torch.randn(8192, 8192, device="cuda"), torch.empty(8192, 8192, device="cuda")
+    torch.cuda.synchronize()
+    pb.lib.plast_b200_tune(13, 1200)
+    try:
+        O.orthogonalise([pb.Tensor.wrap_pointer(x.data_ptr(), x.shape)], [pb.Tensor.wrap_pointer(out.data_ptr(), x.shape)], steps=2)
+    finally:
+        pb.lib.plast_b200_tune(13, -1)
+    assert not O.muon_status()
+    assert torch.isfinite(out).all()
