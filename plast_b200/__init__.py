@@ -266,6 +266,7 @@ class Tensor:
         self._np = None
         self._dptr = None
         self.grad = None
+        self._owns_grad = False
         n = int(np.prod(shape)) if shape else 1
         self._storage_elems = n if _storage_elems is None else _storage_elems
         if _ptr is not None:
@@ -304,13 +305,16 @@ class Tensor:
         g = Tensor(shape, device=self.device, dtype=self.c.dtype)
         g.zero_()
         self.grad = g
+        self._owns_grad = True
         self.c.grad = C.pointer(g.c)
         self.c.requires_grad = True
         return g
 
     def set_grad(self, grad: "Tensor"):
-        """Makes `grad` (a Tensor over memory of its own or somebody else's) this tensor's gradient."""
+        """Makes `grad` (a Tensor over memory of its own or somebody else's) this tensor's gradient. It stays its
+        owner's: free() of this tensor leaves its memory alone."""
         self.grad = grad
+        self._owns_grad = False
         self.c.grad = C.pointer(grad.c)
         self.c.requires_grad = True
         return grad
@@ -376,7 +380,7 @@ class Tensor:
         if self._dptr is not None:
             lib.arena_free_cuda(self._dptr)
             self._dptr = None
-        if self.grad is not None:
+        if self.grad is not None and self._owns_grad:
             self.grad.free()
 
     def __del__(self):

@@ -80,3 +80,31 @@ def test_the_layer_takes_tensors_only():
                      lambda: optim.step(optim.SGD(0.1), [wrong]), lambda: optim.orthogonalise([wrong], [x])):
             with pytest.raises((AttributeError, TypeError)):
                 call()
+
+
+def test_a_gradient_that_was_set_stays_its_owners(monkeypatch):
+    """Tensors that come and go with one gradient (a step's parameters over the same buffer) do not free it."""
+    freed = []
+
+    class Device:
+        def __getattr__(self, name):
+            return freed.append if name == "arena_free_cuda" else getattr(pb._LazyLib._lib, name)
+
+    grad, other = pb.Tensor((3,), device="cpu"), pb.Tensor((3,), device="cpu")
+    monkeypatch.setattr(pb, "lib", Device())
+    grad._dptr, other._dptr = 11, 12                     # as if they held device memory
+    other.set_grad(grad)
+    del other
+    assert freed == [12]
+    t = pb.Tensor((3,), device="cpu", requires_grad=True)
+    t.grad._dptr = 13
+    t.free()                                             # its own goes with it
+    assert freed == [12, 13]
+    t.attach_grad()._dptr = 14
+    t.set_grad(grad)                                     # replaced: nobody holds it any more
+    assert freed == [12, 13, 14]
+    t.free()
+    del t
+    assert freed == [12, 13, 14] and grad._dptr == 11
+    del grad
+    assert freed == [12, 13, 14, 11]
