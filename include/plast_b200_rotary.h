@@ -29,7 +29,7 @@ extern "C" {
 
 /* rotary as an op of the table: inputs = {x, positions, inv_freq}, params.dim = the pair layout,
  * params.fval = the amplitude (positive; 1 unless a scaling asks for more). The output may be x
- * itself (same data and strides). Backward turns the other way: x->grad += amplitude * R(-angle)
+ * itself (same data and strides); no other overlap. Backward turns the other way: x->grad += amplitude * R(-angle)
  * output->grad; positions and inv_freq receive no gradient (requires_grad on them is refused). */
 void rotary_cuda_forward(const Tensor **inputs, Tensor *output, KernelParams params);
 void rotary_cuda_backward(Tensor **inputs, const Tensor *output, KernelParams params);
@@ -68,7 +68,9 @@ int plast_b200_rotary_frequencies(const PlastRotaryScaling *scaling, u64 rotated
  *   n = x / sqrt(mean(x^2) + epsilon),  u = weight * n,  out = rotary(u)
  * q and k may have different numbers of heads (and shapes) but the same head size; k, k_weight and
  * k_out may be NULL together (one tensor alone). A weight is FLOAT32 with head-size elements along
- * its last dim ([head], [1, head], ...), or NULL for none. An output may be its own input.
+ * its last dim ([head], [1, head], ...), or NULL for none. An output may be its own input (same data and
+ * strides) and shares no element with any other tensor of the call, nor does the gradient of an input
+ * in backward but with the gradient of its own output.
  * Backward recomputes the norm from q and k, reads q_out->grad and k_out->grad and adds to the
  * gradients of q, k and the weights, each where requires_grad is set; weight gradients are summed in
  * a fixed order. The sum of squares is held in 32 bits: a head whose elements pass about 10^18 overflows

@@ -529,17 +529,10 @@ static bool check_same_heads(const char *name, const Tensor *x, const Tensor *y,
   return true;
 }
 
-// An output lies over its own input element by element or not at all.
 static bool check_output(const char *name, const Tensor *x, const Tensor *y) {
   if (!check_same_heads(name, x, y, "output")) return false;
   if (has_repeated_elements(y)) {
     set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: the output is an expanded view", name);
-    return false;
-  }
-  bool same = true;
-  for (u64 d = 0; d < x->ndim; ++d) same = same && (x->shape[d] <= 1 || x->strides[d] == y->strides[d]);
-  if (x->data == y->data && !same) {
-    set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: in place, the output needs its input's strides", name);
     return false;
   }
   return true;
@@ -573,6 +566,8 @@ void rotary_cuda_forward(const Tensor **inputs, Tensor *output, KernelParams par
     return;
   const Tensor *const streams[3] = {x, nullptr, output};
   if (!plan_side("rotary", &p.side[0], streams, inputs[1])) return;
+  const Extent others[2] = {extent_of(inputs[1]), extent_of(inputs[2])};
+  if (!check_apart("rotary", "the output", extent_of(output), extent_of(x), others, 2)) return;
   if (numel(x) == 0) return; // nothing to do
   p.side[0].in0 = p.side[0].in1 = (const float *)x->data;
   p.side[0].out = (float *)output->data;
@@ -597,6 +592,8 @@ void rotary_cuda_backward(Tensor **inputs, const Tensor *output, KernelParams pa
     return;
   const Tensor *const streams[3] = {output->grad, nullptr, x->grad};
   if (!plan_side("rotary", &p.side[0], streams, inputs[1])) return;
+  const Extent others[2] = {extent_of(inputs[1]), extent_of(inputs[2])};
+  if (!check_apart("rotary", "the gradient of x", extent_of(x->grad), extent_of(output->grad), others, 2)) return;
   if (numel(x) == 0) return; // nothing to do
   p.side[0].in0 = p.side[0].in1 = (const float *)output->grad->data;
   p.side[0].out = (float *)x->grad->data;
@@ -704,8 +701,6 @@ void plast_b200_qk_norm_rotary(const Tensor *q, const Tensor *k, const Tensor *q
   for (int i = 0; i < 2; ++i) {
     if (!xs[i]) continue;
     if (!check_output(name, xs[i], outs[i])) return;
-    if (i == 1 && q_out && outs[1]->data == q_out->data && numel(k) > 0)
-      return set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: q_out and k_out are one buffer", name);
     HeadSide &sd = p.side[sides];
     const Tensor *const streams[3] = {xs[i], nullptr, outs[i]};
     if (!plan_side(name, &sd, streams, positions)) return;
@@ -718,6 +713,12 @@ void plast_b200_qk_norm_rotary(const Tensor *q, const Tensor *k, const Tensor *q
     sd.weight = ws[i] ? (const float *)ws[i]->data : nullptr;
     sd.weight_stride = ws[i] ? ws[i]->strides[ws[i]->ndim - 1] : 0;
     ++sides;
+  }
+  // both sides run at once: an output lies over its own input at most
+  const Extent in[2] = {extent_of(q), extent_of(k)}, out[2] = {extent_of(q_out), extent_of(k_out)};
+  for (int i = 0; i < (k ? 2 : 1); ++i) {
+    const Extent others[6] = {in[1 - i], out[1 - i], extent_of(q_weight), extent_of(k_weight), extent_of(positions), extent_of(inv_freq)};
+    if (!check_apart(name, i ? "k_out" : "q_out", out[i], in[i], others, 6)) return;
   }
   if (sides) launch_heads<true, false>(p, sides, 0);
   note_kernel("qk_norm_rotary");
@@ -767,8 +768,18 @@ void plast_b200_qk_norm_rotary_backward(Tensor *q, Tensor *k, Tensor *q_weight, 
     ++sides;
   }
   if (!sides) return; // nothing to do
-  if (sides == 2 && p.side[0].out && p.side[0].out == p.side[1].out)
-    return set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: the gradients of q and k are one buffer", name);
+  // Both sides run at once: the gradient of an input lies over the gradient of its output at most, that of a weight (added
+  // afterwards) over the other weight's at most.
+  auto written = [](const Tensor *t) { return extent_of(t && t->requires_grad ? t->grad : nullptr); };
+  const Extent in[2] = {extent_of(q), extent_of(k)}, dout[2] = {extent_of(q_out ? q_out->grad : nullptr), extent_of(k_out ? k_out->grad : nullptr)};
+  for (int i = 0; i < (k ? 2 : 1); ++i) {
+    const Extent others[8] = {in[0], in[1], dout[1 - i], written(xs[1 - i]), extent_of(q_weight), extent_of(k_weight), extent_of(positions), extent_of(inv_freq)};
+    if (!check_apart(name, i ? "the gradient of k" : "the gradient of q", written(xs[i]), dout[i], others, 8)) return;
+  }
+  const Extent dqw = written(q_weight), dkw = written(k_weight);
+  if (share_an_element(dqw, dkw) && // but for a shared weight, whose dims before the last may differ
+      (dqw.t->data != dkw.t->data || dqw.t->strides[dqw.t->ndim - 1] != dkw.t->strides[dkw.t->ndim - 1]))
+    return set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: the gradients of the weights overlap", name);
   const unsigned max_blocks = (unsigned)sm_count() * 2; // all resident: each keeps one partial sum
   float *scratch = nullptr;
   if (wants_weight[0] || wants_weight[1]) {

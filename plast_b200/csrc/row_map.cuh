@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "overlap.h"
 
 namespace pb {
 
@@ -61,6 +62,14 @@ inline bool is_packed(const Tensor *t) {
     expect *= t->shape[d];
   }
   return true;
+}
+
+// A tensor that is written may lie over `own` (may be NULL) element by element, and over none of the others.
+inline bool check_apart(const char *name, const char *what, const Extent &written, const Extent &own, const Extent *others, int n) {
+  bool ok = !own.t || !share_an_element(written, own) || same_elements(written.t, own.t);
+  for (int i = 0; ok && i < n; ++i) ok = !share_an_element(written, others[i]);
+  if (!ok) set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: %s overlaps another tensor of the call", name, what);
+  return ok;
 }
 
 // A tensor that is written element by element must not hold one element at two indices (an

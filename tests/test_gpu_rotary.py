@@ -287,3 +287,48 @@ def test_offsets_beyond_32_bits():
     pb.synchronize()
     want = R.rotate(np.arange(64.0)[None], np.array([3]), freq, True)[0]
     np.testing.assert_allclose(x[2, -1].cpu().numpy(), want, atol=1e-5)
+
+
+def test_heads_of_one_fused_row():
+    """Queries, keys and values side by side in a row, as one product gives them: normed and rotated in place, and the
+    gradients added into the slices of one row of gradients. The same bits as with buffers of their own."""
+    rs = np.random.RandomState(12)
+    v = qk_case(rs, (2, 30, 6, 64), (2, 30, 2, 64), 32)
+    t = qk_run(v, 0, 1e-6)
+    B, T, H, K, D = 2, 30, 6, 2, 64
+    row = (H + 2 * K) * D
+
+    def fused(q, k):
+        host = data(rs, B, T, row)
+        host[..., :H * D], host[..., H * D:(H + K) * D] = q.reshape(B, T, -1), k.reshape(B, T, -1)
+        whole = pb.Tensor.from_numpy(host)
+        return host, whole, [whole.view((B, T, n, D), (T * row, row, D, 1), offset=o) for n, o in ((H, 0), (K, H * D))]
+
+    def same(whole, host, q, k):
+        got = whole.numpy()
+        assert np.array_equal(got[..., :H * D], q.reshape(B, T, -1)) and np.array_equal(got[..., H * D:(H + K) * D], k.reshape(B, T, -1))
+        assert np.array_equal(got[..., (H + K) * D:], host[..., (H + K) * D:])      # the values
+
+    host, whole, (q, k) = fused(v["q"], v["k"])
+    dhost, dwhole, (dq, dk) = fused(v["start_q"], v["start_k"])
+    q.set_grad(dq)
+    k.set_grad(dk)
+    weights = [pb.Tensor.from_numpy(v[s], requires_grad=True) for s in ("qw", "kw")]
+    pb.qk_norm_rotary_backward(q, k, *weights, t["pos"], t["freq"], t["qo"], t["ko"], epsilon=1e-6)
+    same(dwhole, dhost, t["q"].grad.numpy(), t["k"].grad.numpy())
+    pb.qk_norm_rotary(q, k, t["qw"], t["kw"], t["pos"], t["freq"], q, k, epsilon=1e-6)
+    same(whole, host, t["qo"].numpy(), t["ko"].numpy())
+    # the rotation alone, of the keys in place, and its gradient over the gradient of its output
+    _, _, (_, k) = fused(v["q"], v["k"])
+    out = pb.Tensor((B, T, K, D))
+    pb.forward("rotary", [pb.Tensor.from_numpy(v["k"]), t["pos"], t["freq"]], out, fval=1.0)
+    pb.forward("rotary", [k, t["pos"], t["freq"]], k, fval=1.0)
+    assert np.array_equal(k._base.numpy()[..., H * D:(H + K) * D], out.numpy().reshape(B, T, -1))
+    x, y = pb.Tensor.from_numpy(v["k"], requires_grad=True), pb.Tensor((B, T, K, D), requires_grad=True)
+    y.grad.copy_from(v["dk"])
+    x.grad.copy_from(v["dk"])
+    pb.backward("rotary", [x, t["pos"], t["freq"]], y, fval=1.0)
+    want = x.grad.numpy()
+    x.set_grad(y.grad)
+    pb.backward("rotary", [x, t["pos"], t["freq"]], y, fval=1.0)
+    assert np.array_equal(x.grad.numpy(), want)

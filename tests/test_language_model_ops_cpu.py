@@ -248,3 +248,73 @@ def test_orthogonalise_refusals():
     refused("UNSUPPORTED", O.orthogonalise, [x, y], [base.view((4, 6), (6, 1)), base.view((4, 6), (6, 1), offset=18)])
     refused("UNSUPPORTED", O.orthogonalise, [x], [o], 40)
     refused("UNSUPPORTED", O.orthogonalise, [x], [o], 5, -1.0)
+
+
+def test_rotary_refuses_buffers_that_overlap():
+    base, pos, freq = T(1000), T(2, 3, 1, dtype=I), T(8)
+    shape, dense = (2, 3, 4, 16), (192, 64, 16, 1)
+
+    def at(offset, strides=dense):
+        return base.view(shape, strides, offset=offset)
+
+    def f(x, out, pos=pos, freq=freq):
+        refused("UNSUPPORTED", pb.forward, "rotary", [x, pos, freq], out, fval=1.0)
+
+    f(at(0), at(16))                                          # a head on
+    f(at(17), at(0))
+    f(at(0), at(0, (192, 16, 48, 1)))                        # the same memory in another order
+    f(at(0), at(3, (384, 128, 32, 2)))                       # every second element
+    f(at(400), at(0), freq=base.view((8,), (1,), offset=383))
+    f(at(400), at(0), freq=base.view((8,), (2,), offset=100))
+    f(at(400), at(0), pos=pb.Tensor((2, 3, 1), device="cpu", dtype=I, _base=base, _storage_elems=1000))
+    x, out = at(0), T(*shape)
+    x.set_grad(at(400))
+    out.set_grad(at(401))
+    refused("UNSUPPORTED", pb.backward, "rotary", [x, pos, freq], out, fval=1.0)
+    out.set_grad(at(400, (192, 16, 48, 1)))
+    refused("UNSUPPORTED", pb.backward, "rotary", [x, pos, freq], out, fval=1.0)
+
+
+def test_qk_norm_refuses_buffers_that_overlap():
+    base, pos, freq = T(4000), T(2, 3, 1, dtype=I), T(8)
+
+    def q_at(offset):
+        return base.view((2, 3, 4, 16), (192, 64, 16, 1), offset=offset)
+
+    def k_at(offset):
+        return base.view((2, 3, 2, 16), (96, 32, 16, 1), offset=offset)
+
+    def f(q, k, qo, ko, qw=None, kw=None, call=pb.qk_norm_rotary):
+        refused("UNSUPPORTED", call, q, k, qw, kw, pos, freq, qo, ko)
+
+    f(q_at(0), k_at(500), k_at(500).view((2, 3, 4, 16), (192, 64, 16, 1)), k_at(1000))    # q_out begins where k does
+    f(q_at(0), k_at(500), q_at(595), k_at(1000))                                          # one element of k
+    f(q_at(0), k_at(500), q_at(1000), k_at(383))                                          # k_out over the end of q
+    f(q_at(0), k_at(500), q_at(1000), k_at(1100))                                         # over q_out
+    f(q_at(0), k_at(500), q_at(16), k_at(1000))                                           # over its own input, a head on
+    f(q_at(0), k_at(500), q_at(1000), k_at(508))
+    f(q_at(0), k_at(500), q_at(1000), k_at(2000), qw=base.view((16,), (1,), offset=2090))
+    f(q_at(0), None, q_at(1000), None, qw=base.view((16,), (1,), offset=1000))
+
+    back = pb.qk_norm_rotary_backward
+    q, k, qo, ko = q_at(0), k_at(500), T(2, 3, 4, 16), T(2, 3, 2, 16)
+
+    def grads(dq, dk, dqo, dko):
+        for t, g in ((q, dq), (k, dk), (qo, dqo), (ko, dko)):
+            t.set_grad(g)
+
+    grads(q_at(1000), k_at(1383), q_at(2000), k_at(2500))     # dq and dk
+    f(q, k, qo, ko, call=back)
+    grads(q_at(1000), k_at(1500), q_at(2000), k_at(1000))     # dq and the gradient of k_out
+    f(q, k, qo, ko, call=back)
+    grads(q_at(1000), k_at(1500), q_at(1004), k_at(2500))     # dq, four elements off the gradient of q_out
+    f(q, k, qo, ko, call=back)
+    grads(q_at(1000), k_at(100), q_at(2000), k_at(2500))      # dk and q
+    f(q, k, qo, ko, call=back)
+    grads(q_at(1000), k_at(1500), q_at(2000), k_at(2500))
+    qw, kw = T(16), T(16)
+    qw.set_grad(base.view((16,), (1,), offset=3000))
+    kw.set_grad(base.view((16,), (1,), offset=3004))          # the gradients of the weights
+    f(q, k, qo, ko, qw=qw, kw=kw, call=back)
+    kw.set_grad(base.view((16,), (2,), offset=3000))
+    f(q, k, qo, ko, qw=qw, kw=kw, call=back)
