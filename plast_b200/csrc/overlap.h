@@ -24,6 +24,17 @@ struct StrideSum {
     int budget = 4096;
     return reaches(0, target, budget);
   }
+  // 0 by factors that are not all 0 (the ranges are symmetric: the first of them is positive)
+  bool returns() const {
+    int budget = 4096;
+    for (int k = 0; k < n; ++k) {
+      __int128 high = 0; // of the terms behind
+      for (int i = k + 1; i < n; ++i) high += term[i].stride * term[i].high;
+      for (__int128 v = 1; v <= term[k].high && term[k].stride * v <= high; ++v)
+        if (reaches(k + 1, -term[k].stride * v, budget)) return true;
+    }
+    return false;
+  }
 
 private:
   void add_positive(__int128 stride, __int128 low, __int128 high) {
@@ -84,6 +95,22 @@ inline bool share_an_element(const Extent &a, const Extent &b) {
   for (u64 d = 0; d < b.t->ndim; ++d) sum.add((long long)b.t->strides[d], 1 - (__int128)b.t->shape[d], 0);
   return sum.reaches(apart / 4);
 }
+// A tensor that is written element by element must not hold one element at two indices (an expanded view, or strides
+// that let rows run into each other).
+inline bool has_repeated_elements(const Tensor *t) {
+  StrideSum sum;
+  for (u64 d = 0; d < t->ndim; ++d)
+    if (t->shape[d] == 0) return false;
+  for (u64 d = 0; d < t->ndim; ++d) {
+    if (t->shape[d] == 1) continue;
+    if (t->strides[d] == 0) return true;
+    for (u64 e = 0; e < d; ++e)
+      if (t->shape[e] > 1 && (t->strides[e] == t->strides[d] || t->strides[e] == 0 - t->strides[d])) return true;
+    sum.add((long long)t->strides[d], 1 - (__int128)t->shape[d], (__int128)t->shape[d] - 1);
+  }
+  return sum.returns();
+}
+
 // The same elements at the same indices.
 inline bool same_elements(const Tensor *a, const Tensor *b) {
   if (a->data != b->data || a->ndim != b->ndim) return false;

@@ -532,7 +532,7 @@ static bool check_same_heads(const char *name, const Tensor *x, const Tensor *y,
 static bool check_output(const char *name, const Tensor *x, const Tensor *y) {
   if (!check_same_heads(name, x, y, "output")) return false;
   if (has_repeated_elements(y)) {
-    set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: the output is an expanded view", name);
+    set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: the output holds an element at two indices", name);
     return false;
   }
   return true;

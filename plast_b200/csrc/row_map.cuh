@@ -72,14 +72,6 @@ inline bool check_apart(const char *name, const char *what, const Extent &writte
   return ok;
 }
 
-// A tensor that is written element by element must not hold one element at two indices (an
-// expanded view, stride 0).
-inline bool has_repeated_elements(const Tensor *t) {
-  for (u64 d = 0; d < t->ndim; ++d)
-    if (t->shape[d] > 1 && t->strides[d] == 0) return true;
-  return false;
-}
-
 inline bool same_shape(const Tensor *a, const Tensor *b) {
   if (a->ndim != b->ndim) return false;
   for (u64 d = 0; d < a->ndim; ++d)
@@ -112,7 +104,7 @@ inline bool check_grad(const Tensor *t, const char *what) {
     return false;
   }
   if (has_repeated_elements(t->grad)) {
-    set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: the gradient is an expanded view", what);
+    set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: the gradient holds an element at two indices", what);
     return false;
   }
   return true;

@@ -318,3 +318,20 @@ def test_qk_norm_refuses_buffers_that_overlap():
     f(q, k, qo, ko, qw=qw, kw=kw, call=back)
     kw.set_grad(base.view((16,), (2,), offset=3000))
     f(q, k, qo, ko, qw=qw, kw=kw, call=back)
+
+
+def test_outputs_and_gradients_with_an_element_at_two_indices():
+    """Rows that run into each other, without a stride of 0: several threads would write one element."""
+    base, pos, freq = T(1000), T(6, 1, dtype=I), T(4)
+    x, ok = T(6, 3, 8), T(6, 3, 8)
+    for strides in ((23, 8, 1), (24, 7, 1), (1, 24, 3)):
+        out = base.view((6, 3, 8), strides)
+        refused("UNSUPPORTED", pb.forward, "rotary", [x, pos, freq], out, fval=1.0)
+        refused("UNSUPPORTED", pb.qk_norm_rotary, x, None, None, None, pos, freq, out, None)
+        x.set_grad(out)
+        ok.attach_grad()
+        refused("UNSUPPORTED", pb.backward, "rotary", [x, pos, freq], ok, fval=1.0)
+        refused("UNSUPPORTED", pb.qk_norm_rotary_backward, x, None, None, None, pos, freq, ok, None)
+    logits, tok, st, lp = T(6, 40), T(6, dtype=I), T(6, 2), T(6, requires_grad=True)
+    logits.set_grad(base.view((6, 40), (39, 1)))
+    refused("UNSUPPORTED", pb.token_logprob_backward, logits, tok, st, lp)

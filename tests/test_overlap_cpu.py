@@ -24,7 +24,7 @@ static int read_tensor(Tensor *t) { // offset in bytes, dims, shape, strides
 int main() {
   Tensor a, b;
   while (read_tensor(&a) && read_tensor(&b))
-    printf("%d%d%d\n", pb::share_an_element(pb::extent_of(&a), pb::extent_of(&b)), pb::same_elements(&a, &b), 0);
+    printf("%d%d%d\n", pb::share_an_element(pb::extent_of(&a), pb::extent_of(&b)), pb::same_elements(&a, &b), pb::has_repeated_elements(&a));
   return 0;
 }
 """
@@ -87,3 +87,19 @@ def test_slices_of_a_fused_row(probe):
     answers = probe([(q, k), (k, v), (by_heads, v), (q, early), (early, k), (q, q), (q, by_heads), (q, odd)])
     assert [a[0] for a in answers] == [False, False, False, True, True, True, True, True]
     assert [a[1] for a in answers] == [False] * 5 + [True, False, False]
+
+
+def test_elements_at_two_indices(probe):
+    rng = random.Random(4)
+    tensors = []
+    for _ in range(4000):
+        dims = rng.randint(0, 4)
+        shape = [rng.choice([0, 1, 2, 3, 4]) if rng.random() < 0.2 else rng.randint(1, 4) for _ in range(dims)]
+        strides = [rng.choice([1, 2, 3, 4, 5, 7, 12, 16, 48, -1, -6]) if rng.random() < 0.95 else 0 for _ in range(dims)]
+        tensors.append((0, shape, strides))
+    found = [a[2] for a in probe([(t, t) for t in tensors])]
+    assert found == [len(set(elements(t))) < len(elements(t)) for t in tensors]
+    assert 500 < sum(found) < 3500
+    large = [(0, [2, 4096, 32, 128], [4096 * 6144, 6144, 128, 1]), (0, [2, 32, 4096, 128], [4096 * 6144, 128, 6144, 1]),
+             (0, [2, 4096, 32, 128], [4096 * 6144, 6000, 192, 1]), (0, [8192, 65536], [65535, 1])]
+    assert [a[2] for a in probe([(t, t) for t in large])] == [False, False, True, True]
