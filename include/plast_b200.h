@@ -179,8 +179,8 @@ void cross_entropy_cuda_backward(Tensor **inputs, const Tensor *output, KernelPa
  * tokens: INT32, the logits' shape without the last dim (any strides). logprob, entropy, log_norm:
  * FLOAT32, contiguous, one element per row; stats: FLOAT32, contiguous, two elements per row, aligned
  * to 8 bytes; top_logprob (FLOAT32) and top_index (INT32): contiguous, k elements per row,
- * k <= PLAST_TOKEN_TOP_MAX and <= C. All but logprob may be NULL (top_* together). temperature is in
- * [1e-30, 1e30].
+ * k <= PLAST_TOKEN_TOP_MAX and <= C. All but logprob may be NULL (top_* together). No output shares
+ * an element with another tensor of the call. temperature is in [1e-30, 1e30].
  * A token outside [0, C) marks a row of padding: logprob 0 and no gradient through it (as
  * cross_entropy treats such a label); its entropy and the rest are computed. A logit of -inf is a
  * masked token: probability 0. A row without any other logit has log_norm and every log probability

@@ -950,6 +950,11 @@ void plast_b200_token_logprob(const Tensor *logits, const Tensor *tokens, Tensor
       return;
   }
   if (s.rows == 0) return; // nothing to do
+  // rows are read while others are written
+  const Extent all[8] = {extent_of(logits), extent_of(tokens), extent_of(logprob), extent_of(entropy), extent_of(log_norm), extent_of(stats),
+                         extent_of(top ? top_logprob : nullptr), extent_of(top ? top_index : nullptr)};
+  for (int i = 2; i < 8; ++i)
+    if (!check_apart("token_logprob", "an output", all[i], Extent{}, all, i)) return;
 
   LpParams p = {};
   p.x = (const float *)logits->data;
@@ -1020,8 +1025,11 @@ void plast_b200_token_logprob_backward(Tensor *logits, const Tensor *tokens, con
   if (g[1] && !check_row_output(entropy, s.rows, FLOAT32, "token_logprob: entropy")) return;
   if (s.rows == 0 || (!g[0] && !g[1] && !g[2])) return; // nothing to do
 
-  LpGradParams p = {};
   const Tensor *dx = logits->grad;
+  const Extent others[6] = {extent_of(tokens), extent_of(stats), extent_of(g[0] ? logprob->grad : nullptr), extent_of(g[1] ? entropy->grad : nullptr),
+                            extent_of(g[1] ? entropy : nullptr), extent_of(g[2] ? log_norm->grad : nullptr)};
+  if (!check_apart("token_logprob", "the gradient of the logits", extent_of(dx), extent_of(logits), others, 6)) return;
+  LpGradParams p = {};
   p.x = (const float *)logits->data;
   p.token = (const int *)tokens->data;
   p.dx = (float *)dx->data;

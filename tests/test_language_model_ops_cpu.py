@@ -335,3 +335,33 @@ def test_outputs_and_gradients_with_an_element_at_two_indices():
     logits, tok, st, lp = T(6, 40), T(6, dtype=I), T(6, 2), T(6, requires_grad=True)
     logits.set_grad(base.view((6, 40), (39, 1)))
     refused("UNSUPPORTED", pb.token_logprob_backward, logits, tok, st, lp)
+
+
+def test_token_logprob_refuses_buffers_that_overlap():
+    base = T(400)
+    x, tok = base.view((4, 10), (10, 1)), base.view((4,), (1,), offset=40)
+    tok.c.dtype = I
+
+    def at(offset, *shape, dtype=F):
+        t = base.view(shape, pb.contiguous_strides(shape), offset=offset)
+        t.c.dtype = dtype
+        return t
+
+    f = pb.token_logprob
+    refused("UNSUPPORTED", f, x, tok, at(39, 4))                                    # the last logit
+    refused("UNSUPPORTED", f, x, tok, at(40, 4))                                    # the tokens
+    refused("UNSUPPORTED", f, x, tok, at(50, 4), entropy=at(53, 4))
+    refused("UNSUPPORTED", f, x, tok, at(50, 4), log_norm=at(50, 4))
+    refused("UNSUPPORTED", f, x, tok, at(50, 4), stats=at(36, 4, 2))
+    refused("UNSUPPORTED", f, x, tok, at(50, 4), top_logprob=at(60, 4, 3), top_index=at(71, 4, 3, dtype=I))
+    refused("UNSUPPORTED", f, x, tok, at(50, 4), top_logprob=at(60, 4, 3), top_index=at(42, 4, 3, dtype=I))
+    b = pb.token_logprob_backward
+    lp, ent, norm = at(50, 4), at(54, 4), at(58, 4)
+    stats = T(4, 2)
+    for t, offset in ((lp, 100), (ent, 104), (norm, 108)):
+        t.set_grad(at(offset, 4))
+    for offset in (5, 37, 57, 61, 99, 103, 105, 111):
+        x.set_grad(at(offset, 4, 10))
+        if offset != 57:       # over the values of entropy, which are read
+            refused("UNSUPPORTED", b, x, tok, stats, lp, ent if offset in (61, 103, 105) else None, norm)
+        refused("UNSUPPORTED", b, x, tok, stats, lp, ent, norm)
