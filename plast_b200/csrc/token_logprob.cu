@@ -877,29 +877,34 @@ static bool check_stats(const Tensor *t, u64 rows) {
   return true;
 }
 
-// Whether the kernel for many rows serves. Against the other one, measured in us with 0 / 1 / 16 / 32
-// alternatives (or, with fewer rows than resident CTAs, 0 / 5 / 20):
+// Whether the kernel for many rows serves. Against the other one, measured in us with 0 / 1 / 16 / 32 alternatives:
 //   rows for every resident CTA, four to an SM: where a row's stream covers the end of the row before
 //     2048 rows of 32768: 48 / 54 / 56 / 77  (49 / 61 / 80 / 93)
 //     4096 rows of 16384: 46 / 58 / 67 / 106 (52 / 74 / 97 / 112)
 //     4096 rows of 8192:  27 / 47 / 56 / 93  (32 / 53 / 65 / 77)
 //     4096 rows of 4096:  19 / 41 / 49 / 85  (23 / 42 / 47 / 57)
 //     4096 rows of 2048:  21 / 42 / 49 / 83  (12 / 21 / 26 / 36)
-//   more rows than the other one has resident CTAs, two to an SM:
-//     450 rows of 60000:  21 / 27 / 28 (25 / 37 / 50)
-//     300 rows of 200000: 57 / 65 / 67 (54 / 66 / 80)
-//     590 rows of 4096:   5.6 / 7.9 / 9.6 (4.7 / 8.3 / 10.6)
-//   fewer rows: for the alternatives' sake, up to the length where a row is better shared by a cluster
-//     200 rows of 16384:  5.5 / 9.1 / 10.5 (5.4 / 10.4 / 15.1)
-//     75 rows of 60000:   9.9 / 14.8 / 16.1 (9.0 / 15.4 / 20.7)
-//     140 rows of 200000: 43 / 52 / 55 (22 / 30 / 41)
-//   few rows, with 20 alternatives: 24 rows of 24000: 10.4 (13.0), of 60000: 15.2 (15.0)
+// Fewer rows, measured in captured graphs over inputs larger than L2, as the other one's time over this one's with
+// 1 / 9 / 16 / 17 / 20 / 24 / 32 alternatives (0 / 1 / 16 / 20 / 32 from 300 rows on):
+//   more rows than the other one has resident CTAs, two to an SM: always
+//     590 rows of 8192: 1.40 / 1.52 / 1.51 / 1.83 / 1.31, of 65536 (60000 up to 16): 1.15 / 1.23 / 1.61 / 1.51 / 1.39
+//     300 rows of 8192: 1.23 / 1.31 / 1.20 / 1.30 / 0.94, of 65536 (60000 up to 16): 1.13 / 1.16 / 1.36 / 1.42 / 1.20
+//   more than one to an SM: for 9 to 24 alternatives, whose selection a CTA of the other one does after its stream
+//     200 rows of 8192:   -   / 1.00 / 1.06 / 1.38 / 1.29 / 1.02 / 0.88
+//     200 rows of 32768: 0.91 / 1.07 / 1.10 / 1.27 / 1.23 / 1.09 / 0.97
+//     200 rows of 65536: 0.81 / 0.98 / 1.02 / 1.20 / 1.17 /  -   /  -
+//   up to one to an SM, where the other one shares a row among up to eight CTAs: for 17 to 22 alternatives (two of each of
+//   its sixteen warps' lanes have to be in its bound) and rows that are not long
+//     148 rows of 8192:   -   / 0.83 / 0.98 / 1.30 / 1.21 / 0.96 / 0.81, of 32768: 0.82 / 0.90 / 0.96 / 1.14 / 1.08 / 1.01 / 0.86
+//     24 rows of 8192:    -   / 0.86 / 0.92 / 1.12 / 1.02 / 0.83 / 0.70, of 32768:  -   / 0.60 / 0.71 / 0.95 / 0.92 / 0.82 / 0.76
+//     1 row of 8192 / 16384 / 40960 with 17: 0.91 / 0.97 / 0.92, with 32: 0.56 / 0.67 / 0.72
 static bool rows_kernel_serves(u64 rows, u64 cols, u64 top) {
   const u64 sms = (u64)sm_count();
   if (rows >= sms * kLpRowCtas) return cols >= (top == 0 ? 4096 : top <= 16 ? 8192 : 16384);
-  if (rows > sms * 2) return cols >= 8192;
-  if (top > 16 && cols >= 8192 && cols <= 40960) return true;
-  return top > 0 && rows >= sms / 2 && cols >= 16384 && cols <= 65536;
+  if (cols < 8192) return false;
+  if (rows > sms * 2) return true;
+  if (rows > sms) return top >= 9 && top <= 24 && cols <= 65536;
+  return top >= 17 && top <= 22 && rows >= 8 && cols <= (rows >= sms / 2 ? 32768 : 24576);
 }
 
 static unsigned lp_threads(u64 cols, unsigned most) { // one trip of the CTA covers threads * 16 logits

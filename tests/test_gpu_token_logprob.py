@@ -414,3 +414,19 @@ def test_on_both_sides_of_the_rule(rows, cols, top):
     rs = np.random.RandomState(rows + cols)
     x, token = rs.randn(rows, cols).astype(np.float32), rs.randint(0, cols, rows)
     check(run(x, token, 1.0, top), x, token, 1.0, top)
+
+
+@pytest.mark.parametrize("rows, cols, top, by_rows", [
+    (1, 8192, 17, False), (1, 40960, 32, False), (24, 24000, 32, False), (148, 16384, 16, False), (148, 16384, 23, False),
+    (7, 16384, 20, False), (8, 24576, 17, True), (8, 24577, 17, False), (148, 32768, 22, True), (148, 32769, 22, False),
+    (149, 8192, 9, True), (149, 8192, 8, False), (200, 65536, 24, True), (200, 65537, 24, False), (296, 8192, 25, False),
+    (297, 8192, 32, True), (297, 8191, 32, False)])
+def test_few_rows_go_where_they_are_measured_to_be_faster(rows, cols, top, by_rows):
+    """The borders of the rule on a GPU of 148 SMs; the results on both sides."""
+    torch = pytest.importorskip("torch")
+    rs = np.random.RandomState(rows + cols)
+    x, token = rs.randn(rows, cols).astype(np.float32), rs.randint(0, cols, rows)
+    t = run(x, token, 1.0, top)
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert pb.last_kernel() == ("token_logprob_rows_top" if by_rows else "token_logprob_top")
+    check(t, x, token, 1.0, top)
