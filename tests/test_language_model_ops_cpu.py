@@ -365,3 +365,22 @@ def test_token_logprob_refuses_buffers_that_overlap():
         if offset != 57:       # over the values of entropy, which are read
             refused("UNSUPPORTED", b, x, tok, stats, lp, ent if offset in (61, 103, 105) else None, norm)
         refused("UNSUPPORTED", b, x, tok, stats, lp, ent, norm)
+
+
+@pytest.mark.parametrize("rotated,base,factor,slow,fast,context", [(128, 10000.0, 16.0, 1, 32, 4096), (64, 500000.0, 4.0, 1, 32, 8192),
+                                                                   (96, 10000.0, 8.0, 2, 20, 2048)])
+def test_the_ramp_of_the_parts_table(rotated, base, factor, slow, fast, context):
+    """Between the pair that makes `fast` turns over the context and the one that makes `slow`, both rounded outwards to
+    whole pairs, the share of the divided frequency grows linearly with the pair's index."""
+    i = np.arange(rotated // 2)
+    plain = base ** (-2.0 * i / rotated)
+
+    def pair(turns):
+        return rotated * np.log(context / (2 * np.pi * turns)) / (2 * np.log(base))
+
+    low, high = np.floor(pair(fast)), np.ceil(pair(slow))
+    assert 2 < low and high < rotated // 2 - 2          # the ramp lies inside
+    share = np.clip((i - low) / (high - low), 0, 1)
+    table, _ = pb.rotary_frequencies(rotated, base, "parts", factor=factor, slow=slow, fast=fast, context=context)
+    np.testing.assert_allclose(table, plain / factor * share + plain * (1 - share), rtol=2.0 ** -23)
+    assert ((share > 0) & (share < 1)).sum() > 5
