@@ -1,4 +1,4 @@
-// Matrix products with fp32 accuracy on the tensor cores: panels of split fp16 operands, and the
+// Matrix products of 22-bit operands with fp32 sums on the tensor cores: panels of split fp16 operands, and the
 // device-side pieces (barriers, bulk copies, tcgen05) that a kernel over them is made of.
 //
 // An fp32 value v, scaled by 2^14, is kept as two fp16 numbers, hi = fp16(v) and lo = fp16(v - hi):

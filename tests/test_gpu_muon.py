@@ -464,3 +464,106 @@ def test_a_product_may_take_longer_than_the_limit_of_a_wait():
         pb.lib.plast_b200_tune(13, -1)
     assert not O.muon_status()
     assert torch.isfinite(out).all()
+
+
+# ---- accuracy ------------------------------------------------------------------------------------------
+# What a panel cannot hold: 2^-39 of a value below 2^-14. The elements of X are stored after every step and carried on by
+# the following ones, which multiply them by at most a = 3.4445 where X is small: 1 + a + ... + a^5 = 685.
+FLOOR, CARRIED = 2.0 ** -39, sum(3.4445 ** s for s in range(6))
+
+
+@pytest.mark.parametrize("scale", [1e-25, 1e-18, 1e-15, 1e-13])
+def test_far_below_epsilon_an_absolute_error_is_left(scale):
+    """X begins with |x| / epsilon, so the steps are linear to first order: X <- a X. Per step an element carries twice
+    2^-22 of it for its storage, and 8 * 2^-22 for the diagonal of the moved polynomial (2.3 and 0.7 * 1.93 and 2.03 *
+    0.49 with 2^-22 each, rounded up); off the diagonal the polynomial's 2^-39 times the sum of a column, below one more
+    2^-39."""
+    base = np.random.RandomState(31).randn(60, 90).astype(np.float32)
+    x = base * np.float32(scale)
+    want = R.orthogonalise(x)
+    bound = 2 * CARRIED * FLOOR + 5 * 12 * 2.0 ** -22 * np.abs(want)
+    got = orth([x])[0]
+    assert (np.abs(got - want) <= bound).all(), np.max(np.abs(got - want) / bound)
+    assert np.abs(want).max() < 2 * CARRIED * FLOOR or got.any()
+
+
+def fp32_steps(x, steps=5):
+    """The same steps with products of fp32 operands and fp32 sums, on the GPU (torch, no TF32)."""
+    torch = pytest.importorskip("torch")
+    assert not torch.backends.cuda.matmul.allow_tf32
+    a, b, c = R.COEFFICIENTS
+    y = torch.from_numpy(x).cuda()
+    y = y.t() if x.shape[0] > x.shape[1] else y
+    y = (y / torch.linalg.norm(y.double()).float())
+    for _ in range(steps):
+        g = y @ y.t()
+        y = a * y + (b * g + c * (g @ g)) @ y
+    y = y.t() if x.shape[0] > x.shape[1] else y
+    return y.cpu().numpy()
+
+
+def exact_steps(x, steps=5):
+    """R.orthogonalise on the GPU."""
+    torch = pytest.importorskip("torch")
+    a, b, c = (float(np.float32(v)) for v in R.COEFFICIENTS)
+    y = torch.from_numpy(x).cuda().double()
+    y = y.t() if x.shape[0] > x.shape[1] else y
+    y = y / (torch.linalg.norm(y) + float(np.float32(1e-7)))
+    for _ in range(steps):
+        g = y @ y.t()
+        y = a * y + (b * g + c * (g @ g)) @ y
+    y = y.t() if x.shape[0] > x.shape[1] else y
+    return y.cpu().numpy()
+
+
+@pytest.mark.parametrize("shape", [(512, 2048), (2048, 300), (700, 700)])
+@pytest.mark.parametrize("small", [1.0, 1e-3, 1e-5, 1e-6, 1e-8])
+def test_rows_of_two_sizes(shape, small):
+    """Row by row (of the shorter side), relative to the row: as the same steps in fp32, and the 2^-39 of a row's n
+    elements, of its m elements of the polynomial (times |X| <= 1.21) and of X X^T (times 1.93 + 2 * 2.03 * 0.75 <= 5
+    in the polynomial: 7.3 sqrt(m) together), carried on by the following steps."""
+    rs = np.random.RandomState(32)
+    x = rs.randn(*shape)
+    tall = shape[0] > shape[1]
+    rows = x.T if tall else x                       # a view
+    rows[::2] *= small
+    x = x.astype(np.float32)
+    got, want, plain = (v.T if tall else v for v in (orth([x])[0].astype(np.float64), exact_steps(x), fp32_steps(x).astype(np.float64)))
+    m, n = want.shape
+    size = np.linalg.norm(want, axis=1)
+    error, fp32 = (np.linalg.norm(v - want, axis=1) / size for v in (got, plain))
+    bound = 4 * max(fp32.max(), 2.0 ** -22) + CARRIED * FLOOR * (np.sqrt(n) + 7.3 * np.sqrt(m)) / size
+    assert (error <= bound).all(), (error.max(), np.max(error / bound))
+
+
+@pytest.mark.parametrize("shapes", [[(1024, 1024)] * 4 + [(1024, 4096)], [(2048, 3000)], [(4096, 2048)], [(1500, 3100), (1600, 900)]])
+def test_large_matrices_are_as_exact_as_products_in_fp32(shapes):
+    """Sizes at which the built-in choice takes pairs of CTAs: twice the error of the same steps in fp32, and the 22 bits
+    of the operands."""
+    rs = np.random.RandomState(33)
+    xs = [rs.randn(*s).astype(np.float32) for s in shapes]
+    for x, got in zip(xs, orth(xs)):
+        want = exact_steps(x)
+        assert rel(got, want) <= 2 * rel(fp32_steps(x), want) + 2.0 ** -21
+
+
+@pytest.mark.parametrize("kind", ["identity", "permutation", "blocks", "wide"])
+def test_sums_that_truncate_nothing(kind):
+    """One or two terms to a sum, so that nothing is truncated when it is added up, while the drained sums are raised by one
+    or three units of 2^-23 (the average truncation of full sums). The singular values are all alike and go one way x ->
+    f(x); every product adds at most 6 * 2^-23 of its terms (three units, an operand's 2^-23 each, lo lo), in units of x:
+    the gram matrix through 1.93 + 2 * 2.03 |s|, s = x^2 - 0.7; the polynomial 2.03 s^2 + 1.93 |s| + 3; apply 2.3 + 1.15 + |q|.
+    f' carries it on."""
+    rs, n = np.random.RandomState(34), 256
+    x = {"identity": np.eye(n), "permutation": np.eye(n)[rs.permutation(n)] * np.where(rs.rand(n) < 0.5, 1, -1)[:, None],
+         "blocks": np.kron(np.eye(n // 2), np.array([[1.0, 1.0], [1.0, -1.0]])), "wide": np.eye(n, 4 * n, 37)}[kind].astype(np.float32)
+    got, want = orth([x])[0], R.orthogonalise(x)
+    a, b, c = R.COEFFICIENTS
+    v, off = 1.0 / np.sqrt(n), 2.0 ** -22 / np.sqrt(n)
+    for _ in range(5):
+        s, eta = v * v - 0.7, 6 * 2.0 ** -23
+        poly = b * v * v + c * v ** 4
+        off = abs(a + 3 * b * v * v + 5 * c * v ** 4) * off + eta * v * (v * v * (1.93 + 4.06 * abs(s)) + 2.03 * s * s + 1.93 * abs(s) + 3
+                                                                   + 3.45 + abs(poly + 2.3))
+        v = v * (a + poly)
+    assert rel(got, want) <= off / abs(v), (rel(got, want), off / abs(v))
