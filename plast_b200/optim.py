@@ -83,6 +83,9 @@ def _address_array(params):
 
 def step(optimizer, params) -> None:
     """One optimiser step on the GPU over a list of parameters (Tensor objects with .grad)."""
+    moments = getattr(optimizer, "_moments", None)
+    if moments is not None and optimizer.m and len(moments) < len(params):
+        raise ValueError(f"{len(params)} parameters, but {len(moments)} momenta were given")
     _STEP[type(optimizer)](C.byref(optimizer), _address_array(params), len(params))
     check_error()
 

@@ -116,3 +116,13 @@ def test_addresses_are_a_list_of_pointers(count):
     packed = pb._addresses(ts)
     at = pb.C.cast(pb.C.c_char_p(packed), TENSORS)
     assert len(packed) == 8 * count and [at[i].contents.shape[0] for i in range(count)] == [i + 1 for i in range(count)]
+
+
+@pytest.mark.parametrize("count", [0, 1])
+def test_a_momentum_for_every_parameter(count):
+    """The library reads a momentum per parameter from the caller's array."""
+    from plast_b200 import optim
+    params = [pb.Tensor((4, 4), device="cpu", requires_grad=True) for _ in range(2)]
+    opt = optim.Muon.create(moments=[pb.Tensor((4, 4), device="cpu") for _ in range(count)])
+    with pytest.raises(ValueError):
+        optim.step(opt, params)
