@@ -567,3 +567,13 @@ def test_sums_that_truncate_nothing(kind):
                                                                    + 3.45 + abs(poly + 2.3))
         v = v * (a + poly)
     assert rel(got, want) <= off / abs(v), (rel(got, want), off / abs(v))
+
+
+@pytest.mark.parametrize("steps", [0, 1, 5])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+def test_one_infinity_or_nan_makes_its_matrix_nan(steps, value):
+    x = np.random.RandomState(35).randn(70, 50).astype(np.float32)
+    bad = x.copy()
+    bad[40, 20] = value
+    got = orth([bad, x], steps)
+    assert np.isnan(got[0]).all() and np.isfinite(got[1]).all()
