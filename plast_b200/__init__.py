@@ -377,16 +377,19 @@ class Tensor:
             return flat[:1].reshape(())
         return np.lib.stride_tricks.as_strided(flat, shape=shape, strides=[s * 4 for s in strides]).copy()
 
-    def free(self):
+    def _free_memory(self):
         if self._dptr is not None:
             lib.arena_free_cuda(self._dptr)
             self._dptr = None
+
+    def free(self):
+        self._free_memory()
         if self.grad is not None and self._owns_grad:
             self.grad.free()
 
     def __del__(self):
         try:
-            self.free()
+            self._free_memory()         # the gradient's goes with the last that holds it
         except Exception:
             pass
 

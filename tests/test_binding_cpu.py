@@ -108,6 +108,13 @@ def test_a_gradient_that_was_set_stays_its_owners(monkeypatch):
     assert freed == [12, 13, 14] and grad._dptr == 11
     del grad
     assert freed == [12, 13, 14, 11]
+    t, other = pb.Tensor((3,), device="cpu"), pb.Tensor((3,), device="cpu")
+    other.set_grad(t.attach_grad())
+    t.grad._dptr = 15
+    del t                                                # the other one holds it
+    assert freed[4:] == []
+    del other
+    assert freed[4:] == [15]
 
 
 @pytest.mark.parametrize("count", [0, 1, 3, 8, 9, 40])
