@@ -736,6 +736,7 @@ void plast_b200_qk_norm_rotary_backward(Tensor *q, Tensor *k, Tensor *q_weight, 
   int sides = 0;
   bool wants_weight[2] = {};
   WeightGradParams wg = {};
+  Extent in[2] = {}, dout[2] = {}; // of the sides that are computed
   for (int i = 0; i < 2; ++i) {
     if (!xs[i]) continue;
     const bool need_x = xs[i]->requires_grad, need_w = ws[i] && ws[i]->requires_grad;
@@ -745,6 +746,8 @@ void plast_b200_qk_norm_rotary_backward(Tensor *q, Tensor *k, Tensor *q_weight, 
         !check_same_heads(name, xs[i], outs[i]->grad, "gradient of the output"))
       return;
     if (need_w && !check_grad(ws[i], "qk_norm_rotary: weight")) return;
+    in[i] = extent_of(xs[i]);
+    dout[i] = extent_of(outs[i]->grad);
     if (need_w && peer_bracket_open())
       return set_error(PLAST_B200_ERR_UNSUPPORTED, "%s: weight gradients are not combined inside a peer bracket", name);
     HeadSide &sd = p.side[sides];
@@ -771,7 +774,6 @@ void plast_b200_qk_norm_rotary_backward(Tensor *q, Tensor *k, Tensor *q_weight, 
   // Both sides run at once: the gradient of an input lies over the gradient of its output at most, that of a weight (added
   // afterwards) over the other weight's at most.
   auto written = [](const Tensor *t) { return extent_of(t && t->requires_grad ? t->grad : nullptr); };
-  const Extent in[2] = {extent_of(q), extent_of(k)}, dout[2] = {extent_of(q_out ? q_out->grad : nullptr), extent_of(k_out ? k_out->grad : nullptr)};
   for (int i = 0; i < (k ? 2 : 1); ++i) {
     const Extent others[8] = {in[0], in[1], dout[1 - i], written(xs[1 - i]), extent_of(q_weight), extent_of(k_weight), extent_of(positions), extent_of(inv_freq)};
     if (!check_apart(name, i ? "the gradient of k" : "the gradient of q", written(xs[i]), dout[i], others, 8)) return;

@@ -332,3 +332,16 @@ def test_heads_of_one_fused_row():
     x.set_grad(y.grad)
     pb.backward("rotary", [x, t["pos"], t["freq"]], y, fval=1.0)
     assert np.array_equal(x.grad.numpy(), want)
+
+
+def test_a_side_without_gradients_is_not_looked_at():
+    """Keys that want no gradient: what their output's gradient lies over is of no matter."""
+    v = qk_case(np.random.RandomState(13), (2, 5, 4, 64), (2, 5, 4, 64), 32)
+    t = qk_run(v, 0, 1e-6)
+    want = t["q"].grad.numpy()
+    q, k, ko = pb.Tensor.from_numpy(v["q"], requires_grad=True), pb.Tensor.from_numpy(v["k"]), pb.Tensor(v["k"].shape)
+    q.grad.copy_from(v["start_q"])
+    ko.set_grad(q.grad)
+    qw, kw = pb.Tensor.from_numpy(v["qw"]), pb.Tensor.from_numpy(v["kw"])
+    pb.qk_norm_rotary_backward(q, k, qw, kw, t["pos"], t["freq"], t["qo"], ko)
+    assert np.array_equal(q.grad.numpy(), want)
