@@ -110,7 +110,7 @@ typedef struct {
  *   data = data (1 - lr weight_decay) - lr s orthogonalised(u)
  * optimizer->m holds one momentum per parameter, contiguous and of its size; where it is NULL the
  * first step creates zeros for the list (freed by plast_b200_muon_state_release, like Adam's), so a
- * first step is not captured into a graph. No parameter or momentum may overlap another buffer of the
+ * first step cannot be captured into a graph and is refused there. No parameter or momentum may overlap another buffer of the
  * call. A call that is refused changes nothing. */
 void muon_step_cuda(Muon *optimizer, Tensor **parameters, int num_parameters);
 void plast_b200_muon_state_release(Tensor **m);

@@ -1290,6 +1290,15 @@ struct MuonState {
 static std::mutex g_muon_mutex;
 static std::unordered_map<Tensor **, MuonState> g_muon_states; // keyed by the m array
 
+// A call that needs the host's view of the device cannot be part of a graph; refused before it spoils the capture.
+static bool check_not_captured(const char *what) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (!check_cuda(cudaStreamIsCapturing(stream(), &status))) return false;
+  if (status == cudaStreamCaptureStatusNone) return true;
+  set_error(PLAST_B200_ERR_UNSUPPORTED, "muon: %s cannot be captured into a graph", what);
+  return false;
+}
+
 // m[i] = zeros like parameters[i], for every parameter that a step updates
 static Tensor **create_momenta(Tensor **parameters, int n) {
   Tensor **m = (Tensor **)calloc(n > 0 ? n : 1, sizeof(Tensor *));
@@ -1378,6 +1387,7 @@ static void muon_step(Muon *opt, Tensor **parameters, int num_parameters) {
     if (it != g_muon_states.end() && num_parameters > it->second.n)
       return set_error(PLAST_B200_ERR_SHAPE, "muon: %d parameters, but the momenta were created for %d", num_parameters, it->second.n);
   } else if (!mats.empty()) {
+    if (!check_not_captured("a first step, which creates the momenta,")) return;
     opt->m = create_momenta(parameters, num_parameters);
     if (!opt->m) return;
     made = true;
@@ -1457,6 +1467,7 @@ int plast_b200_muon_status(void) {
   static std::unordered_map<int, unsigned> told; // per device: what an earlier look has seen
   int device = 0;
   unsigned now = 0;
+  if (!check_not_captured("a look at the status")) return -1;
   PB_CUDA_RET(cudaGetDevice(&device), -1);
   PB_CUDA_RET(cudaMemcpyFromSymbolAsync(&now, g_ns_gave_up, sizeof now, 0, cudaMemcpyDeviceToHost, stream()), -1);
   PB_CUDA_RET(cudaStreamSynchronize(stream()), -1);

@@ -577,3 +577,33 @@ def test_one_infinity_or_nan_makes_its_matrix_nan(steps, value):
     bad[40, 20] = value
     got = orth([bad, x], steps)
     assert np.isnan(got[0]).all() and np.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("mode", ["global", "thread_local", "relaxed"])
+def test_a_first_step_and_the_status_are_refused_in_a_capture(mode):
+    """Neither spoils the capture: what else it holds replays, and the momenta's zero-fill is not part of it."""
+    torch = pytest.importorskip("torch")
+    rs = np.random.RandomState(36)
+    x, out = pb.Tensor.from_numpy(rs.randn(50, 60).astype(np.float32)), pb.Tensor((50, 60))
+    want = orth([x.numpy()])[0]
+    p = pb.Tensor.from_numpy(rs.randn(50, 60).astype(np.float32), requires_grad=True)
+    opt, stream, codes = O.Muon.create(), torch.cuda.Stream(), []
+    pb.synchronize()
+    pb.lib.plast_b200_set_stream(C.c_void_p(stream.cuda_stream))
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode=mode):
+            for call in (lambda: O.step(opt, [p]), O.muon_status):
+                try:
+                    call()
+                except pb.PlastError as e:
+                    codes.append(pb.ERROR_NAMES[e.code])
+            O.orthogonalise([x], [out])
+        assert codes == ["UNSUPPORTED"] * 2 and not opt.m
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(out.numpy(), want)
+    finally:
+        pb.lib.plast_b200_set_stream(None)
