@@ -11,8 +11,8 @@
 //
 // What bounds it, on a B200: large matrices the way of the operands from L2 to the SMs (a pair of CTAs brings
 // 128 KB for every 1,536 cycles of products on its 256 x 256 tile; it takes 1,900) and the power cap: one
-// 4096 x 8192 in 6.45 ms, 1.12 PFLOP/s of fp16 products. Matrices of 1024: 16 square and 8 of 4096 x 1024 in
-// 3.48 ms, 0.78 PFLOP/s, as every 16 K blocks a tile is stored. Small ones the chain of 3 products a step: 8 us
+// 4096 x 8192 in 6.6 ms, 1.10 PFLOP/s of fp16 products. Matrices of 1024: 16 square and 8 of 4096 x 1024 in
+// 3.57 ms, 0.76 PFLOP/s, as every 16 K blocks a tile is stored. Small ones the chain of 3 products a step: 8 us
 // each where a tile has a CTA of its own (six matrices of up to 512: 130 us).
 #include "plast_b200_optim.h"
 #include "row_map.cuh"

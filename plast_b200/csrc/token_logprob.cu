@@ -45,6 +45,9 @@ struct LpParams {
   double inv_temperature;
 };
 
+// 2^t by the special function unit, up to 2^-22 off relative to itself: one instruction per logit in loops that have to keep
+// up with HBM. A row's results stay within 1e-7 of 64 bits (4.7e-8 to 9.6e-8 for 1 to 8192 rows of 32768 to 131072, the
+// same formulas in elementary fp32 steps 6.5e-8 to 1.7e-7).
 __device__ __forceinline__ float ex2(float t) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
@@ -449,8 +452,8 @@ __global__ void __launch_bounds__(kLpMaxThreads, 2) token_logprob_kernel(const _
 // A persistent CTA whose eight warps stream one row after the other while a ninth finishes the row before.
 // The end of a row is a chain of short steps (joining statistics, alternatives, logarithms) of 3 us, with
 // alternatives 6 to 7 beside the stream; in the streaming warps it leaves HBM idle for as long. Measured: 8192
-// rows of 65536 in 313 us without alternatives (6.9 TB/s) and 343 with sixteen, 2048 rows of 32768 in 49 and 56
-// (the last row's end among them). With short rows the finishing warp is the bound, hence the rule at the launch.
+// rows of 65536 in 318 to 330 us without alternatives (6.5 to 6.8 TB/s) and 360 with sixteen, 2048 rows of 32768 in
+// 48 and 57 (the last row's end among them). With short rows the finishing warp is the bound, hence the rule at the launch.
 //
 // The stream notes the largest logit of every thread and piece (one or more trips). A lane of the finishing
 // warp looks after eight threads; the k-th largest of the lanes' largest notes (above 16: of the largest
